@@ -18,7 +18,8 @@ LIB_PATH = os.path.join(_HERE, "libhgcalml_b200.so")
 HGC_OK = 0
 NOT_TAKEN = 1  # of the host binding: the arguments want the tensor operations
 STATUS_BITS = {1: "bin index out of range", 2: "flat bin index overflow",
-               4: "gathered index out of range", 8: "iteration cap reached"}
+               4: "gathered index out of range", 8: "iteration cap reached",
+               16: "row splits that do not ascend from 0 to the number of rows"}
 
 
 class HgcError(RuntimeError):
@@ -72,6 +73,13 @@ def _load():
         "hgc_select_knn_grad": (I, [P] * 5 + [I] * 3 + [P, S, P]),
         "hgc_select_knn_grad_ordered": (I, [P] * 5 + [I] * 3 + [P, P, S, P]),
         "hgc_select_knn_grad_after": (I, [P] * 5 + [I] * 3 + [P, P, S, P]),
+        "hgc_cross_attention_workspace_bytes": (S, [I] * 7),
+        "hgc_cross_attention": (I, [P] * 8 + [I] * 6 + [P, ctypes.c_float, I, P, S, P]),
+        "hgc_cross_attention_grad_workspace_bytes": (S, [I] * 7),
+        "hgc_cross_attention_grad": (I, [P] * 12 + [I] * 6 + [P, ctypes.c_float, I, P, S, P]),
+        "hgc_norm_rotate": (I, [P, I, I, I, I, I, I, ctypes.c_double, ctypes.c_float, I, P]),
+        "hgc_norm_rotate_grad_workspace_bytes": (S, [P, I, I]),
+        "hgc_norm_rotate_grad": (I, [P, I, I, I, I, I, I, ctypes.c_double, ctypes.c_float, I, P, S, P]),
         "hgc_binned_assign_to_condensates_workspace_bytes": (S, [I] * 4),
         "hgc_binned_assign_to_condensates": (I, [I, I] + [P] * 4 + [P] + [P] * 2 + [P] * 4 + [P] * 4 + [P] * 3
                                              + [P, I, I, I, I] + [P, S, P]),

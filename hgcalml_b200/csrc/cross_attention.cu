@@ -1,0 +1,695 @@
+// Attention between two ragged sets of rows of the same events, forward and backward: products in float32 on the CUDA cores,
+// for every type, width and stride, and the C entries.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - m_i) / l_i,  s_ij = scale q_i.k_j over the keys j of i's event that can be seen
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i.v_j - delta_i),  delta_i = do_i.o_i,  dq_i = scale sum_j ds_ij k_j,
+//   dk_j = scale sum_i ds_ij q_i
+//
+// A row without keys has o = 0, and -inf for the logarithm of its sum.  Gradients of shared key heads are summed inside the
+// kernel and parts of a split are joined in their order: no atomics, so results do not change from run to run.
+#include "cross_attention.cuh"
+
+namespace hgc {
+namespace attn {
+namespace {
+
+constexpr int kRows = 64;        // rows and columns of a tile
+constexpr int kThreads = 256;    // 16 x 16; a thread has rows ty + 16 i and columns tx + 16 j
+constexpr int kPitchP = kRows + 4;
+
+// Rows of `dp` floats, 4 more apart: 16-byte reads of 8 consecutive rows meet no bank twice, and one row is read by 16 threads
+// at once.
+template <int DP> constexpr int kPitch = DP + 4;
+
+// acc[i][j] += a[ty + 16 i] . b[tx + 16 j]
+template <int DP, int TM>
+__device__ __forceinline__ void dots(float (&acc)[TM][4], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
+{
+    constexpr int P = kPitch<DP>;
+#pragma unroll 2
+    for (int d = 0; d < DP; d += 4) {
+        float4 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = *reinterpret_cast<const float4 *>(b + (tx + 16 * j) * P + d);
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const float4 x = *reinterpret_cast<const float4 *>(a + (ty + 16 * i) * P + d);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                acc[i][j] = fmaf(x.x, y[j].x, acc[i][j]);
+                acc[i][j] = fmaf(x.y, y[j].y, acc[i][j]);
+                acc[i][j] = fmaf(x.z, y[j].z, acc[i][j]);
+                acc[i][j] = fmaf(x.w, y[j].w, acc[i][j]);
+            }
+        }
+    }
+}
+
+// acc[i][c] += sum_k a[ty + 16 i][k] b[k][column c of tx]; columns tx * V + 16 V g + v
+template <int DP> constexpr int kVec = DP / 16 < 4 ? DP / 16 : 4;
+template <int DP, int TM>
+__device__ __forceinline__ void weighted_rows(float (&acc)[TM][DP / 16], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
+{
+    constexpr int P = kPitch<DP>, V = kVec<DP>, C = DP / 16;
+#pragma unroll 2
+    for (int k = 0; k < kRows; k += 4) {
+        float y[4][C];
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+            for (int c = 0; c < C; c += V) {
+                const float *from = b + (k + kk) * P + tx * V + c * 16;
+                if constexpr (V == 4) {
+                    const float4 q = *reinterpret_cast<const float4 *>(from);
+                    y[kk][c] = q.x; y[kk][c + 1] = q.y; y[kk][c + 2] = q.z; y[kk][c + 3] = q.w;
+                } else {
+                    const float2 q = *reinterpret_cast<const float2 *>(from);
+                    y[kk][c] = q.x; y[kk][c + 1] = q.y;
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const float4 x = *reinterpret_cast<const float4 *>(a + (ty + 16 * i) * kPitchP + k);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                acc[i][c] = fmaf(x.x, y[0][c], acc[i][c]);
+                acc[i][c] = fmaf(x.y, y[1][c], acc[i][c]);
+                acc[i][c] = fmaf(x.z, y[2][c], acc[i][c]);
+                acc[i][c] = fmaf(x.w, y[3][c], acc[i][c]);
+            }
+        }
+    }
+}
+template <int DP> __device__ __forceinline__ int column(int tx, int c)
+{
+    constexpr int V = kVec<DP>;
+    return tx * V + c / V * (16 * V) + c % V;
+}
+
+// Rows [begin, begin + n) of one head as floats; what is not there, and the keys that cannot be seen, are zeros, whatever the
+// memory holds: a weight of zero would not make up for an infinity.
+template <typename T, int DP>
+__device__ __forceinline__ void load_keys(float *__restrict__ dst, const Strided &s, int head, int begin, int n, int dim,
+                                          const unsigned char *__restrict__ mask)
+{
+    const T *__restrict__ p = static_cast<const T *>(s.p) + head * s.head;
+    for (int i = threadIdx.x; i < kRows * DP; i += kThreads) {
+        const int r = i / DP, d = i % DP;
+        const bool in = r < n && d < dim && (mask == nullptr || __ldg(mask + begin + r) != 0);
+        dst[r * kPitch<DP> + d] = in ? to_float(p[(long long)(begin + r) * s.row + d]) : 0.f;
+    }
+}
+// Rows of a tile of queries: row r is head r % pack of token r / pack.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void load_queries(float *__restrict__ dst, const Strided &s, int head0, int begin, int n, int pack, int dim)
+{
+    const T *__restrict__ p = static_cast<const T *>(s.p);
+    for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
+        const int r = i / DP, d = i % DP;
+        dst[r * kPitch<DP> + d] = r < n && d < dim
+            ? to_float(p[(long long)(begin + r / pack) * s.row + (long long)(head0 + r % pack) * s.head + d]) : 0.f;
+    }
+}
+
+// The block's tile, found by the first warp; blocks of one call that have nothing to do leave here.
+__device__ __forceinline__ Tile block_tile(const int *rs, int n, int n_events, int rows)
+{
+    __shared__ Tile s_tile;
+    if (threadIdx.x < 32) {
+        const Tile t = find_tile(rs, n, n_events, rows, blockIdx.x);
+        if (threadIdx.x == 0) s_tile = t;
+    }
+    __syncthreads();
+    return s_tile;
+}
+
+// keys of an event; none behind the last one
+__device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int event)
+{
+    if (event >= n_events) return make_int2(0, 0);
+    return make_int2(split_at(rs, event, n), split_at(rs, event + 1, n));
+}
+
+// ------------------------------------------------------------------------------------------------------------- forward
+// A block takes a tile of queries (with the heads that share a key head) through the keys of its event, 64 at a time, with the
+// running maximum and sum of every row.
+template <typename T, int DP, int TM>
+__global__ void __launch_bounds__(kThreads)
+forward_kernel(const __grid_constant__ Args a)
+{
+    pdl_begin();
+    constexpr int M = 16 * TM, P = kPitch<DP>, C = DP / 16;
+    extern __shared__ __align__(16) float s_mem[];
+    float *s_q = s_mem, *s_k = s_q + M * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P;
+    __shared__ unsigned char s_seen[kRows];
+    const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
+    const int tokens = M / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_splits(a, t, kThreads);
+    const Tile tile = block_tile(a.rs_q, a.n_q, a.n_events, tokens);
+    if (tile.begin >= tile.end) return;
+    const int n_rows = (tile.end - tile.begin) * a.pack;
+    const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
+    const int2 part = part_of(max(0, (keys.y - keys.x + kRows - 1) / kRows), blockIdx.z, a.splits);
+    load_queries<T, DP, M>(s_q, a.q, head0, tile.begin, n_rows, a.pack, a.dim);
+    const float c = a.scale * kLog2e;
+    float o[TM][C], m[TM], l[TM];
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < C; j++) o[i][j] = 0.f;
+    }
+    for (int step = part.x; step < part.y; step++) {
+        const int k0 = keys.x + step * kRows, n = min(kRows, keys.y - k0);
+        __syncthreads();
+        load_keys<T, DP>(s_k, a.k, kv, k0, n, a.dim, a.mask);
+        load_keys<T, DP>(s_v, a.v, kv, k0, n, a.dim, a.mask);
+        if (t < kRows) s_seen[t] = t < n && (a.mask == nullptr || a.mask[k0 + t] != 0);
+        __syncthreads();
+        float s[TM][4] = {};
+        dots<DP, TM>(s, s_q, s_k, ty, tx);
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (!s_seen[tx + 16 * j]) s[i][j] = -INFINITY;
+                top = fmaxf(top, s[i][j]);
+            }
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float next = fmaxf(m[i], top), base = next == -INFINITY ? 0.f : next;
+            const float shrink = exp2f((m[i] - base) * c);
+            m[i] = next;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float p = exp2f((s[i][j] - base) * c);
+                sum += p;
+                s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = p;
+            }
+            l[i] = l[i] * shrink + sum;  // of this thread's columns
+#pragma unroll
+            for (int j = 0; j < C; j++) o[i][j] *= shrink;
+        }
+        __syncthreads();
+        weighted_rows<DP, TM>(o, s_p, s_v, ty, tx);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        float sum = l[i];
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        const int r = ty + 16 * i;
+        if (r >= n_rows) continue;
+        const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float lse = sum == 0.f ? -INFINITY : m[i] * a.scale + logf(sum);
+        float *lse_to = a.splits > 1 ? a.part_lse + (long long)blockIdx.z * a.n_q * a.heads : a.lse;
+        if (tx == 0) lse_to[row] = lse;
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+            const int d = column<DP>(tx, j);
+            if (d >= a.dim) continue;
+            if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = o[i][j] * inv;
+            else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(o[i][j] * inv);
+        }
+    }
+}
+
+// Joins the parts of a row: every part holds its own softmax and the logarithm of its sum.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_forward_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, T *__restrict__ out, float *__restrict__ lse,
+                    long long n_rows, int dim, int splits)
+{
+    pdl_begin();
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= n_rows) return;
+    float top = -INFINITY;
+    for (int s = 0; s < splits; s++) top = fmaxf(top, part_lse[s * n_rows + row]);
+    float sum = 0.f;
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int s = 0; s < splits; s++) sum += exp2f((part_lse[s * n_rows + row] - base) * kLog2e);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int d = lane_id(); d < dim; d += 32) {
+        float o = 0.f;
+        for (int s = 0; s < splits; s++) {
+            const float w = exp2f((part_lse[s * n_rows + row] - base) * kLog2e);
+            if (w != 0.f) o = fmaf(w, part[(s * n_rows + row) * dim + d], o);
+        }
+        out[row * dim + d] = from_float<T>(o * inv);
+    }
+    if (lane_id() == 0) lse[row] = sum == 0.f ? -INFINITY : top + logf(sum);
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+// What both gradients go by.  The first `n_count` blocks: the keys of an event that can be seen, counted up to two; with one key
+// the weights do not depend on the scores, so the gradients of q and k are zero and not what is left of two sums that cancel.
+// The others: delta = sum of out * grad, a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+prepare_backward_kernel(const __grid_constant__ Args a, float *__restrict__ delta, int *__restrict__ visible, int n_count)
+{
+    pdl_begin();
+    const int t = threadIdx.x;
+    if ((int)blockIdx.x < n_count) {
+        const int e = blockIdx.x;
+        if (e == 0) check_splits(a, t, kThreads);
+        if (e >= a.n_events) return;
+        const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, e);
+        int n = a.mask == nullptr ? max(0, keys.y - keys.x) : 0;
+        for (int base = keys.x; a.mask != nullptr && base < keys.y && n < 2; base += kThreads)
+            n += __syncthreads_count(base + t < keys.y && a.mask[base + t] != 0);
+        if (t == 0) visible[e] = min(n, 2);
+        return;
+    }
+    const long long row = (long long)(blockIdx.x - n_count) * (kThreads / 32) + (t >> 5);
+    if (row >= (long long)a.n_q * a.heads) return;
+    const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ grad = static_cast<const T *>(a.grad);
+    float sum = 0.f;
+    for (int d = lane_id(); d < a.dim; d += 32) sum = fmaf(to_float(out[row * a.dim + d]), to_float(grad[row * a.dim + d]), sum);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    if (lane_id() == 0) delta[row] = sum;
+}
+
+// dq of a tile of queries: the keys of the event pass by once more.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads)
+grad_queries_kernel(const __grid_constant__ Args a)
+{
+    pdl_begin();
+    constexpr int P = kPitch<DP>, C = DP / 16;
+    extern __shared__ __align__(16) float s_mem[];
+    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P;
+    __shared__ unsigned char s_seen[kRows];
+    const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
+    const int tokens = kRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
+    const Tile tile = block_tile(a.rs_q, a.n_q, a.n_events, tokens);
+    if (tile.begin >= tile.end) return;
+    const int n_rows = (tile.end - tile.begin) * a.pack;
+    int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
+    if (tile.event < a.n_events && a.visible[tile.event] < 2) keys.y = keys.x;
+    const int2 part = part_of(max(0, (keys.y - keys.x + kRows - 1) / kRows), blockIdx.z, a.splits);
+    const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
+    load_queries<T, DP, kRows>(s_q, a.q, head0, tile.begin, n_rows, a.pack, a.dim);
+    load_queries<T, DP, kRows>(s_g, grad, head0, tile.begin, n_rows, a.pack, a.dim);
+    const float c = a.scale * kLog2e;
+    float dq[4][C] = {}, lse[4], delta[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = ty + 16 * i;
+        const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
+        lse[i] = r < n_rows ? a.lse[row] * kLog2e : INFINITY;
+        delta[i] = r < n_rows ? a.delta[row] : 0.f;
+    }
+    for (int step = part.x; step < part.y; step++) {
+        const int k0 = keys.x + step * kRows, n = min(kRows, keys.y - k0);
+        __syncthreads();
+        load_keys<T, DP>(s_k, a.k, kv, k0, n, a.dim, a.mask);
+        load_keys<T, DP>(s_v, a.v, kv, k0, n, a.dim, a.mask);
+        if (t < kRows) s_seen[t] = t < n && (a.mask == nullptr || a.mask[k0 + t] != 0);
+        __syncthreads();
+        float s[4][4] = {}, dp[4][4] = {};
+        dots<DP, 4>(s, s_q, s_k, ty, tx);
+        dots<DP, 4>(dp, s_g, s_v, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool seen = s_seen[tx + 16 * j] && ty + 16 * i < n_rows;
+                const float p = seen ? exp2f(fmaf(s[i][j], c, -lse[i])) : 0.f;
+                s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
+            }
+        __syncthreads();
+        weighted_rows<DP, 4>(dq, s_p, s_k, ty, tx);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = ty + 16 * i;
+        if (r >= n_rows) continue;
+        const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+            const int d = column<DP>(tx, j);
+            if (d >= a.dim) continue;
+            const float v = dq[i][j] * a.scale;
+            if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = v;
+            else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(v);
+        }
+    }
+}
+
+// dk and dv of a tile of keys: the queries of the event pass by, with all heads that share the key head.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads)
+grad_keys_kernel(const __grid_constant__ Args a)
+{
+    pdl_begin();
+    constexpr int P = kPitch<DP>, C = DP / 16;
+    extern __shared__ __align__(16) float s_mem[];
+    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P,
+          *s_d = s_p + kRows * kPitchP;
+    __shared__ float s_lse[kRows], s_delta[kRows];
+    const int t = threadIdx.x, ty = t >> 4, tx = t & 15, kv = blockIdx.y;
+    const Tile tile = block_tile(a.rs_k, a.n_k, a.n_events, kRows);
+    if (tile.begin >= tile.end) return;
+    const int n_keys = tile.end - tile.begin, tokens = kRows / a.pack;
+    const int2 queries = rows_of(a.rs_q, a.n_q, a.n_events, tile.event);
+    const int blocks = max(0, (queries.y - queries.x + tokens - 1) / tokens), packs = a.group / a.pack;
+    const int2 part = part_of(blocks, blockIdx.z, a.splits);
+    const bool varies = tile.event < a.n_events && a.visible[tile.event] > 1;
+    const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
+    load_keys<T, DP>(s_k, a.k, kv, tile.begin, n_keys, a.dim, a.mask);
+    load_keys<T, DP>(s_v, a.v, kv, tile.begin, n_keys, a.dim, a.mask);
+    const float c = a.scale * kLog2e;
+    float dk[4][C] = {}, dv[4][C] = {};
+    bool seen[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = ty + 16 * i;
+        seen[i] = r < n_keys && (a.mask == nullptr || a.mask[tile.begin + r] != 0);
+    }
+    for (int step = part.x * packs; step < part.y * packs; step++) {
+        const int q0 = queries.x + step / packs * tokens, head0 = kv * a.group + step % packs * a.pack;
+        const int n = min(tokens, queries.y - q0) * a.pack;
+        __syncthreads();
+        load_queries<T, DP, kRows>(s_q, a.q, head0, q0, n, a.pack, a.dim);
+        load_queries<T, DP, kRows>(s_g, grad, head0, q0, n, a.pack, a.dim);
+        if (t < kRows) {
+            const long long row = (long long)(q0 + t / a.pack) * a.heads + head0 + t % a.pack;
+            s_lse[t] = t < n ? a.lse[row] * kLog2e : INFINITY;
+            s_delta[t] = t < n ? a.delta[row] : 0.f;
+        }
+        __syncthreads();
+        float s[4][4] = {}, dp[4][4] = {};
+        dots<DP, 4>(s, s_k, s_q, ty, tx);
+        dots<DP, 4>(dp, s_v, s_g, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool in = seen[i] && tx + 16 * j < n;
+                const float p = in ? exp2f(fmaf(s[i][j], c, -s_lse[tx + 16 * j])) : 0.f;
+                s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = p;
+                s_d[(ty + 16 * i) * kPitchP + tx + 16 * j] = in && varies ? p * (dp[i][j] - s_delta[tx + 16 * j]) : 0.f;
+            }
+        __syncthreads();
+        weighted_rows<DP, 4>(dv, s_p, s_g, ty, tx);
+        weighted_rows<DP, 4>(dk, s_d, s_q, ty, tx);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = ty + 16 * i;
+        if (r >= n_keys) continue;
+        const long long row = (long long)(tile.begin + r) * a.kv_heads + kv;
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+            const int d = column<DP>(tx, j);
+            if (d >= a.dim) continue;
+            if (a.splits > 1) {
+                const long long at = ((long long)blockIdx.z * a.n_k * a.kv_heads + row) * a.dim + d;
+                a.part[at] = dk[i][j] * a.scale;
+                a.part2[at] = dv[i][j];
+            } else {
+                static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(dk[i][j] * a.scale);
+                static_cast<T *>(a.to2)[row * a.dim + d] = from_float<T>(dv[i][j]);
+            }
+        }
+    }
+}
+
+// Sums the parts of one or two gradients, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_gradient_kernel(const float *__restrict__ part, const float *__restrict__ part2, T *__restrict__ to, T *__restrict__ to2,
+                     long long n, int splits)
+{
+    pdl_begin();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float a = 0.f, b = 0.f;
+    for (int s = 0; s < splits; s++) {
+        a += part[s * n + i];
+        if (part2 != nullptr) b += part2[s * n + i];
+    }
+    to[i] = from_float<T>(a);
+    if (part2 != nullptr) to2[i] = from_float<T>(b);
+}
+
+// -------------------------------------------------------------------------------------------------------------- host
+template <typename K>
+int launch(K kernel, dim3 grid, size_t smem, cudaStream_t stream, const Args &a)
+{
+    HGC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    HGC_CUDA_TRY(launch_pdl(kernel, grid, kThreads, smem, stream, a));
+    HGC_LAUNCH_CHECK();
+    return HGC_OK;
+}
+
+// How many parts the long axis is split into: as many as it takes to give every multiprocessor `per_sm` blocks, but parts of at
+// least `least` steps of a mean event.  Depends on sizes alone, so that the workspace can be asked for.
+int split_count(long long blocks, long long mean_steps, int per_sm, int least)
+{
+    const long long want = (long long)per_sm * sm_count() / (blocks > 0 ? blocks : 1);
+    long long s = mean_steps / least;
+    if (s > want) s = want;
+    return s < 1 ? 1 : s > 128 ? 128 : (int)s;
+}
+
+// What a call of these sizes needs; the kernels and the workspace queries go by the same numbers.
+struct Plan {
+    int group, pack, splits, splits_q, splits_k;
+    long long tiles_q, tiles_q64, tiles_k;
+};
+
+constexpr int kForwardTM = 4;
+
+bool sizes_ok(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
+{
+    return n_q >= 0 && n_k >= 0 && n_rs >= 1 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && dim >= 1;
+}
+bool sizes_supported(int heads, int dim) { return heads <= 65535 && dim <= kMaxDim; }
+
+Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads)
+{
+    Plan p;
+    const int events = n_rs - 1;
+    p.group = heads / kv_heads;
+    p.pack = p.group <= kMaxPack ? p.group : 1;
+    const int tokens = kRows / p.pack, m = 16 * kForwardTM / p.pack;
+    p.tiles_q = tile_count(n_q, m, events);
+    p.tiles_q64 = tile_count(n_q, tokens, events);
+    p.tiles_k = tile_count(n_k, kRows, events);
+    const int some = events > 0 ? events : 1;
+    // tiles that have rows, if the events are alike
+    const auto filled = [&](int n, int rows) { return (long long)some * ((n / some + rows) / rows); };
+    const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
+    p.splits = split_count(filled(n_q, m) * (heads / p.pack), steps_k, 4, 4);
+    p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
+    p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);
+    return p;
+}
+
+struct ForwardBuffers {
+    float *part = nullptr, *part_lse = nullptr;
+};
+template <typename C> ForwardBuffers carve_forward(C &c, const Plan &p, int n_q, int heads, int dim)
+{
+    ForwardBuffers b;
+    if (p.splits > 1) {
+        const size_t rows = (size_t)p.splits * n_q * heads;
+        if constexpr (std::is_same_v<C, Carver>) {
+            b.part = c.template take<float>(rows * dim);
+            b.part_lse = c.template take<float>(rows);
+        } else {
+            c.template take<float>(rows * dim);
+            c.template take<float>(rows);
+        }
+    }
+    return b;
+}
+
+struct BackwardBuffers {
+    float *delta = nullptr, *part_q = nullptr, *part_k = nullptr, *part_v = nullptr;
+    int *visible = nullptr;
+};
+template <typename C> BackwardBuffers carve_backward(C &c, const Plan &p, int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
+{
+    BackwardBuffers b;
+    const size_t rows = (size_t)n_q * heads, parts_q = p.splits_q > 1 ? p.splits_q * rows * dim : 0,
+                 parts_k = p.splits_k > 1 ? (size_t)p.splits_k * n_k * kv_heads * dim : 0;
+    if constexpr (std::is_same_v<C, Carver>) {
+        b.delta = c.template take<float>(rows);
+        b.visible = c.template take<int>(n_rs);
+        b.part_q = c.template take<float>(parts_q);
+        b.part_k = c.template take<float>(parts_k);
+        b.part_v = c.template take<float>(parts_k);
+    } else {
+        c.template take<float>(rows);
+        c.template take<int>(n_rs);
+        c.template take<float>(parts_q);
+        c.template take<float>(parts_k);
+        c.template take<float>(parts_k);
+    }
+    return b;
+}
+
+template <typename T, int DP> int run_forward(const Args &a, const Plan &p, cudaStream_t stream)
+{
+    constexpr int M = 16 * kForwardTM;
+    const size_t smem = sizeof(float) * ((M + 2 * kRows) * kPitch<DP> + M * kPitchP);
+    if (const int rc = launch(forward_kernel<T, DP, kForwardTM>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a)) return rc;
+    if (a.splits > 1) {
+        const long long rows = (long long)a.n_q * a.heads;
+        HGC_CUDA_TRY(launch_pdl(join_forward_kernel<T>, div_up(rows, 8), 256, 0, stream, a.part, a.part_lse, static_cast<T *>(a.to), a.lse, rows,
+                                a.dim, a.splits));
+        HGC_LAUNCH_CHECK();
+    }
+    return HGC_OK;
+}
+
+template <typename T> int join_gradient(const Args &a, long long n, cudaStream_t stream)
+{
+    if (a.splits == 1 || n == 0) return HGC_OK;
+    HGC_CUDA_TRY(launch_pdl(join_gradient_kernel<T>, div_up(n, 256), 256, 0, stream, a.part, a.part2, static_cast<T *>(a.to), static_cast<T *>(a.to2), n,
+                            a.splits));
+    HGC_LAUNCH_CHECK();
+    return HGC_OK;
+}
+
+template <typename T, int DP> int run_backward(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void *dk, void *dv, cudaStream_t stream)
+{
+    const size_t smem_q = sizeof(float) * (4 * kRows * kPitch<DP> + kRows * kPitchP);
+    const size_t smem_k = smem_q + sizeof(float) * kRows * kPitchP;
+    if (dq != nullptr && a.n_q > 0) {
+        a.to = dq; a.to2 = nullptr; a.part = b.part_q; a.part2 = nullptr; a.splits = p.splits_q;
+        if (const int rc = launch(grad_queries_kernel<T, DP>, dim3((unsigned)p.tiles_q64, a.heads / a.pack, a.splits), smem_q, stream, a)) return rc;
+        if (const int rc = join_gradient<T>(a, (long long)a.n_q * a.heads * a.dim, stream)) return rc;
+    }
+    if (dk != nullptr && a.n_k > 0) {
+        a.to = dk; a.to2 = dv; a.part = b.part_k; a.part2 = b.part_v; a.splits = p.splits_k;
+        if (const int rc = launch(grad_keys_kernel<T, DP>, dim3((unsigned)p.tiles_k, a.kv_heads, a.splits), smem_k, stream, a)) return rc;
+        if (const int rc = join_gradient<T>(a, (long long)a.n_k * a.kv_heads * a.dim, stream)) return rc;
+    }
+    return HGC_OK;
+}
+
+template <typename T> int forward_of(const Args &a, const Plan &p, cudaStream_t stream)
+{
+    return a.dim <= 32 ? run_forward<T, 32>(a, p, stream) : a.dim <= 64 ? run_forward<T, 64>(a, p, stream) : run_forward<T, 128>(a, p, stream);
+}
+
+template <typename T>
+int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void *dk, void *dv, cudaStream_t stream)
+{
+    const long long rows = (long long)a.n_q * a.heads;
+    const int n_count = a.n_events > 0 ? a.n_events : 1;
+    HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + div_up(rows, kThreads / 32), kThreads, 0, stream, a, b.delta, b.visible, n_count));
+    HGC_LAUNCH_CHECK();
+    return a.dim <= 32 ? run_backward<T, 32>(a, p, b, dq, dk, dv, stream)
+         : a.dim <= 64 ? run_backward<T, 64>(a, p, b, dq, dk, dv, stream) : run_backward<T, 128>(a, p, b, dq, dk, dv, stream);
+}
+
+Args args_of(const void *q, const void *k, const void *v, const int *rs_q, const int *rs_k, const unsigned char *mask, float *lse, int n_q, int n_k,
+             int n_rs, int heads, int kv_heads, int dim, const long long *strides, float scale, const Plan &p, void *workspace)
+{
+    const long long dq = (long long)heads * dim, dk = (long long)kv_heads * dim;
+    Args a = {};
+    a.q = strides ? Strided{q, strides[0], strides[1]} : Strided{q, dq, dim};
+    a.k = strides ? Strided{k, strides[2], strides[3]} : Strided{k, dk, dim};
+    a.v = strides ? Strided{v, strides[4], strides[5]} : Strided{v, dk, dim};
+    a.rs_q = rs_q; a.rs_k = rs_k; a.mask = mask; a.lse = lse;
+    a.status = static_cast<unsigned *>(workspace);
+    a.n_q = n_q; a.n_k = n_k; a.n_events = n_rs - 1;
+    a.heads = heads; a.kv_heads = kv_heads; a.group = p.group; a.pack = p.pack; a.dim = dim; a.scale = scale;
+    return a;
+}
+
+bool scale_ok(float scale) { return scale > 0.f && scale <= 3.4e38f; }
+bool strides_ok(const long long *strides)
+{
+    if (strides)
+        for (int i = 0; i < 6; i++)
+            if (strides[i] < 0) return false;
+    return true;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace hgc
+
+using namespace hgc;
+using namespace hgc::attn;
+
+extern "C" size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype)
+{
+    (void)dtype;
+    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_heads, dim)) return 0;
+    Sizer s;
+    carve_forward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads), n_q, n_heads, dim);
+    return s.used;
+}
+
+extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void *d_v, const int *d_q_row_splits, const int *d_k_row_splits,
+                                   const unsigned char *d_key_mask, void *d_out, float *d_lse, int n_q, int n_k, int n_rs, int n_heads,
+                                   int n_kv_heads, int dim, const long long *strides, float scale, int dtype, void *workspace,
+                                   size_t workspace_bytes, hgc_stream_t stream_)
+{
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !scale_ok(scale) || !strides_ok(strides) || dtype < 0 || dtype > HGC_BFLOAT16)
+        return HGC_ERR_INVALID_ARGUMENT;
+    if (!sizes_supported(n_heads, dim)) return HGC_ERR_UNSUPPORTED;
+    if (n_q == 0) return HGC_OK;
+    if (!d_q || !d_out || !d_lse || !d_q_row_splits || !d_k_row_splits || (n_k > 0 && (!d_k || !d_v))) return HGC_ERR_INVALID_ARGUMENT;
+    if (const int rc = check_workspace(workspace, workspace_bytes,
+                                       hgc_cross_attention_workspace_bytes(n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype)))
+        return rc;
+    const Plan p = plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads);
+    Args a = args_of(d_q, d_k, d_v, d_q_row_splits, d_k_row_splits, d_key_mask, d_lse, n_q, n_k, n_rs, n_heads, n_kv_heads, dim, strides, scale, p,
+                     workspace);
+    Carver carver(workspace);
+    const ForwardBuffers b = carve_forward(carver, p, n_q, n_heads, dim);
+    a.to = d_out; a.part = b.part; a.part_lse = b.part_lse; a.splits = p.splits;
+    return dtype == HGC_FLOAT32 ? forward_of<float>(a, p, stream)
+         : dtype == HGC_FLOAT16 ? forward_of<__half>(a, p, stream) : forward_of<__nv_bfloat16>(a, p, stream);
+}
+
+extern "C" size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype)
+{
+    (void)dtype;
+    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_heads, dim)) return 0;
+    Sizer s;
+    carve_backward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads), n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
+    return s.used;
+}
+
+extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q, const void *d_k, const void *d_v, const void *d_out,
+                                        const float *d_lse, const int *d_q_row_splits, const int *d_k_row_splits,
+                                        const unsigned char *d_key_mask, void *d_grad_q, void *d_grad_k, void *d_grad_v, int n_q, int n_k,
+                                        int n_rs, int n_heads, int n_kv_heads, int dim, const long long *strides, float scale, int dtype,
+                                        void *workspace, size_t workspace_bytes, hgc_stream_t stream_)
+{
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !scale_ok(scale) || !strides_ok(strides) || dtype < 0 || dtype > HGC_BFLOAT16)
+        return HGC_ERR_INVALID_ARGUMENT;
+    if (!sizes_supported(n_heads, dim)) return HGC_ERR_UNSUPPORTED;
+    if (n_q == 0 && n_k == 0) return HGC_OK;
+    if (!d_q_row_splits || !d_k_row_splits || (n_q > 0 && (!d_grad_out || !d_q || !d_out || !d_lse)) || (n_k > 0 && (!d_k || !d_v)) ||
+        !d_grad_k != !d_grad_v)
+        return HGC_ERR_INVALID_ARGUMENT;
+    if (const int rc = check_workspace(workspace, workspace_bytes,
+                                       hgc_cross_attention_grad_workspace_bytes(n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype)))
+        return rc;
+    const Plan p = plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads);
+    Args a = args_of(d_q, d_k, d_v, d_q_row_splits, d_k_row_splits, d_key_mask, const_cast<float *>(d_lse), n_q, n_k, n_rs, n_heads, n_kv_heads, dim,
+                     strides, scale, p, workspace);
+    Carver carver(workspace);
+    const BackwardBuffers b = carve_backward(carver, p, n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
+    a.grad = d_grad_out; a.out = d_out; a.delta = b.delta; a.visible = b.visible;
+    return dtype == HGC_FLOAT32 ? backward_of<float>(a, p, b, d_grad_q, d_grad_k, d_grad_v, stream)
+         : dtype == HGC_FLOAT16 ? backward_of<__half>(a, p, b, d_grad_q, d_grad_k, d_grad_v, stream)
+                                : backward_of<__nv_bfloat16>(a, p, b, d_grad_q, d_grad_k, d_grad_v, stream);
+}

@@ -1,0 +1,106 @@
+// What the kernels of the attention between two ragged sets of rows share: the arguments of a call, which rows a block works
+// on, and how the long axis is split.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace hgc {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxDim = 128;
+// Heads that share a key head are packed into the rows of a tile up to this many, so that keys and values are read once for all
+// of them; beyond it every head has its own tiles.
+constexpr int kMaxPack = 32;
+
+// One call.  Rows of q, k and v are `row` and heads `head` elements apart, columns lie next to each other; every other tensor
+// is dense.
+struct Strided {
+    const void *p;
+    long long row, head;
+};
+
+struct Args {
+    Strided q, k, v;
+    const int *rs_q, *rs_k;        // [n_events + 1]
+    const unsigned char *mask;     // [n_k], zero: no query sees the key; may be null
+    const void *grad, *out;        // of the backward pass
+    const float *delta;            // [n_q, heads], sum of out * grad
+    const int *visible;            // [n_events], keys that can be seen, counted up to two
+    float *lse;                    // [n_q, heads], natural logarithm of the sum of exp(scale * q.k)
+    void *to, *to2;                // result: out, dq, or dk and dv
+    float *part, *part2;           // the same of every part of a split, in float32
+    float *part_lse;               // [splits, n_q, heads]
+    const float *bounds;           // largest norms of the rows of grad and of v (half precision's backward pass)
+    unsigned *status;
+    int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits;
+    float scale;
+};
+
+__device__ __forceinline__ int split_at(const int *__restrict__ rs, int i, int n) { return min(max(__ldg(rs + i), 0), n); }
+
+// The tiles of a ragged batch: event e owns the tile numbers from rs[e] / rows + e on, which leaves room for its last, partly
+// filled tile whatever the lengths are, so that the host can size a grid (n / rows + n_events + 1) without reading the splits.
+// What follows the last event is one more event, which has rows but no counterpart.
+struct Tile {
+    int event, begin, end;  // rows [begin, end); none: begin >= end
+};
+
+inline __host__ __device__ long long tile_count(int n, int rows, int n_events) { return (long long)n / rows + n_events + 1; }
+
+// All 32 lanes of a warp call this; 32 events are looked at in a step.
+__device__ __forceinline__ Tile find_tile(const int *__restrict__ rs, int n, int n_events, int rows, int tile)
+{
+    int lo = 0, hi = n_events + 1;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5, at = lo + lane_id() * step;
+        const bool before = at < hi && split_at(rs, at, n) / rows + at <= tile;
+        const unsigned votes = __ballot_sync(0xffffffffu, before);
+        const int ahead = max(votes == 0xffffffffu ? 32 : __ffs(~votes) - 1, 1);
+        lo += (ahead - 1) * step;
+        hi = min(lo + step, hi);
+    }
+    const int first = split_at(rs, lo, n), last = lo < n_events ? split_at(rs, lo + 1, n) : n;
+    const long long begin = first + (long long)(tile - first / rows - lo) * rows;
+    Tile t;
+    t.event = lo;
+    t.begin = begin < 0 || begin > last ? last : (int)begin;
+    t.end = min(last, t.begin + rows);
+    return t;
+}
+
+// Steps [first, last) of part `s` of `n_parts` of a row of `steps`.
+__device__ __forceinline__ int2 part_of(int steps, int s, int n_parts)
+{
+    const int each = (steps + n_parts - 1) / n_parts;
+    return make_int2(min(s * each, steps), min((s + 1) * each, steps));
+}
+
+// Sets the status word: whether the splits ascend from zero to at most the number of rows.  Every access is clamped to the
+// tensors whatever they hold.  One block of a call's first kernel does it, all of its threads together.
+__device__ __forceinline__ void check_splits(const Args &a, int t, int threads)
+{
+    bool bad = false;
+    for (int i = t; i <= a.n_events; i += threads) {
+        const int q = __ldg(a.rs_q + i), k = __ldg(a.rs_k + i);
+        bad |= q > (i < a.n_events ? __ldg(a.rs_q + i + 1) : a.n_q) || k > (i < a.n_events ? __ldg(a.rs_k + i + 1) : a.n_k);
+        bad |= i == 0 && (q != 0 || k != 0);
+    }
+    const int any = __syncthreads_or(bad);
+    if (t == 0) *a.status = any ? HGC_STATUS_ROW_SPLITS : 0u;
+}
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+}  // namespace attn
+}  // namespace hgc

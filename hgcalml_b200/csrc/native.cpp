@@ -142,6 +142,144 @@ int collect(const Tensor &dist, const Tensor &indices, int first_slot, int k, co
                                scale, subtract_self, data<int>(order), stream_of(features));
 }
 
+int type_code(const Tensor &t)
+{
+    return t.scalar_type() == at::kFloat ? HGC_FLOAT32 : t.scalar_type() == at::kHalf ? HGC_FLOAT16 : HGC_BFLOAT16;
+}
+
+// Of tensors that have at most one row or head, torch gives any distance between them.
+long long distance(const Tensor &t, int dim, long long dense) { return t.size(dim) > 1 ? (long long)t.stride(dim) : dense; }
+void distances(const Tensor &t, long long *to)
+{
+    to[1] = distance(t, 1, t.size(2));
+    to[0] = distance(t, 0, to[1] * t.size(1));
+}
+
+bool fits(const Tensor &t) { return t.size(0) <= 0x7fffffff; }
+
+// (rows, logarithms of the sums, status)
+std::tuple<Tensor, Tensor, int> cross_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &rs_q, const Tensor &rs_k,
+                                                const MaybeTensor &mask, double scale)
+{
+    if (!fits(q) || !fits(k) || !fits(rs_q)) return {q, q, HGC_ERR_UNSUPPORTED};
+    const int n_q = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), n_k = (int)k.size(0), kv_heads = (int)k.size(1);
+    const int n_rs = (int)rs_q.size(0), type = type_code(q);
+    long long strides[6];
+    distances(q, strides);
+    distances(k, strides + 2);
+    distances(v, strides + 4);
+    Tensor out = like(q, q.sizes(), q.scalar_type()), lse = like(q, {n_q, heads}, at::kFloat);
+    Tensor ws = workspace(q, hgc_cross_attention_workspace_bytes(n_q, n_k, n_rs, heads, kv_heads, dim, type));
+    const int rc = hgc_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), data<int>(rs_q), data<int>(rs_k), data<unsigned char>(mask), out.data_ptr(),
+                                       data<float>(lse), n_q, n_k, n_rs, heads, kv_heads, dim, strides, (float)scale, type, ws.data_ptr(),
+                                       (size_t)ws.numel(), stream_of(q));
+    return {out, lse, rc};
+}
+
+// (gradients of q, k, v or None, status)
+std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, int> cross_attention_grad(const Tensor &grad, const Tensor &q, const Tensor &k, const Tensor &v,
+                                                                            const Tensor &out, const Tensor &lse, const Tensor &rs_q,
+                                                                            const Tensor &rs_k, const MaybeTensor &mask, double scale,
+                                                                            bool need_q, bool need_k)
+{
+    MaybeTensor dq, dk, dv;
+    if (!fits(q) || !fits(k) || !fits(rs_q)) return {dq, dk, dv, HGC_ERR_UNSUPPORTED};
+    const int n_q = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), n_k = (int)k.size(0), kv_heads = (int)k.size(1);
+    const int n_rs = (int)rs_q.size(0), type = type_code(q);
+    long long strides[6];
+    distances(q, strides);
+    distances(k, strides + 2);
+    distances(v, strides + 4);
+    if (need_q) dq = like(q, q.sizes(), q.scalar_type());
+    if (need_k) {
+        dk = like(k, k.sizes(), k.scalar_type());
+        dv = like(k, k.sizes(), k.scalar_type());
+    }
+    const auto at = [](const MaybeTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; };
+    Tensor ws = workspace(q, hgc_cross_attention_grad_workspace_bytes(n_q, n_k, n_rs, heads, kv_heads, dim, type));
+    const int rc = hgc_cross_attention_grad(grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), data<float>(lse), data<int>(rs_q),
+                                            data<int>(rs_k), data<unsigned char>(mask), at(dq), at(dk), at(dv), n_q, n_k, n_rs, heads, kv_heads,
+                                            dim, strides, (float)scale, type, ws.data_ptr(), (size_t)ws.numel(), stream_of(q));
+    return {dq, dk, dv, rc};
+}
+
+// One of the two sets of rows of a norm_rotate call.
+void describe(hgc_norm_rotate_rows &r, const Tensor &x, const MaybeTensor &weight, const MaybeTensor &positions)
+{
+    long long strides[2];
+    distances(x, strides);
+    r.d_x = x.data_ptr();
+    r.row_stride = strides[0];
+    r.head_stride = strides[1];
+    r.n = (int)x.size(0);
+    r.n_heads = (int)x.size(1);
+    if (weight.has_value()) {
+        r.d_weight = weight->data_ptr();
+        r.weight_type = type_code(*weight);
+    }
+    if (positions.has_value()) r.d_positions = positions->data_ptr();
+}
+int position_code(const MaybeTensor &a, const MaybeTensor &b)
+{
+    if (!a.has_value() && !b.has_value()) return HGC_POSITION_FLOAT32;
+    const at::ScalarType t = a.has_value() ? a->scalar_type() : b->scalar_type();
+    return t == at::kFloat ? HGC_POSITION_FLOAT32 : t == at::kInt ? HGC_POSITION_INT32 : HGC_POSITION_INT64;
+}
+
+// (queries, keys or None, status)
+std::tuple<Tensor, MaybeTensor, int> norm_rotate(const Tensor &q, const MaybeTensor &k, const MaybeTensor &wq, const MaybeTensor &wk, const MaybeTensor &pq,
+                                                 const MaybeTensor &pk, int rotary, int axes, bool interleaved, double base, double eps)
+{
+    if (!fits(q) || (k.has_value() && !fits(*k))) return {q, k, HGC_ERR_UNSUPPORTED};
+    hgc_norm_rotate_rows sets[2] = {};
+    Tensor yq = like(q, q.sizes(), q.scalar_type());
+    MaybeTensor yk;
+    describe(sets[0], q, wq, pq);
+    sets[0].d_y = yq.data_ptr();
+    if (k.has_value()) {
+        yk = like(q, k->sizes(), q.scalar_type());
+        describe(sets[1], *k, wk, pk);
+        sets[1].d_y = yk->data_ptr();
+    }
+    const int rc = hgc_norm_rotate(sets, k.has_value() ? 2 : 1, (int)q.size(2), rotary, axes, position_code(pq, pk), interleaved, base, (float)eps,
+                                   type_code(q), stream_of(q));
+    return {yq, yk, rc};
+}
+
+// (gradients of the first and second rows, of their weights, status); the second set may be missing
+std::tuple<Tensor, MaybeTensor, MaybeTensor, MaybeTensor, int> norm_rotate_grad(
+        const Tensor &grad1, const MaybeTensor &grad2, const Tensor &x1, const MaybeTensor &x2, const MaybeTensor &w1, const MaybeTensor &w2,
+        const MaybeTensor &p1, const MaybeTensor &p2, bool need_w1, bool need_w2, int rotary, int axes, bool interleaved, double base, double eps)
+{
+    const bool two = x2.has_value();
+    MaybeTensor d2, dw1, dw2;
+    if (!fits(x1) || (two && !fits(*x2))) return {x1, d2, dw1, dw2, HGC_ERR_UNSUPPORTED};
+    hgc_norm_rotate_rows sets[2] = {};
+    Tensor d1 = like(x1, x1.sizes(), x1.scalar_type());
+    describe(sets[0], x1, w1, p1);
+    sets[0].d_grad_y = grad1.data_ptr();
+    sets[0].d_grad_x = d1.data_ptr();
+    if (need_w1) {
+        dw1 = like(*w1, w1->sizes(), w1->scalar_type());
+        sets[0].d_grad_weight = dw1->data_ptr();
+    }
+    if (two) {
+        d2 = like(x1, x2->sizes(), x1.scalar_type());
+        describe(sets[1], *x2, w2, p2);
+        sets[1].d_grad_y = grad2->data_ptr();
+        sets[1].d_grad_x = d2->data_ptr();
+        if (need_w2) {
+            dw2 = like(*w2, w2->sizes(), w2->scalar_type());
+            sets[1].d_grad_weight = dw2->data_ptr();
+        }
+    }
+    const int n_sets = two ? 2 : 1, dim = (int)x1.size(2);
+    Tensor ws = workspace(x1, hgc_norm_rotate_grad_workspace_bytes(sets, n_sets, dim));
+    const int rc = hgc_norm_rotate_grad(sets, n_sets, dim, rotary, axes, position_code(p1, p2), interleaved, base, (float)eps, type_code(x1),
+                                        ws.data_ptr(), (size_t)ws.numel(), stream_of(x1));
+    return {d1, d2, dw1, dw2, rc};
+}
+
 Tensor host_int()  // page-locked, so that the copy that fills it needs no staging
 {
     return at::empty({1}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
@@ -298,6 +436,10 @@ PYBIND11_MODULE(_native, m)
     m.def("collect", &collect, unlocked);
     m.def("condensates", &condensates, unlocked);
     m.def("merge_noise", &merge_noise, unlocked);
+    m.def("cross_attention", &cross_attention, unlocked);
+    m.def("cross_attention_grad", &cross_attention_grad, unlocked);
+    m.def("norm_rotate", &norm_rotate, unlocked);
+    m.def("norm_rotate_grad", &norm_rotate_grad, unlocked);
     m.def("dense", &dense, unlocked);
     m.def("bias_act", &bias_act, unlocked);
     m.def("copy_columns", &copy_columns, unlocked);

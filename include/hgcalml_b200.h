@@ -45,6 +45,12 @@ extern "C" {
 #define HGC_STATUS_FLAT_BIN_OVERFLOW   2u  /* a flat bin index was >= the number of bins           */
 #define HGC_STATUS_INDEX_OUT_OF_RANGE  4u  /* a gathered index was >= its table size               */
 #define HGC_STATUS_ITERATION_CAP       8u  /* an iterative kernel stopped at its iteration cap     */
+#define HGC_STATUS_ROW_SPLITS         16u  /* row splits do not ascend from 0 to at most the rows  */
+
+/* Types of the tensors of the entries that take a `dtype`. */
+#define HGC_FLOAT32  0
+#define HGC_FLOAT16  1
+#define HGC_BFLOAT16 2
 
 typedef void *hgc_stream_t; /* cudaStream_t */
 
@@ -401,6 +407,78 @@ int hgc_push_knn_grad(
 int hgc_push_knn_grad_ordered(
         const float *d_grad, const float *d_weights, const float *d_feat, const int *d_idxs,
         float *d_feat_grad, float *d_w_grad, int n_vert, int n_neigh, int n_feat, const int *d_order, hgc_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention between two ragged sets of rows of the same events (hits and condensates, a few object queries and
+ * the hits they look at, two views of an event).  (No counterpart in the reference.)
+ *
+ * Event e has the queries d_q[d_q_row_splits[e] .. d_q_row_splits[e+1]) and the keys and values
+ * [d_k_row_splits[e] .. d_k_row_splits[e+1]); both splits have n_rs entries.  For every head h of the n_heads,
+ * with the key head h / (n_heads / n_kv_heads):
+ *   d_out[i,h,:] = sum_j p_ij d_v[j,:],  p_ij = exp(scale q_i.k_j) / sum_j' exp(scale q_i.k_j')
+ * over the keys j of i's event with d_key_mask[j] != 0 (d_key_mask may be NULL: all of them).  What stands in
+ * masked rows of d_k and d_v does not matter, infinities and NaN included.  A query without keys, and a row behind
+ * the last event, gets zeros.  d_lse[i,h] = log of the sum of exp(scale q_i.k_j), -infinity without keys.
+ * d_q [n_q, n_heads, dim], d_k and d_v [n_k, n_kv_heads, dim], of the type `dtype`, with the distances in elements
+ * of rows and heads in strides = {q row, q head, k row, k head, v row, v head} (host memory; NULL: dense); columns
+ * lie next to each other.  d_out, d_lse (float32) and everything the gradient takes and gives besides are dense.
+ * Sums, weights and gradients are held in float32; in 16 bits, weights are rounded once to the type of the values
+ * they meet.  scale > 0.  Limits: dim <= 128, n_heads <= 65535.
+ *
+ * The gradient: d_grad_out [n_q, n_heads, dim] is that of d_out; d_out and d_lse are the forward pass's, as are all
+ * other arguments.  d_grad_q may be NULL, and d_grad_k and d_grad_v both, where they are not wanted; gradients of
+ * masked keys, of rows behind the last event and of q and k in events with one key are zero.  Results do not change
+ * from run to run.
+ *
+ * Splits that do not ascend from 0 to at most the number of rows set HGC_STATUS_ROW_SPLITS; the results are then
+ * unspecified.  A wait inside a kernel that did not end in time sets HGC_STATUS_ITERATION_CAP.
+ * ------------------------------------------------------------------------------------- */
+size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype);
+int hgc_cross_attention(
+        const void *d_q, const void *d_k, const void *d_v, const int *d_q_row_splits, const int *d_k_row_splits,
+        const unsigned char *d_key_mask, void *d_out, float *d_lse,
+        int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, const long long *strides, float scale, int dtype,
+        void *workspace, size_t workspace_bytes, hgc_stream_t stream);
+size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype);
+int hgc_cross_attention_grad(
+        const void *d_grad_out, const void *d_q, const void *d_k, const void *d_v, const void *d_out, const float *d_lse,
+        const int *d_q_row_splits, const int *d_k_row_splits, const unsigned char *d_key_mask,
+        void *d_grad_q, void *d_grad_k, void *d_grad_v,
+        int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, const long long *strides, float scale, int dtype,
+        void *workspace, size_t workspace_bytes, hgc_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Norm of the heads of queries and keys and their rotation by positions, in one pass.  (No counterpart in the
+ * reference.)  One or two sets of rows in one launch, the queries and the keys of an attention:
+ *   n = x / sqrt(mean(x^2) + eps) * weight   over the dim columns of a head, then
+ * the leading rotary_dim columns, in n_axes equal parts, turn with the row's n_axes positions: the part of axis a
+ * has the pairs (i, i + pairs) -- or (2 i, 2 i + 1) with `interleaved` -- of its columns, pairs = rotary_dim /
+ * (2 n_axes), and pair i turns by position / base^(i / pairs).  Angles are reduced in double, so that far positions
+ * keep their digits; everything else is float32, rounded once.
+ * d_x [n, n_heads, dim] with the given distances in elements; d_weight [dim] of the type weight_type (HGC_FLOAT32 or
+ * the rows' type), NULL: ones; d_positions [n, n_axes] of the type position_type, NULL: no rotation; d_y dense.
+ * The gradient reads d_x, d_weight, d_positions and d_grad_y (dense) and writes d_grad_x (dense) and, where it is
+ * not NULL, d_grad_weight [dim] of the weight's type; positions get none.  Results do not change from run to run.
+ * 0 <= rotary_dim <= dim, a multiple of 2 n_axes; base > 1; eps >= 0.  Limit: dim <= 128.
+ * ------------------------------------------------------------------------------------- */
+#define HGC_POSITION_FLOAT32 0
+#define HGC_POSITION_INT32   1
+#define HGC_POSITION_INT64   2
+typedef struct {
+    const void *d_x, *d_weight, *d_positions;
+    void *d_y;
+    const void *d_grad_y;
+    void *d_grad_x, *d_grad_weight;
+    long long row_stride, head_stride;
+    int n, n_heads, weight_type;
+} hgc_norm_rotate_rows;
+int hgc_norm_rotate(
+        const hgc_norm_rotate_rows *sets, int n_sets, int dim, int rotary_dim, int n_axes, int position_type,
+        int interleaved, double base, float eps, int dtype, hgc_stream_t stream);
+size_t hgc_norm_rotate_grad_workspace_bytes(const hgc_norm_rotate_rows *sets, int n_sets, int dim);
+int hgc_norm_rotate_grad(
+        const hgc_norm_rotate_rows *sets, int n_sets, int dim, int rotary_dim, int n_axes, int position_type,
+        int interleaved, double base, float eps, int dtype, void *workspace, size_t workspace_bytes, hgc_stream_t stream);
 
 #ifdef __cplusplus
 }
