@@ -123,13 +123,6 @@ __device__ __forceinline__ Tile block_tile(const int *rs, int n, int n_events, i
     return s_tile;
 }
 
-// keys of an event; none behind the last one
-__device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int event)
-{
-    if (event >= n_events) return make_int2(0, 0);
-    return make_int2(split_at(rs, event, n), split_at(rs, event + 1, n));
-}
-
 // ------------------------------------------------------------------------------------------------------------- forward
 // A block takes a tile of queries (with the heads that share a key head) through the keys of its event, 64 at a time, with the
 // running maximum and sum of every row.
@@ -461,7 +454,7 @@ int split_count(long long blocks, long long mean_steps, int per_sm, int least)
 
 // What a call of these sizes needs; the kernels and the workspace queries go by the same numbers.
 struct Plan {
-    int group, pack, splits, splits_q, splits_k;
+    int group, pack, splits, splits_mma, splits_q, splits_k;
     long long tiles_q, tiles_q64, tiles_k;
 };
 
@@ -473,7 +466,7 @@ bool sizes_ok(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 }
 bool sizes_supported(int heads, int dim) { return heads <= 65535 && dim <= kMaxDim; }
 
-Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads)
+Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 {
     Plan p;
     const int events = n_rs - 1;
@@ -488,6 +481,8 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads)
     const auto filled = [&](int n, int rows) { return (long long)some * ((n / some + rows) / rows); };
     const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
     p.splits = split_count(filled(n_q, m) * (heads / p.pack), steps_k, 4, 4);
+    const int mma_tokens = kMmaRows / p.pack;
+    p.splits_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 4, 2);
     p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
     p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);
     return p;
@@ -499,8 +494,9 @@ struct ForwardBuffers {
 template <typename C> ForwardBuffers carve_forward(C &c, const Plan &p, int n_q, int heads, int dim)
 {
     ForwardBuffers b;
-    if (p.splits > 1) {
-        const size_t rows = (size_t)p.splits * n_q * heads;
+    const int splits = p.splits > p.splits_mma ? p.splits : p.splits_mma;
+    if (splits > 1) {
+        const size_t rows = (size_t)splits * n_q * heads;
         if constexpr (std::is_same_v<C, Carver>) {
             b.part = c.template take<float>(rows * dim);
             b.part_lse = c.template take<float>(rows);
@@ -541,14 +537,7 @@ template <typename T, int DP> int run_forward(const Args &a, const Plan &p, cuda
 {
     constexpr int M = 16 * kForwardTM;
     const size_t smem = sizeof(float) * ((M + 2 * kRows) * kPitch<DP> + M * kPitchP);
-    if (const int rc = launch(forward_kernel<T, DP, kForwardTM>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a)) return rc;
-    if (a.splits > 1) {
-        const long long rows = (long long)a.n_q * a.heads;
-        HGC_CUDA_TRY(launch_pdl(join_forward_kernel<T>, div_up(rows, 8), 256, 0, stream, a.part, a.part_lse, static_cast<T *>(a.to), a.lse, rows,
-                                a.dim, a.splits));
-        HGC_LAUNCH_CHECK();
-    }
-    return HGC_OK;
+    return launch(forward_kernel<T, DP, kForwardTM>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a);
 }
 
 template <typename T> int join_gradient(const Args &a, long long n, cudaStream_t stream)
@@ -577,9 +566,20 @@ template <typename T, int DP> int run_backward(Args a, const Plan &p, const Back
     return HGC_OK;
 }
 
-template <typename T> int forward_of(const Args &a, const Plan &p, cudaStream_t stream)
+template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStream_t stream)
 {
-    return a.dim <= 32 ? run_forward<T, 32>(a, p, stream) : a.dim <= 64 ? run_forward<T, 64>(a, p, stream) : run_forward<T, 128>(a, p, stream);
+    const bool mma = mma_takes(a, dtype);
+    a.splits = mma ? p.splits_mma : p.splits;
+    if (const int rc = mma ? mma_forward(a, dtype, stream)
+                     : a.dim <= 32 ? run_forward<T, 32>(a, p, stream)
+                     : a.dim <= 64 ? run_forward<T, 64>(a, p, stream) : run_forward<T, 128>(a, p, stream))
+        return rc;
+    if (a.splits == 1) return HGC_OK;
+    const long long rows = (long long)a.n_q * a.heads;
+    HGC_CUDA_TRY(launch_pdl(join_forward_kernel<T>, div_up(rows, 8), 256, 0, stream, a.part, a.part_lse, static_cast<T *>(a.to), a.lse, rows, a.dim,
+                            a.splits));
+    HGC_LAUNCH_CHECK();
+    return HGC_OK;
 }
 
 template <typename T>
@@ -629,7 +629,7 @@ extern "C" size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs
     (void)dtype;
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_heads, dim)) return 0;
     Sizer s;
-    carve_forward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads), n_q, n_heads, dim);
+    carve_forward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim), n_q, n_heads, dim);
     return s.used;
 }
 
@@ -647,14 +647,14 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
     if (const int rc = check_workspace(workspace, workspace_bytes,
                                        hgc_cross_attention_workspace_bytes(n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype)))
         return rc;
-    const Plan p = plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads);
+    const Plan p = plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
     Args a = args_of(d_q, d_k, d_v, d_q_row_splits, d_k_row_splits, d_key_mask, d_lse, n_q, n_k, n_rs, n_heads, n_kv_heads, dim, strides, scale, p,
                      workspace);
     Carver carver(workspace);
     const ForwardBuffers b = carve_forward(carver, p, n_q, n_heads, dim);
-    a.to = d_out; a.part = b.part; a.part_lse = b.part_lse; a.splits = p.splits;
-    return dtype == HGC_FLOAT32 ? forward_of<float>(a, p, stream)
-         : dtype == HGC_FLOAT16 ? forward_of<__half>(a, p, stream) : forward_of<__nv_bfloat16>(a, p, stream);
+    a.to = d_out; a.part = b.part; a.part_lse = b.part_lse;
+    return dtype == HGC_FLOAT32 ? forward_of<float>(a, p, dtype, stream)
+         : dtype == HGC_FLOAT16 ? forward_of<__half>(a, p, dtype, stream) : forward_of<__nv_bfloat16>(a, p, dtype, stream);
 }
 
 extern "C" size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype)
@@ -662,7 +662,7 @@ extern "C" size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int
     (void)dtype;
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_heads, dim)) return 0;
     Sizer s;
-    carve_backward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads), n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
+    carve_backward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim), n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
     return s.used;
 }
 
@@ -683,7 +683,7 @@ extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q,
     if (const int rc = check_workspace(workspace, workspace_bytes,
                                        hgc_cross_attention_grad_workspace_bytes(n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype)))
         return rc;
-    const Plan p = plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads);
+    const Plan p = plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
     Args a = args_of(d_q, d_k, d_v, d_q_row_splits, d_k_row_splits, d_key_mask, const_cast<float *>(d_lse), n_q, n_k, n_rs, n_heads, n_kv_heads, dim,
                      strides, scale, p, workspace);
     Carver carver(workspace);

@@ -102,5 +102,18 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// keys of an event; none behind the last one
+__device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int event)
+{
+    if (event >= n_events) return make_int2(0, 0);
+    return make_int2(split_at(rs, event, n), split_at(rs, event + 1, n));
+}
+
+// The kernels on the tensor cores (cross_attention_mma.cu): 16-bit types, heads of whole 16-byte vectors, aligned rows.
+bool mma_takes(const Args &a, int dtype);
+constexpr int kMmaRows = 128;
+inline __host__ __device__ int mma_keys(int dim) { return dim <= 64 ? 128 : 64; }  // keys of a step of the forward pass
+int mma_forward(const Args &a, int dtype, cudaStream_t stream);
+
 }  // namespace attn
 }  // namespace hgc

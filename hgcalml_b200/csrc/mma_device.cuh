@@ -1,0 +1,196 @@
+// Tensor-core building blocks for kernels whose accumulators live in tensor memory: barriers, tile copies, matrix products.
+//
+// Tiles in shared memory are rows of 128 bytes, swizzled in groups of eight rows as the copy engine writes them (1024-byte
+// aligned); wider rows are several such tiles behind each other.  The same tile serves a product that sums along its rows (K-major)
+// and one that sums over them (MN-major).
+#pragma once
+
+#include "common.cuh"
+
+namespace hgc {
+namespace mma {
+
+__device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+// ----------------------------------------------------------------------------------------------------------- barriers
+__device__ __forceinline__ void barrier_init(unsigned bar, unsigned count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_init_done()
+{
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void arrive(unsigned bar)
+{
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_expect(unsigned bar, unsigned bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+
+// Waits end: after kPatience, or when another wait of the block has given up, the block's flag is set, every later wait returns
+// and no more copies or products are issued, so that the block runs to its end and frees its tensor memory.
+constexpr unsigned long long kPatience = 4000000000ull;  // ns
+__device__ __forceinline__ unsigned long long now()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity)
+{
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
+{
+    if (try_wait(bar, parity)) return true;
+    const unsigned long long begin = now();
+    do {
+        for (int i = 0; i < 16; i++)
+            if (try_wait(bar, parity)) return true;
+        if (*gave_up) return false;
+    } while (now() - begin < kPatience);
+    *gave_up = 1;
+    flag_status(status, HGC_STATUS_ITERATION_CAP);
+    return false;
+}
+// the same for a warp, whose lanes go on together
+__device__ __forceinline__ bool wait_warp(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
+{
+    return __all_sync(0xffffffffu, wait(bar, parity, gave_up, status));
+}
+// A wait for what is under way whatever happened before.
+__device__ __forceinline__ void drain(unsigned bar, unsigned parity)
+{
+    const unsigned long long begin = now();
+    while (!try_wait(bar, parity) && now() - begin < kPatience) {}
+}
+
+// -------------------------------------------------------------------------------------------------------- tile copies
+// A box of a three-dimensional tensor (columns, heads, rows) to shared memory; what lies outside the tensor is filled with zeros.
+__device__ __forceinline__ void copy_box(unsigned dst, const void *map, unsigned bar, int column, int head, int row)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(column), "r"(head), "r"(row) : "memory");
+}
+// Ordinary writes to shared memory before, products that read them after.
+__device__ __forceinline__ void writes_before_products() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------------------------------------- products
+template <typename T> struct Code;
+template <> struct Code<__half> { static constexpr unsigned value = 0; };
+template <> struct Code<__nv_bfloat16> { static constexpr unsigned value = 1; };
+
+// 128 x n products of 16-bit operands with sums in float32; `over_rows`: the second operand is summed over its rows.
+template <typename T> __device__ __forceinline__ unsigned shape(int n, bool over_rows)
+{
+    return (1u << 4) | (Code<T>::value << 7) | (Code<T>::value << 10) | ((over_rows ? 1u : 0u) << 16) | ((unsigned)(n >> 3) << 17) | (8u << 24);
+}
+// Operand in shared memory; `apart`: bytes between the tiles of 64 columns (used where columns are not summed over).
+__device__ __forceinline__ unsigned long long operand(unsigned address, unsigned apart)
+{
+    return (unsigned long long)((address & 0x3ffff) >> 4) | (unsigned long long)(apart >> 4) << 16 | (unsigned long long)(1024 >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+// d (+)= a b, 16 summed elements; one thread issues
+__device__ __forceinline__ void product(unsigned d, unsigned long long a, unsigned long long b, unsigned shape, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"((unsigned)add) : "memory");
+}
+// the same with the first operand in tensor memory
+__device__ __forceinline__ void product_from_tmem(unsigned d, unsigned a, unsigned long long b, unsigned shape, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(shape), "r"((unsigned)add) : "memory");
+}
+// The barrier is arrived at when all products that this thread has issued are done.
+__device__ __forceinline__ void arrive_when_done(unsigned bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// d[128 x n] (+)= a[128 rows] . b[n rows], both K-major, `steps` times 16 columns; tiles of 64 columns lie a_apart and b_apart bytes
+// behind each other.
+__device__ __forceinline__ void product_along(unsigned d, unsigned a, unsigned a_apart, unsigned b, unsigned b_apart, int steps, unsigned shape)
+{
+    for (int k = 0; k < steps; k++)
+        product(d, operand(a + (k >> 2) * a_apart + (k & 3) * 32, 16), operand(b + (k >> 2) * b_apart + (k & 3) * 32, 16), shape, k > 0);
+}
+// d[128 x columns] (+)= a[128 x 16 steps, in tensor memory] b[16 steps rows], tiles of 64 columns `apart` bytes behind each other
+__device__ __forceinline__ void product_over(unsigned d, unsigned a, unsigned b, unsigned apart, int steps, unsigned shape, bool add)
+{
+    for (int k = 0; k < steps; k++) product_from_tmem(d, a + 8 * k, operand(b + 2048 * k, apart), shape, add || k > 0);
+}
+
+// ------------------------------------------------------------------------------------------------------ tensor memory
+// One warp allocates and frees; the address is written to shared memory.
+__device__ __forceinline__ void tmem_alloc(unsigned *to, unsigned columns)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_address(to)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(unsigned address, unsigned columns)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(address), "r"(columns) : "memory");
+}
+#define HGC_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+#define HGC_R16(v, i) HGC_R4(v, i), HGC_R4(v, i + 4), HGC_R4(v, i + 8), HGC_R4(v, i + 12)
+#define HGC_S4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
+#define HGC_S16(v, i) HGC_S4(v, i), HGC_S4(v, i + 4), HGC_S4(v, i + 8), HGC_S4(v, i + 12)
+// A lane's row of 32 or 16 columns.  Warp w of a group of four reaches rows 32 w .. 32 w + 31.
+__device__ __forceinline__ void tmem_load32(unsigned (&v)[32], unsigned address)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+                 "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : HGC_R16(v, 0), HGC_R16(v, 16) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void tmem_load16(unsigned (&v)[16], unsigned address)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : HGC_R16(v, 0) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void tmem_store16(unsigned address, const unsigned (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(address), HGC_S16(v, 0) : "memory");
+}
+// What was loaded may be used: the registers pass through, so that no use of them moves ahead of the wait.
+#define HGC_P4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
+#define HGC_P16(v, i) HGC_P4(v, i), HGC_P4(v, i + 4), HGC_P4(v, i + 8), HGC_P4(v, i + 12)
+__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void use_after(unsigned (&v)[32]) { asm volatile("" : HGC_P16(v, 0), HGC_P16(v, 16) :: "memory"); }
+__device__ __forceinline__ void use_after(unsigned (&v)[16]) { asm volatile("" : HGC_P16(v, 0) :: "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x)  // relative error 2^-22
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two floats rounded to 16 bits, the first in the lower half
+template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float a, float b)
+{
+    unsigned r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b)
+{
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+}  // namespace mma
+}  // namespace hgc
