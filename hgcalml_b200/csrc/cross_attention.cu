@@ -240,15 +240,18 @@ join_forward_kernel(const float *__restrict__ part, const float *__restrict__ pa
 // ------------------------------------------------------------------------------------------------------------ backward
 // What both gradients go by.  The first `n_count` blocks: the keys of an event that can be seen, counted up to two; with one key
 // the weights do not depend on the scores, so the gradients of q and k are zero and not what is left of two sums that cancel.
-// The others: delta = sum of out * grad, a warp per row.
+// The next `n_rows` blocks, a warp per row of the queries: what its exponents are less by (log2 of its sum, less `shift`; infinity
+// without keys) and delta.  bounds: the largest squared norm of the rows of grad there, and of v in the blocks that follow.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-prepare_backward_kernel(const __grid_constant__ Args a, float *__restrict__ delta, int *__restrict__ visible, int n_count)
+prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ stats, int *__restrict__ visible, float *__restrict__ bounds, float shift,
+                        int n_count, int n_rows)
 {
     pdl_begin();
     const int t = threadIdx.x;
-    if ((int)blockIdx.x < n_count) {
-        const int e = blockIdx.x;
+    int block = blockIdx.x;
+    if (block < n_count) {
+        const int e = block;
         if (e == 0) check_splits(a, t, kThreads);
         if (e >= a.n_events) return;
         const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, e);
@@ -258,14 +261,45 @@ prepare_backward_kernel(const __grid_constant__ Args a, float *__restrict__ delt
         if (t == 0) visible[e] = min(n, 2);
         return;
     }
-    const long long row = (long long)(blockIdx.x - n_count) * (kThreads / 32) + (t >> 5);
-    if (row >= (long long)a.n_q * a.heads) return;
-    const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ grad = static_cast<const T *>(a.grad);
-    float sum = 0.f;
-    for (int d = lane_id(); d < a.dim; d += 32) sum = fmaf(to_float(out[row * a.dim + d]), to_float(grad[row * a.dim + d]), sum);
+    block -= n_count;
+    float norm = 0.f;
+    if (block < n_rows) {
+        const long long row = (long long)block * (kThreads / 32) + (t >> 5);
+        if (row < (long long)a.n_q * a.heads) {
+            const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ grad = static_cast<const T *>(a.grad);
+            float sum = 0.f;
+            for (int d = lane_id(); d < a.dim; d += 32) {
+                const float g = to_float(grad[row * a.dim + d]);
+                sum = fmaf(to_float(out[row * a.dim + d]), g, sum);
+                norm = fmaf(g, g, norm);
+            }
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    if (lane_id() == 0) delta[row] = sum;
+            for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            if (lane_id() == 0) {
+                const float lse = a.lse[row];
+                stats[row] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e - shift, sum);
+            }
+            if (row / a.heads >= split_at(a.rs_q, a.n_events, a.n_q)) norm = 0.f;  // behind the last event: of no one's concern
+        }
+    } else {
+        const long long row = (long long)(block - n_rows) * (kThreads / 32) + (t >> 5);
+        const int key = (int)(row / a.kv_heads), head = (int)(row - (long long)key * a.kv_heads);
+        if (row < (long long)a.n_k * a.kv_heads && key < split_at(a.rs_k, a.n_events, a.n_k) && (a.mask == nullptr || a.mask[key] != 0)) {
+            const T *__restrict__ v = static_cast<const T *>(a.v.p) + key * a.v.row + head * a.v.head;
+            for (int d = lane_id(); d < a.dim; d += 32) norm = fmaf(to_float(v[d]), to_float(v[d]), norm);
+        }
+    }
+    if (bounds == nullptr) return;
+    __shared__ float s_norm[kThreads / 32];
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, w);
+    if (lane_id() == 0) s_norm[t >> 5] = norm;
+    __syncthreads();
+    if (t == 0) {
+        for (int i = 1; i < kThreads / 32; i++) norm = fmaxf(norm, s_norm[i]);
+        // norms are not negative, so their bits are in the order of their values, whatever the order of the blocks
+        if (norm > 0.f) atomicMax(reinterpret_cast<unsigned *>(bounds) + (block < n_rows ? 0 : 1), __float_as_uint(norm));
+    }
 }
 
 // dq of a tile of queries: the keys of the event pass by once more.
@@ -295,8 +329,9 @@ grad_queries_kernel(const __grid_constant__ Args a)
     for (int i = 0; i < 4; i++) {
         const int r = ty + 16 * i;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
-        lse[i] = r < n_rows ? a.lse[row] * kLog2e : INFINITY;
-        delta[i] = r < n_rows ? a.delta[row] : 0.f;
+        const float2 stat = r < n_rows ? a.stats[row] : make_float2(INFINITY, 0.f);
+        lse[i] = stat.x;
+        delta[i] = stat.y;
     }
     for (int step = part.x; step < part.y; step++) {
         const int k0 = keys.x + step * kRows, n = min(kRows, keys.y - k0);
@@ -345,7 +380,7 @@ grad_keys_kernel(const __grid_constant__ Args a)
     extern __shared__ __align__(16) float s_mem[];
     float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P,
           *s_d = s_p + kRows * kPitchP;
-    __shared__ float s_lse[kRows], s_delta[kRows];
+    __shared__ float2 s_stats[kRows];
     const int t = threadIdx.x, ty = t >> 4, tx = t & 15, kv = blockIdx.y;
     const Tile tile = block_tile(a.rs_k, a.n_k, a.n_events, kRows);
     if (tile.begin >= tile.end) return;
@@ -373,8 +408,7 @@ grad_keys_kernel(const __grid_constant__ Args a)
         load_queries<T, DP, kRows>(s_g, grad, head0, q0, n, a.pack, a.dim);
         if (t < kRows) {
             const long long row = (long long)(q0 + t / a.pack) * a.heads + head0 + t % a.pack;
-            s_lse[t] = t < n ? a.lse[row] * kLog2e : INFINITY;
-            s_delta[t] = t < n ? a.delta[row] : 0.f;
+            s_stats[t] = t < n ? a.stats[row] : make_float2(INFINITY, 0.f);
         }
         __syncthreads();
         float s[4][4] = {}, dp[4][4] = {};
@@ -385,9 +419,9 @@ grad_keys_kernel(const __grid_constant__ Args a)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const bool in = seen[i] && tx + 16 * j < n;
-                const float p = in ? exp2f(fmaf(s[i][j], c, -s_lse[tx + 16 * j])) : 0.f;
+                const float p = in ? exp2f(fmaf(s[i][j], c, -s_stats[tx + 16 * j].x)) : 0.f;
                 s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = p;
-                s_d[(ty + 16 * i) * kPitchP + tx + 16 * j] = in && varies ? p * (dp[i][j] - s_delta[tx + 16 * j]) : 0.f;
+                s_d[(ty + 16 * i) * kPitchP + tx + 16 * j] = in && varies ? p * (dp[i][j] - s_stats[tx + 16 * j].y) : 0.f;
             }
         __syncthreads();
         weighted_rows<DP, 4>(dv, s_p, s_g, ty, tx);
@@ -454,7 +488,7 @@ int split_count(long long blocks, long long mean_steps, int per_sm, int least)
 
 // What a call of these sizes needs; the kernels and the workspace queries go by the same numbers.
 struct Plan {
-    int group, pack, splits, splits_mma, splits_q, splits_k;
+    int group, pack, splits, splits_mma, splits_q, splits_q_mma, splits_k, splits_k_mma;
     long long tiles_q, tiles_q64, tiles_k;
 };
 
@@ -484,7 +518,9 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     const int mma_tokens = kMmaRows / p.pack;
     p.splits_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 4, 2);
     p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
+    p.splits_q_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / kMmaGradStep, 4, 4);
     p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);
+    p.splits_k_mma = split_count(filled(n_k, kMmaRows) * kv_heads, n_q / some / (kMmaGradStep / p.pack), 2, 4);
     return p;
 }
 
@@ -509,23 +545,27 @@ template <typename C> ForwardBuffers carve_forward(C &c, const Plan &p, int n_q,
 }
 
 struct BackwardBuffers {
-    float *delta = nullptr, *part_q = nullptr, *part_k = nullptr, *part_v = nullptr;
+    float2 *stats = nullptr;
+    float *bounds = nullptr, *part_q = nullptr, *part_k = nullptr, *part_v = nullptr;
     int *visible = nullptr;
 };
 template <typename C> BackwardBuffers carve_backward(C &c, const Plan &p, int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 {
     BackwardBuffers b;
-    const size_t rows = (size_t)n_q * heads, parts_q = p.splits_q > 1 ? p.splits_q * rows * dim : 0,
-                 parts_k = p.splits_k > 1 ? (size_t)p.splits_k * n_k * kv_heads * dim : 0;
+    const int splits_q = p.splits_q > p.splits_q_mma ? p.splits_q : p.splits_q_mma, splits_k = p.splits_k > p.splits_k_mma ? p.splits_k : p.splits_k_mma;
+    const size_t rows = (size_t)n_q * heads, parts_q = splits_q > 1 ? splits_q * rows * dim : 0,
+                 parts_k = splits_k > 1 ? (size_t)splits_k * n_k * kv_heads * dim : 0;
     if constexpr (std::is_same_v<C, Carver>) {
-        b.delta = c.template take<float>(rows);
+        b.stats = c.template take<float2>(rows);
         b.visible = c.template take<int>(n_rs);
+        b.bounds = c.template take<float>(2);
         b.part_q = c.template take<float>(parts_q);
         b.part_k = c.template take<float>(parts_k);
         b.part_v = c.template take<float>(parts_k);
     } else {
-        c.template take<float>(rows);
+        c.template take<float2>(rows);
         c.template take<int>(n_rs);
+        c.template take<float>(2);
         c.template take<float>(parts_q);
         c.template take<float>(parts_k);
         c.template take<float>(parts_k);
@@ -549,21 +589,15 @@ template <typename T> int join_gradient(const Args &a, long long n, cudaStream_t
     return HGC_OK;
 }
 
-template <typename T, int DP> int run_backward(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void *dk, void *dv, cudaStream_t stream)
+template <typename T, int DP> int run_grad_queries(const Args &a, const Plan &p, cudaStream_t stream)
 {
-    const size_t smem_q = sizeof(float) * (4 * kRows * kPitch<DP> + kRows * kPitchP);
-    const size_t smem_k = smem_q + sizeof(float) * kRows * kPitchP;
-    if (dq != nullptr && a.n_q > 0) {
-        a.to = dq; a.to2 = nullptr; a.part = b.part_q; a.part2 = nullptr; a.splits = p.splits_q;
-        if (const int rc = launch(grad_queries_kernel<T, DP>, dim3((unsigned)p.tiles_q64, a.heads / a.pack, a.splits), smem_q, stream, a)) return rc;
-        if (const int rc = join_gradient<T>(a, (long long)a.n_q * a.heads * a.dim, stream)) return rc;
-    }
-    if (dk != nullptr && a.n_k > 0) {
-        a.to = dk; a.to2 = dv; a.part = b.part_k; a.part2 = b.part_v; a.splits = p.splits_k;
-        if (const int rc = launch(grad_keys_kernel<T, DP>, dim3((unsigned)p.tiles_k, a.kv_heads, a.splits), smem_k, stream, a)) return rc;
-        if (const int rc = join_gradient<T>(a, (long long)a.n_k * a.kv_heads * a.dim, stream)) return rc;
-    }
-    return HGC_OK;
+    const size_t smem = sizeof(float) * (4 * kRows * kPitch<DP> + kRows * kPitchP);
+    return launch(grad_queries_kernel<T, DP>, dim3((unsigned)p.tiles_q64, a.heads / a.pack, a.splits), smem, stream, a);
+}
+template <typename T, int DP> int run_grad_keys(const Args &a, const Plan &p, cudaStream_t stream)
+{
+    const size_t smem = sizeof(float) * (4 * kRows * kPitch<DP> + 2 * kRows * kPitchP);
+    return launch(grad_keys_kernel<T, DP>, dim3((unsigned)p.tiles_k, a.kv_heads, a.splits), smem, stream, a);
 }
 
 template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStream_t stream)
@@ -583,14 +617,34 @@ template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStrea
 }
 
 template <typename T>
-int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void *dk, void *dv, cudaStream_t stream)
+int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void *dk, void *dv, int dtype, cudaStream_t stream)
 {
-    const long long rows = (long long)a.n_q * a.heads;
-    const int n_count = a.n_events > 0 ? a.n_events : 1;
-    HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + div_up(rows, kThreads / 32), kThreads, 0, stream, a, b.delta, b.visible, n_count));
+    const auto aligned = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
+    const bool mma = mma_takes(a, dtype) && aligned(dq) && aligned(dk) && aligned(dv), bounded = mma && dtype == HGC_FLOAT16;
+    const int n_count = a.n_events > 0 ? a.n_events : 1, n_rows = div_up((long long)a.n_q * a.heads, kThreads / 32),
+              n_values = bounded ? div_up((long long)a.n_k * a.kv_heads, kThreads / 32) : 0;
+    if (bounded) HGC_CUDA_TRY(cudaMemsetAsync(b.bounds, 0, 2 * sizeof(float), stream));
+    HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + n_rows + n_values, kThreads, 0, stream, a, b.stats, b.visible,
+                            bounded ? b.bounds : nullptr, bounded ? kHalfShift : 0.f, n_count, n_rows));
     HGC_LAUNCH_CHECK();
-    return a.dim <= 32 ? run_backward<T, 32>(a, p, b, dq, dk, dv, stream)
-         : a.dim <= 64 ? run_backward<T, 64>(a, p, b, dq, dk, dv, stream) : run_backward<T, 128>(a, p, b, dq, dk, dv, stream);
+    a.stats = b.stats; a.visible = b.visible; a.bounds = b.bounds;
+    if (dq != nullptr && a.n_q > 0) {
+        a.to = dq; a.to2 = nullptr; a.part = b.part_q; a.part2 = nullptr; a.splits = mma ? p.splits_q_mma : p.splits_q;
+        if (const int rc = mma ? mma_grad_queries(a, dtype, stream)
+                         : a.dim <= 32 ? run_grad_queries<T, 32>(a, p, stream)
+                         : a.dim <= 64 ? run_grad_queries<T, 64>(a, p, stream) : run_grad_queries<T, 128>(a, p, stream))
+            return rc;
+        if (const int rc = join_gradient<T>(a, (long long)a.n_q * a.heads * a.dim, stream)) return rc;
+    }
+    if (dk != nullptr && a.n_k > 0) {
+        a.to = dk; a.to2 = dv; a.part = b.part_k; a.part2 = b.part_v; a.splits = mma ? p.splits_k_mma : p.splits_k;
+        if (const int rc = mma ? mma_grad_keys(a, dtype, stream)
+                         : a.dim <= 32 ? run_grad_keys<T, 32>(a, p, stream)
+                         : a.dim <= 64 ? run_grad_keys<T, 64>(a, p, stream) : run_grad_keys<T, 128>(a, p, stream))
+            return rc;
+        if (const int rc = join_gradient<T>(a, (long long)a.n_k * a.kv_heads * a.dim, stream)) return rc;
+    }
+    return HGC_OK;
 }
 
 Args args_of(const void *q, const void *k, const void *v, const int *rs_q, const int *rs_k, const unsigned char *mask, float *lse, int n_q, int n_k,
@@ -688,8 +742,8 @@ extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q,
                      strides, scale, p, workspace);
     Carver carver(workspace);
     const BackwardBuffers b = carve_backward(carver, p, n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
-    a.grad = d_grad_out; a.out = d_out; a.delta = b.delta; a.visible = b.visible;
-    return dtype == HGC_FLOAT32 ? backward_of<float>(a, p, b, d_grad_q, d_grad_k, d_grad_v, stream)
-         : dtype == HGC_FLOAT16 ? backward_of<__half>(a, p, b, d_grad_q, d_grad_k, d_grad_v, stream)
-                                : backward_of<__nv_bfloat16>(a, p, b, d_grad_q, d_grad_k, d_grad_v, stream);
+    a.grad = d_grad_out; a.out = d_out;
+    return dtype == HGC_FLOAT32 ? backward_of<float>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream)
+         : dtype == HGC_FLOAT16 ? backward_of<__half>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream)
+                                : backward_of<__nv_bfloat16>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream);
 }

@@ -28,13 +28,13 @@ struct Args {
     const int *rs_q, *rs_k;        // [n_events + 1]
     const unsigned char *mask;     // [n_k], zero: no query sees the key; may be null
     const void *grad, *out;        // of the backward pass
-    const float *delta;            // [n_q, heads], sum of out * grad
+    const float2 *stats;           // [n_q, heads]: what the exponents of a row's weights are less by, and delta, the sum of out * grad
     const int *visible;            // [n_events], keys that can be seen, counted up to two
     float *lse;                    // [n_q, heads], natural logarithm of the sum of exp(scale * q.k)
     void *to, *to2;                // result: out, dq, or dk and dv
     float *part, *part2;           // the same of every part of a split, in float32
     float *part_lse;               // [splits, n_q, heads]
-    const float *bounds;           // largest norms of the rows of grad and of v (half precision's backward pass)
+    const float *bounds;           // largest squared norms of the rows of grad and of v (half precision's backward pass)
     unsigned *status;
     int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits;
     float scale;
@@ -113,7 +113,12 @@ __device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int 
 bool mma_takes(const Args &a, int dtype);
 constexpr int kMmaRows = 128;
 inline __host__ __device__ int mma_keys(int dim) { return dim <= 64 ? 128 : 64; }  // keys of a step of the forward pass
+constexpr int kMmaGradStep = 64;  // keys, or queries, of a step of the backward pass
 int mma_forward(const Args &a, int dtype, cudaStream_t stream);
+int mma_grad_queries(const Args &a, int dtype, cudaStream_t stream);
+int mma_grad_keys(const Args &a, int dtype, cudaStream_t stream);
+// Weights of the backward pass in half precision are held 2^14 times as large.
+constexpr float kHalfShift = 14.f;
 
 }  // namespace attn
 }  // namespace hgc
