@@ -95,7 +95,7 @@ __device__ __forceinline__ void load_keys(float *__restrict__ dst, const Strided
     const T *__restrict__ p = static_cast<const T *>(s.p) + head * s.head;
     for (int i = threadIdx.x; i < kRows * DP; i += kThreads) {
         const int r = i / DP, d = i % DP;
-        const bool in = r < n && d < dim && (mask == nullptr || __ldg(mask + begin + r) != 0);
+        const bool in = r < n && d < dim && (mask == nullptr || fresh(mask + begin + r) != 0);
         dst[r * kPitch<DP> + d] = in ? to_float(p[(long long)(begin + r) * s.row + d]) : 0.f;
     }
 }

@@ -40,7 +40,11 @@ struct Args {
     float scale;
 };
 
-__device__ __forceinline__ int split_at(const int *__restrict__ rs, int i, int n) { return min(max(__ldg(rs + i), 0), n); }
+// What a kernel before this one may have written is read after pdl_begin(), by a load that cannot move ahead of it as one of
+// read-only data could.
+template <typename T> __device__ __forceinline__ T fresh(const T *p) { return *const_cast<const volatile T *>(p); }
+
+__device__ __forceinline__ int split_at(const int *rs, int i, int n) { return min(max(fresh(rs + i), 0), n); }
 
 // The tiles of a ragged batch: event e owns the tile numbers from rs[e] / rows + e on, which leaves room for its last, partly
 // filled tile whatever the lengths are, so that the host can size a grid (n / rows + n_events + 1) without reading the splits.
@@ -52,7 +56,7 @@ struct Tile {
 inline __host__ __device__ long long tile_count(int n, int rows, int n_events) { return (long long)n / rows + n_events + 1; }
 
 // All 32 lanes of a warp call this; 32 events are looked at in a step.
-__device__ __forceinline__ Tile find_tile(const int *__restrict__ rs, int n, int n_events, int rows, int tile)
+__device__ __forceinline__ Tile find_tile(const int *rs, int n, int n_events, int rows, int tile)
 {
     int lo = 0, hi = n_events + 1;
     while (hi - lo > 1) {
@@ -85,8 +89,8 @@ __device__ __forceinline__ void check_splits(const Args &a, int t, int threads)
 {
     bool bad = false;
     for (int i = t; i <= a.n_events; i += threads) {
-        const int q = __ldg(a.rs_q + i), k = __ldg(a.rs_k + i);
-        bad |= q > (i < a.n_events ? __ldg(a.rs_q + i + 1) : a.n_q) || k > (i < a.n_events ? __ldg(a.rs_k + i + 1) : a.n_k);
+        const int q = fresh(a.rs_q + i), k = fresh(a.rs_k + i);
+        bad |= q > (i < a.n_events ? fresh(a.rs_q + i + 1) : a.n_q) || k > (i < a.n_events ? fresh(a.rs_k + i + 1) : a.n_k);
         bad |= i == 0 && (q != 0 || k != 0);
     }
     const int any = __syncthreads_or(bad);

@@ -31,7 +31,7 @@ __device__ __forceinline__ bool seen_words(unsigned (&seen)[W], const unsigned c
 #pragma unroll
     for (int w = 0; w < W; w++) {
         const int key = 32 * w + lane_id();
-        const bool in = key < n && (mask == nullptr || __ldg(mask + k0 + key) != 0);
+        const bool in = key < n && (mask == nullptr || fresh(mask + k0 + key) != 0);
         seen[w] = __ballot_sync(0xffffffffu, in);
         all = all && seen[w] == 0xffffffffu;
     }
@@ -104,7 +104,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
     const unsigned tmem = steps > 0 ? s_tmem : 0;
 
     if (warp == 4) {
-        if (lane == 0 && steps > 0) {
+        if (steps > 0 && elect()) {
             arrive_expect(q_full, CHUNKS * kTile * a.pack * tokens);
             for (int c = 0; c < CHUNKS; c++) copy_box(s_q + c * kMmaRows * kTile, &maps.q, q_full, 64 * c, head0, tile.begin);
             int k_copies = 0, v_copies = 0;
@@ -136,11 +136,12 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             const int stage = j % F::kStages;
             const bool ok = wait_warp(k_full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
             after_sync();
-            if (lane == 0 && ok) {
-                product_along(tmem + F::kScores, s_q, kMmaRows * kTile, s_k + stage * F::kTileBytes, N * kTile, depth, shape_s);
+            if (ok && elect()) {
+                product_along<CHUNKS, kMmaRows * kTile, N * kTile>(tmem + F::kScores, s_q, s_k + stage * F::kTileBytes, depth, shape_s);
                 arrive_when_done(s_full);
                 arrive_when_done(k_empty + 8 * stage);
             }
+            __syncwarp();
         };
         if (steps > 0 && wait_warp(q_full, 0, gave_up, a.status)) {
             scores(0);
@@ -157,14 +158,14 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 if (!wait_warp(p_full, j & 1, gave_up, a.status)) break;
                 after_sync();
                 if (j + 1 < steps) scores(j + 1);
-                if (lane == 0 && !*gave_up) {
-                    product_over(tmem + F::kOut, tmem + F::kWeights, s_v + stage * F::kTileBytes, N * kTile, N / 16, shape_o, j > 0);
+                if (elect()) {
+                    product_over<N / 16, N * kTile>(tmem + F::kOut, tmem + F::kWeights, s_v + stage * F::kTileBytes, shape_o, j > 0);
                     arrive_when_done(o_full);
                     arrive_when_done(v_empty + 8 * stage);
                 }
                 __syncwarp();
             }
-            if (lane == 0) {  // no product is under way when the tensor memory is freed
+            if (elect()) {  // no product is under way when the tensor memory is freed
                 arrive_when_done(all_done);
                 drain(all_done, 0);
             }
@@ -298,7 +299,7 @@ template <> struct Range<__half> { static constexpr float kShift = kHalfShift; }
 template <typename T> __device__ __forceinline__ float slope_factor(const Args &a)
 {
     if (Range<T>::kShift == 0.f) return 1.f;
-    const float bound = sqrtf(__ldg(a.bounds)) * sqrtf(__ldg(a.bounds + 1));
+    const float bound = sqrtf(fresh(a.bounds)) * sqrtf(fresh(a.bounds + 1));
     return bound > 0.f && bound < 1e30f ? exp2f(-ceilf(log2f(bound))) : 1.f;
 }
 
@@ -332,322 +333,161 @@ __device__ __forceinline__ void store16(void *to, float *part, long long at, int
     }
 }
 
-// dq: as the forward pass, with S = Q K^T and dP = dO V^T, from which dS (16 bits) goes into dQ += dS K.  64 keys a step, so that two
-// blocks fit a multiprocessor.  Wide heads: dS takes the place of S, and V has one stage.
-template <int CHUNKS> struct GradQueries {
-    static constexpr int kKeys = kMmaGradStep, kStagesK = 2, kStagesV = CHUNKS == 1 ? 2 : 1;
-    static constexpr int kTileBytes = kKeys * kTile * CHUNKS, kQueryBytes = kMmaRows * kTile * CHUNKS;
-    static constexpr int kTiles = 2 * kQueryBytes + (kStagesK + kStagesV) * kTileBytes, kSmem = kTiles + 256;
-    static constexpr bool kInPlace = CHUNKS == 2;
-    static constexpr int kScores = 0, kProducts = 64, kSlopes = kInPlace ? 0 : 128, kOut = kInPlace ? 128 : 160, kColumns = 256;
-    static constexpr int kBarriers = 1 + 2 * kStagesK + 2 * kStagesV + 4;
+// Both gradients are the same walk.  A block keeps 128 rows of two tensors (KEYS: keys and values, else queries and grad) and the
+// rows of the two others of the event pass by, 64 a step:
+//   KEYS: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q;  else S = Q K^T, dP = dO V^T, dQ += dS K
+// with a kept row per lane.  P and dS (16 bits) take the places of S and dP in tensor memory, from where they are an operand of the
+// sums.  One block has a multiprocessor and all 512 columns: the sums, and as many buffers for S and dP as there is room for, so
+// that two groups of four warps, which take the steps in turn, find the next step's scores done.
+// (Two blocks of 256 columns, each with one buffer, waited for products two thirds of the time: 16k x 16k rows, 8 heads of 64, 3.2 ms.)
+template <int CHUNKS, bool KEYS> struct Grad {
+    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 320;
+    static constexpr int kTileBytes = kStep * kTile * CHUNKS, kKeptBytes = kMmaRows * kTile * CHUNKS;
+    static constexpr int kBuffers = KEYS && CHUNKS == 2 ? 2 : 3, kSums = 128 * kBuffers, kSums2 = kSums + 64 * CHUNKS, kColumns = 512;
+    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 2 * 2 * kStep * 4, kSmem = kTiles + kStats + 256;
+    static constexpr int kBarriers = 2 + 2 * kStages + 3 * kBuffers;
+    static_assert((KEYS ? kSums2 : kSums) + 64 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 256, "room");
 };
 
-template <typename T, int CHUNKS>
-__global__ void __launch_bounds__(kBlock, 2)
-grad_queries_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps)
+template <typename T, int CHUNKS, bool KEYS>
+__global__ void __launch_bounds__(Grad<CHUNKS, KEYS>::kThreads, 1)
+grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps)
 {
     pdl_begin();
-    using F = GradQueries<CHUNKS>;
-    constexpr int N = F::kKeys, W = N / 32;
+    using F = Grad<CHUNKS, KEYS>;
+    constexpr int N = F::kStep, W = N / 32, B = F::kBuffers;
+    constexpr bool kScaled = Range<T>::kShift != 0.f;
     extern __shared__ __align__(1024) char s_raw[];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int tokens = kMmaRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
-    const Tile tile = find_tile(a.rs_q, a.n_q, a.n_events, tokens, blockIdx.x);
+    const int tokens = (KEYS ? N : kMmaRows) / a.pack;  // of a tile of queries
+    const int kv = KEYS ? blockIdx.y : blockIdx.y * a.pack / a.group, packs = KEYS ? a.group / a.pack : 1;
+    const Tile tile = KEYS ? find_tile(a.rs_k, a.n_k, a.n_events, kMmaRows, blockIdx.x) : find_tile(a.rs_q, a.n_q, a.n_events, tokens, blockIdx.x);
     if (tile.begin >= tile.end) return;
-    const int n_rows = (tile.end - tile.begin) * a.pack;
-    int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
-    if (tile.event < a.n_events && a.visible[tile.event] < 2) keys.y = keys.x;
-    const int2 part = part_of(max(0, (keys.y - keys.x + N - 1) / N), blockIdx.z, a.splits);
-    const int steps = part.y - part.x, first = keys.x + part.x * N;
+    const int n_rows = KEYS ? tile.end - tile.begin : (tile.end - tile.begin) * a.pack;
+    const bool varies = tile.event < a.n_events && fresh(a.visible + tile.event) > 1;
+    int2 others = KEYS ? rows_of(a.rs_q, a.n_q, a.n_events, tile.event) : rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
+    if (!KEYS && !varies) others.y = others.x;
+    const int rows_a_step = KEYS ? tokens : N;
+    const int2 part = part_of(max(0, (others.y - others.x + rows_a_step - 1) / rows_a_step), blockIdx.z, a.splits);
+    const int first_step = part.x * packs, steps = part.y * packs - first_step;
+    // first row (of a head, or packed heads) of a step
+    const auto row_of = [&](int j) { return others.x + (first_step + j) / packs * rows_a_step; };
+    const auto head_of = [&](int j) { return KEYS ? kv * a.group + (first_step + j) % packs * a.pack : kv; };
 
-    const unsigned s_q = smem_address(s_raw), s_g = s_q + F::kQueryBytes, s_k = s_g + F::kQueryBytes, s_v = s_k + F::kStagesK * F::kTileBytes;
-    const unsigned bar = s_q + F::kTiles, q_full = bar, k_full = bar + 8, k_empty = k_full + 8 * F::kStagesK, v_full = k_empty + 8 * F::kStagesK,
-                   v_empty = v_full + 8 * F::kStagesV, s_full = v_empty + 8 * F::kStagesV, p_full = s_full + 8, o_full = p_full + 8, all_done = o_full + 8;
-    static_assert(8 * F::kBarriers + 8 <= 256, "room behind the tiles");
-    unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + 8 * F::kBarriers);
-    volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
-    if (steps > 0) {
-        if (t == 0) {
-            for (int i = 0; i < F::kBarriers; i++) barrier_init(bar + 8 * i, bar + 8 * i == p_full ? 4 : 1);
-            barrier_init_done();
-            *gave_up = 0;
-        }
-        if (warp == 5) tmem_alloc(s_tmem, F::kColumns);
-        before_sync();
-        __syncthreads();
-        after_sync();
-    }
-    const unsigned tmem = steps > 0 ? *s_tmem : 0;
-
-    if (warp == 4) {
-        if (lane == 0 && steps > 0) {
-            arrive_expect(q_full, 2 * CHUNKS * kTile * a.pack * tokens);
-            for (int c = 0; c < CHUNKS; c++) {
-                copy_box(s_q + c * kMmaRows * kTile, &maps.q, q_full, 64 * c, head0, tile.begin);
-                copy_box(s_g + c * kMmaRows * kTile, &maps.grad, q_full, 64 * c, head0, tile.begin);
-            }
-            int k_copies = 0, v_copies = 0;
-            for (int j = 0; j < steps; j++) {
-                const int sk = j % F::kStagesK, sv = j % F::kStagesV;
-                if (j >= F::kStagesK && !wait(k_empty + 8 * sk, (j / F::kStagesK & 1) ^ 1, gave_up, a.status)) break;
-                arrive_expect(k_full + 8 * sk, F::kTileBytes);
-                for (int c = 0; c < CHUNKS; c++) copy_box(s_k + sk * F::kTileBytes + c * N * kTile, &maps.k, k_full + 8 * sk, 64 * c, kv, first + j * N);
-                k_copies++;
-                if (j >= F::kStagesV && !wait(v_empty + 8 * sv, (j / F::kStagesV & 1) ^ 1, gave_up, a.status)) break;
-                arrive_expect(v_full + 8 * sv, F::kTileBytes);
-                for (int c = 0; c < CHUNKS; c++) copy_box(s_v + sv * F::kTileBytes + c * N * kTile, &maps.v, v_full + 8 * sv, 64 * c, kv, first + j * N);
-                v_copies++;
-            }
-            drain(q_full, 0);
-            for (int j = max(0, k_copies - F::kStagesK); j < k_copies; j++) drain(k_full + 8 * (j % F::kStagesK), j / F::kStagesK & 1);
-            for (int j = max(0, v_copies - F::kStagesV); j < v_copies; j++) drain(v_full + 8 * (j % F::kStagesV), j / F::kStagesV & 1);
-        }
-        __syncwarp();
-    } else if (warp == 5) {
-        const int depth = (a.dim + 15) / 16;
-        const unsigned shape_s = shape<T>(N, false), shape_o = shape<T>(16 * depth, true);
-        const auto scores = [&](int j) {
-            const int sk = j % F::kStagesK, sv = j % F::kStagesV;
-            unsigned seen[W];
-            const bool all = seen_words<W>(seen, a.mask, first + j * N, keys.y - (first + j * N));
-            bool ok = wait_warp(k_full + 8 * sk, j / F::kStagesK & 1, gave_up, a.status);
-            if (ok && !all) {
-                clear_unseen<W>(s_k + sk * F::kTileBytes, CHUNKS, seen);
-                writes_before_products();
-                __syncwarp();
-            }
-            ok = ok && wait_warp(v_full + 8 * sv, j / F::kStagesV & 1, gave_up, a.status);
-            after_sync();
-            if (lane == 0 && ok) {
-                product_along(tmem + F::kScores, s_q, kMmaRows * kTile, s_k + sk * F::kTileBytes, N * kTile, depth, shape_s);
-                product_along(tmem + F::kProducts, s_g, kMmaRows * kTile, s_v + sv * F::kTileBytes, N * kTile, depth, shape_s);
-                arrive_when_done(s_full);
-                arrive_when_done(v_empty + 8 * sv);
-            }
-            __syncwarp();
-        };
-        if (steps > 0 && wait_warp(q_full, 0, gave_up, a.status)) {
-            scores(0);
-            for (int j = 0; j < steps; j++) {
-                const int sk = j % F::kStagesK;
-                if (!wait_warp(p_full, j & 1, gave_up, a.status)) break;
-                after_sync();
-                if (!F::kInPlace && j + 1 < steps) scores(j + 1);
-                if (lane == 0 && !*gave_up) {
-                    product_over(tmem + F::kOut, tmem + F::kSlopes, s_k + sk * F::kTileBytes, N * kTile, N / 16, shape_o, j > 0);
-                    arrive_when_done(o_full);
-                    arrive_when_done(k_empty + 8 * sk);
-                }
-                __syncwarp();
-                if (F::kInPlace && j + 1 < steps) {
-                    if (!wait_warp(o_full, j & 1, gave_up, a.status)) break;
-                    scores(j + 1);
-                }
-            }
-            if (lane == 0) {
-                arrive_when_done(all_done);
-                drain(all_done, 0);
-            }
-            __syncwarp();
-        }
-    } else {
-        const unsigned rows = tmem + ((unsigned)warp << 21);
-        const bool idle = warp * 32 >= n_rows, store = t < n_rows;
-        const long long row = (long long)(tile.begin + t / a.pack) * a.heads + head0 + t % a.pack;
-        const float c = a.scale * kLog2e, factor = slope_factor<T>(a);
-        const float2 stat = store ? a.stats[row] : make_float2(INFINITY, 0.f);
-        const float shift = stat.x, delta = stat.y * factor;
-        for (int j = 0; j < steps; j++) {
-            unsigned seen[W];
-            const bool all = seen_words<W>(seen, a.mask, first + j * N, keys.y - (first + j * N));
-            if (!wait_warp(s_full, j & 1, gave_up, a.status)) break;
-            after_sync();
-            unsigned slopes[W][16];
-            if (!idle) {
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    unsigned s[32], g[32];
-                    tmem_load32(s, rows + F::kScores + 32 * w);
-                    tmem_load32(g, rows + F::kProducts + 32 * w);
-                    tmem_loaded();
-                    use_after(s);
-                    use_after(g);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const float p = exp2_fast(fmaf(__uint_as_float(s[i]), c, -shift));
-                        const float d = Range<T>::kShift == 0.f ? __uint_as_float(g[i]) - delta : fmaf(__uint_as_float(g[i]), factor, -delta);
-                        s[i] = __float_as_uint(p * d);
-                    }
-                    if (!all) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (!((seen[w] >> i) & 1u)) s[i] = 0;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) slopes[w][i] = pack2<T>(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                }
-            }
-            // where the slopes go, the last step's product has been
-            if (!F::kInPlace && j > 0 && !wait_warp(o_full, (j - 1) & 1, gave_up, a.status)) break;
-            if (!idle) {
-                after_sync();
-#pragma unroll
-                for (int w = 0; w < W; w++) tmem_store16(rows + F::kSlopes + 16 * w, slopes[w]);
-                tmem_stored();
-            }
-            before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(p_full);
-        }
-        const bool done = steps > 0 && wait_warp(o_full, (steps - 1) & 1, gave_up, a.status);
-        if (done) after_sync();
-        const float back = a.scale * exp2f(-Range<T>::kShift) / factor;
-        float *to_part = a.splits > 1 ? a.part + blockIdx.z * (long long)a.n_q * a.heads * a.dim : nullptr;
-        if (!idle)
-            for (int d = 0; d < a.dim; d += 16) {
-                unsigned o[16] = {};
-                if (done) {
-                    tmem_load16(o, rows + F::kOut + d);
-                    tmem_loaded();
-                    use_after(o);
-                }
-                if (store) store16<T>(a.to, to_part, row * a.dim, d, a.dim, o, back);
-                __syncwarp();
-            }
-    }
-    if (steps > 0) {
-        before_sync();
-        __syncthreads();
-        after_sync();
-        if (warp == 5) tmem_free(tmem, F::kColumns);
-    }
-}
-
-// dk and dv of 128 keys: a lane has a key, columns are queries.  S^T = K Q^T and dP^T = V dO^T give P^T and dS^T (16 bits, in their
-// places), which go into dV += P^T dO and dK += dS^T Q straight from tensor memory.  Narrow heads: 256 columns and two blocks on a
-// multiprocessor.  Wide ones: all 512 columns, and two groups of four warps that take the steps in turn.
-template <int CHUNKS> struct GradKeys {
-    static constexpr int kQueries = kMmaGradStep, kGroups = CHUNKS, kStages = CHUNKS == 1 ? 2 : 3, kThreads = 128 * kGroups + 64;
-    static constexpr int kTileBytes = kQueries * kTile * CHUNKS, kKeyBytes = kMmaRows * kTile * CHUNKS;
-    static constexpr int kTiles = 2 * kKeyBytes + 2 * kStages * kTileBytes, kStats = kGroups * kQueries * 8, kSmem = kTiles + kStats + 256;
-    static constexpr int kDk = 128 * kGroups, kDv = kDk + 64 * CHUNKS, kColumns = 256 * CHUNKS;
-    static constexpr int kBarriers = 1 + 2 * kStages + 3 * kGroups + 1;
-};
-
-template <typename T, int CHUNKS>
-__global__ void __launch_bounds__(GradKeys<CHUNKS>::kThreads, CHUNKS == 1 ? 2 : 1)
-grad_keys_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps)
-{
-    pdl_begin();
-    using F = GradKeys<CHUNKS>;
-    constexpr int N = F::kQueries, G = F::kGroups;
-    extern __shared__ __align__(1024) char s_raw[];
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, kv = blockIdx.y;
-    const Tile tile = find_tile(a.rs_k, a.n_k, a.n_events, kMmaRows, blockIdx.x);
-    if (tile.begin >= tile.end) return;
-    const int n_keys = tile.end - tile.begin, tokens = N / a.pack, packs = a.group / a.pack;
-    const int2 queries = rows_of(a.rs_q, a.n_q, a.n_events, tile.event);
-    const int2 part = part_of(max(0, (queries.y - queries.x + tokens - 1) / tokens), blockIdx.z, a.splits);
-    const int begin = part.x * packs, steps = part.y * packs - begin;
-    const bool varies = tile.event < a.n_events && a.visible[tile.event] > 1;
-
-    const unsigned s_k = smem_address(s_raw), s_v = s_k + F::kKeyBytes, s_q = s_v + F::kKeyBytes, s_g = s_q + F::kStages * F::kTileBytes;
-    const unsigned bar = s_k + F::kTiles + F::kStats, k_full = bar, q_full = bar + 8, q_empty = q_full + 8 * F::kStages, s_full = q_empty + 8 * F::kStages,
-                   p_full = s_full + 8 * G, used = p_full + 8 * G, all_done = used + 8 * G;
-    static_assert(8 * F::kBarriers + 8 <= 256, "room behind the tiles");
-    float2 *s_stats = reinterpret_cast<float2 *>(s_raw + F::kTiles);
+    const unsigned s_kept = smem_address(s_raw), s_kept2 = s_kept + F::kKeptBytes, s_step = s_kept2 + F::kKeptBytes,
+                   s_step2 = s_step + F::kStages * F::kTileBytes;
+    const unsigned bar = s_kept + F::kTiles + F::kStats, kept_full = bar, all_done = bar + 8, full = all_done + 8, empty = full + 8 * F::kStages,
+                   s_full = empty + 8 * F::kStages, p_full = s_full + 8 * B, used = p_full + 8 * B;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + F::kStats + 8 * F::kBarriers);
     volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
     if (steps > 0) {
         if (t == 0) {
             for (int i = 0; i < F::kBarriers; i++) {
-                const unsigned b = bar + 8 * i;
-                barrier_init(b, b >= p_full && b < used ? 4 : 1);
+                const unsigned at = bar + 8 * i;
+                barrier_init(at, at >= p_full && at < used ? 4 : 1);
             }
             barrier_init_done();
             *gave_up = 0;
         }
-        if (warp == 4 * G + 1) tmem_alloc(s_tmem, F::kColumns);
+        if (warp == 9) tmem_alloc(s_tmem, F::kColumns);
         before_sync();
         __syncthreads();
         after_sync();
     }
     const unsigned tmem = steps > 0 ? *s_tmem : 0;
 
-    if (warp == 4 * G) {
-        if (lane == 0 && steps > 0) {
-            arrive_expect(k_full, 2 * F::kKeyBytes);
+    if (warp == 8) {
+        if (steps > 0 && elect()) {
+            const int kept_head = KEYS ? kv : blockIdx.y * a.pack;
+            arrive_expect(kept_full, KEYS ? 2 * F::kKeptBytes : 2 * CHUNKS * kTile * a.pack * tokens);
             for (int c = 0; c < CHUNKS; c++) {
-                copy_box(s_k + c * kMmaRows * kTile, &maps.k, k_full, 64 * c, kv, tile.begin);
-                copy_box(s_v + c * kMmaRows * kTile, &maps.v, k_full, 64 * c, kv, tile.begin);
+                copy_box(s_kept + c * kMmaRows * kTile, KEYS ? &maps.k : &maps.q, kept_full, 64 * c, kept_head, tile.begin);
+                copy_box(s_kept2 + c * kMmaRows * kTile, KEYS ? &maps.v : &maps.grad, kept_full, 64 * c, kept_head, tile.begin);
             }
             int copies = 0;
             for (int j = 0; j < steps; j++) {
-                const int stage = j % F::kStages, step = begin + j;
-                if (j >= F::kStages && !wait(q_empty + 8 * stage, (j / F::kStages & 1) ^ 1, gave_up, a.status)) break;
-                arrive_expect(q_full + 8 * stage, 2 * CHUNKS * kTile * a.pack * tokens);
-                const int q0 = queries.x + step / packs * tokens, head0 = kv * a.group + step % packs * a.pack;
+                const int stage = j % F::kStages;
+                if (j >= F::kStages && !wait(empty + 8 * stage, (j / F::kStages & 1) ^ 1, gave_up, a.status)) break;
+                arrive_expect(full + 8 * stage, KEYS ? 2 * CHUNKS * kTile * a.pack * tokens : 2 * F::kTileBytes);
                 for (int c = 0; c < CHUNKS; c++) {
-                    copy_box(s_q + stage * F::kTileBytes + c * N * kTile, &maps.q, q_full + 8 * stage, 64 * c, head0, q0);
-                    copy_box(s_g + stage * F::kTileBytes + c * N * kTile, &maps.grad, q_full + 8 * stage, 64 * c, head0, q0);
+                    copy_box(s_step + stage * F::kTileBytes + c * N * kTile, KEYS ? &maps.q : &maps.k, full + 8 * stage, 64 * c, head_of(j), row_of(j));
+                    copy_box(s_step2 + stage * F::kTileBytes + c * N * kTile, KEYS ? &maps.grad : &maps.v, full + 8 * stage, 64 * c, head_of(j), row_of(j));
                 }
                 copies++;
             }
-            drain(k_full, 0);
-            for (int j = max(0, copies - F::kStages); j < copies; j++) drain(q_full + 8 * (j % F::kStages), j / F::kStages & 1);
+            // no copy is under way when the block leaves
+            drain(kept_full, 0);
+            for (int j = max(0, copies - F::kStages); j < copies; j++) drain(full + 8 * (j % F::kStages), j / F::kStages & 1);
         }
         __syncwarp();
-    } else if (warp == 4 * G + 1) {
+    } else if (warp == 9) {
         const int depth = (a.dim + 15) / 16;
         const unsigned shape_s = shape<T>(N, false), shape_o = shape<T>(16 * depth, true);
         const auto scores = [&](int j) {
-            const int stage = j % F::kStages, g = j % G;
-            const bool ok = wait_warp(q_full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
-            // rows of another event are not summed over, whatever they hold
-            const int n = min(tokens, queries.y - (queries.x + (begin + j) / packs * tokens)) * a.pack;
-            if (ok && n < a.pack * tokens) {
-                clear_rows(s_q + stage * F::kTileBytes, CHUNKS, N, n, a.pack * tokens);
-                clear_rows(s_g + stage * F::kTileBytes, CHUNKS, N, n, a.pack * tokens);
-                writes_before_products();
-                __syncwarp();
+            const int stage = j % F::kStages;
+            const unsigned step = s_step + stage * F::kTileBytes, step2 = s_step2 + stage * F::kTileBytes;
+            bool ok;
+            if (KEYS) {
+                // rows of another event are not summed over, whatever they hold
+                const int n = min(tokens, others.y - row_of(j)) * a.pack;
+                ok = wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
+                if (ok && n < a.pack * tokens) {
+                    clear_rows(step, CHUNKS, N, n, a.pack * tokens);
+                    clear_rows(step2, CHUNKS, N, n, a.pack * tokens);
+                    writes_before_products();
+                    __syncwarp();
+                }
+            } else {
+                unsigned seen[W];
+                const bool all = seen_words<W>(seen, a.mask, row_of(j), others.y - row_of(j));
+                ok = wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
+                if (ok && !all) {
+                    clear_unseen<W>(step, CHUNKS, seen);
+                    writes_before_products();
+                    __syncwarp();
+                }
             }
             after_sync();
-            if (lane == 0 && ok) {
-                product_along(tmem + 128 * g, s_k, kMmaRows * kTile, s_q + stage * F::kTileBytes, N * kTile, depth, shape_s);
-                product_along(tmem + 128 * g + 64, s_v, kMmaRows * kTile, s_g + stage * F::kTileBytes, N * kTile, depth, shape_s);
-                arrive_when_done(s_full + 8 * g);
+            if (ok && elect()) {
+                const unsigned to = tmem + 128 * (j % B);
+                product_along<CHUNKS, kMmaRows * kTile, N * kTile>(to, s_kept, step, depth, shape_s);
+                product_along<CHUNKS, kMmaRows * kTile, N * kTile>(to + 64, s_kept2, step2, depth, shape_s);
+                arrive_when_done(s_full + 8 * (j % B));
             }
             __syncwarp();
         };
         if (steps > 0) {
-            if (a.pack * tokens < N) {  // rows that no copy writes
+            if (KEYS && a.pack * tokens < N) {  // rows that no copy writes
                 for (int i = 0; i < F::kStages; i++) {
-                    clear_rows(s_q + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
-                    clear_rows(s_g + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
+                    clear_rows(s_step + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
+                    clear_rows(s_step2 + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
                 }
                 writes_before_products();
                 __syncwarp();
             }
-            if (wait_warp(k_full, 0, gave_up, a.status)) {
-                for (int j = 0; j < min(G, steps); j++) scores(j);
+            if (wait_warp(kept_full, 0, gave_up, a.status)) {
+                // With a buffer to spare, the scores for the buffer that was freed one step ago follow the sums of this one, and
+                // the tensor cores do not wait; with two buffers that would make the groups wait for each other.
+                constexpr int kLag = B > 2 ? 1 : 0;
+                for (int j = 0; j < min(B, steps); j++) scores(j);
                 for (int j = 0; j < steps; j++) {
-                    const int stage = j % F::kStages, g = j % G;
-                    if (!wait_warp(p_full + 8 * g, j / G & 1, gave_up, a.status)) break;
+                    const int stage = j % F::kStages, b = j % B, freed = j - kLag;
+                    if (!wait_warp(p_full + 8 * b, j / B & 1, gave_up, a.status)) break;
                     after_sync();
-                    if (lane == 0 && !*gave_up) {
-                        product_over(tmem + F::kDv, tmem + 128 * g, s_g + stage * F::kTileBytes, N * kTile, N / 16, shape_o, j > 0);
-                        product_over(tmem + F::kDk, tmem + 128 * g + 64, s_q + stage * F::kTileBytes, N * kTile, N / 16, shape_o, j > 0);
-                        arrive_when_done(used + 8 * g);
-                        arrive_when_done(q_empty + 8 * stage);
+                    if (elect()) {
+                        const unsigned from = tmem + 128 * b, step = s_step + stage * F::kTileBytes, step2 = s_step2 + stage * F::kTileBytes;
+                        if (KEYS) product_over<N / 16, N * kTile>(tmem + F::kSums2, from, step2, shape_o, j > 0);
+                        product_over<N / 16, N * kTile>(tmem + F::kSums, from + 64, step, shape_o, j > 0);
+                        arrive_when_done(used + 8 * b);
+                        arrive_when_done(empty + 8 * stage);
                     }
                     __syncwarp();
-                    if (j + G < steps) {
-                        if (!wait_warp(used + 8 * g, j / G & 1, gave_up, a.status)) break;
-                        scores(j + G);
+                    if (freed >= 0 && freed + B < steps) {
+                        if (!wait_warp(used + 8 * (freed % B), freed / B & 1, gave_up, a.status)) break;
+                        scores(freed + B);
                     }
                 }
-                if (lane == 0) {
+                if (elect()) {  // no product is under way when the tensor memory is freed
                     arrive_when_done(all_done);
                     drain(all_done, 0);
                 }
@@ -656,25 +496,45 @@ grad_keys_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Map
         }
     } else {
         const int g = warp >> 2, r = t & 127;
-        const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21), rows = lanes + 128 * g;
-        const bool store = r < n_keys;
-        const unsigned seen = store && (a.mask == nullptr || __ldg(a.mask + tile.begin + r) != 0) ? 0xffffffffu : 0u;
-        const float c = a.scale * kLog2e, factor = slope_factor<T>(a);
-        float2 *stats = s_stats + g * N;
-        for (int j = g; j < steps; j += G) {
-            const int step = begin + j, q0 = queries.x + step / packs * tokens, head0 = kv * a.group + step % packs * a.pack;
-            float2 mine = make_float2(INFINITY, 0.f);
-            if (r < min(tokens, queries.y - q0) * a.pack) {
-                mine = a.stats[(long long)(q0 + r / a.pack) * a.heads + head0 + r % a.pack];
-                mine.y *= factor;
+        const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21);
+        const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;
+        const float scale = a.scale * kLog2e, factor = slope_factor<T>(a);
+        const pair c = pair_of(scale, scale), f = pair_of(factor, factor);
+        // KEYS: of the columns, in shared memory, negative, first the exponents' and then the slopes'.  Else of this lane's row.
+        float *stats = reinterpret_cast<float *>(s_raw + F::kTiles) + g * 2 * N;
+        const long long row = KEYS ? ((long long)(tile.begin + r) * a.kv_heads + kv)
+                                   : (long long)(tile.begin + r / a.pack) * a.heads + blockIdx.y * a.pack + r % a.pack;
+        pair shift = 0, delta = 0;
+        unsigned seen_row = 0xffffffffu;
+        if (KEYS) {
+            seen_row = store && (a.mask == nullptr || fresh(a.mask + tile.begin + r) != 0) ? 0xffffffffu : 0u;
+        } else {
+            const float2 stat = store ? a.stats[row] : make_float2(INFINITY, 0.f);
+            shift = pair_of(-stat.x, -stat.x);
+            delta = pair_of(-stat.y * factor, -stat.y * factor);
+        }
+        for (int j = g; j < steps; j += 2) {
+            const unsigned rows = lanes + 128 * (j % B);
+            unsigned seen[W];
+            bool all = true;
+            if (KEYS) {
+                float2 mine = make_float2(INFINITY, 0.f);
+                const int q0 = row_of(j);
+                if (r < min(tokens, others.y - q0) * a.pack) mine = a.stats[(long long)(q0 + r / a.pack) * a.heads + head_of(j) + r % a.pack];
+                asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");  // the last step's have been read
+                if (r < N) {
+                    stats[r] = -mine.x;
+                    stats[N + r] = -mine.y * factor;
+                }
+                asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");
+            } else {
+                all = seen_words<W>(seen, a.mask, row_of(j), others.y - row_of(j));
             }
-            asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");  // the last step's have been read
-            if (r < N) stats[r] = mine;
-            asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");
-            if (wait_warp(s_full + 8 * g, j / G & 1, gave_up, a.status)) {  // else on to the next step: the group's barriers count on all warps
+            // if a wait gave up, on to the next step: the group's barriers count on all warps
+            if (wait_warp(s_full + 8 * (j % B), j / B & 1, gave_up, a.status) && !idle) {
                 after_sync();
 #pragma unroll
-                for (int w = 0; w < N / 32; w++) {
+                for (int w = 0; w < W; w++) {
                     unsigned s[32], d[32], p[16], q[16];
                     tmem_load32(s, rows + 32 * w);
                     tmem_load32(d, rows + 64 + 32 * w);
@@ -682,53 +542,68 @@ grad_keys_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Map
                     use_after(s);
                     use_after(d);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float4 st = *reinterpret_cast<const float4 *>(stats + 32 * w + i);
-                        const float p0 = exp2_fast(fmaf(__uint_as_float(s[i]), c, -st.x)), p1 = exp2_fast(fmaf(__uint_as_float(s[i + 1]), c, -st.z));
-                        float d0 = __uint_as_float(d[i]), d1 = __uint_as_float(d[i + 1]);
-                        d0 = Range<T>::kShift == 0.f ? d0 - st.y : fmaf(d0, factor, -st.y);
-                        d1 = Range<T>::kShift == 0.f ? d1 - st.w : fmaf(d1, factor, -st.w);
-                        p[i / 2] = pack2<T>(p0, p1) & seen;
-                        q[i / 2] = pack2<T>(p0 * d0, p1 * d1) & seen;
+                    for (int i = 0; i < 32; i += 4) {
+                        pair x[2] = {shift, shift}, y[2] = {delta, delta};
+                        if (KEYS) {
+                            const ulonglong2 sx = *reinterpret_cast<const ulonglong2 *>(stats + 32 * w + i);
+                            const ulonglong2 sy = *reinterpret_cast<const ulonglong2 *>(stats + N + 32 * w + i);
+                            x[0] = sx.x; x[1] = sx.y; y[0] = sy.x; y[1] = sy.y;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int at = i + 2 * h;
+                            const float2 e = parts(fma2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c, x[h]));
+                            const float2 w2 = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            const pair dp = pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1]));
+                            const float2 slope = parts(mul2(pair_of(w2.x, w2.y), kScaled ? fma2(dp, f, y[h]) : add2(dp, y[h])));
+                            if (KEYS) {
+                                p[at / 2] = pack2<T>(w2.x, w2.y) & seen_row;
+                                q[at / 2] = pack2<T>(slope.x, slope.y) & seen_row;
+                            } else {
+                                q[at / 2] = pack2<T>(slope.x, slope.y);
+                            }
+                        }
+                    }
+                    if (!KEYS && !all) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            q[i] &= ((seen[w] >> (2 * i)) & 1u ? 0x0000ffffu : 0u) | ((seen[w] >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
                     }
                     // in place: these columns have been read, by the lanes that own their rows
-                    tmem_store16(rows + 16 * w, p);
+                    if (KEYS) tmem_store16(rows + 16 * w, p);
                     tmem_store16(rows + 64 + 16 * w, q);
                 }
                 tmem_stored();
             }
             before_sync();
             __syncwarp();
-            if (lane == 0) arrive(p_full + 8 * g);
+            if (lane == 0) arrive(p_full + 8 * (j % B));
         }
-        // the sums are complete when the last step's products are: that of this group's own last step waits for it
-        bool done = steps > 0;
-        if (steps > 0) done = wait_warp(all_done, 0, gave_up, a.status);
+        const bool done = steps > 0 && wait_warp(all_done, 0, gave_up, a.status);
         if (done) after_sync();
-        const long long at = ((long long)(tile.begin + r) * a.kv_heads + kv) * a.dim, all = (long long)a.n_k * a.kv_heads * a.dim;
         const float back = exp2f(-Range<T>::kShift);
-        // one group writes dv, the last one dk
-        for (int which = 0; which < 2; which++) {
-            if (G == 2 && which != g) continue;
-            float *to_part = a.splits > 1 ? (which == 0 ? a.part2 : a.part) + blockIdx.z * all : nullptr;
-            const float f = which == 0 ? back : varies ? a.scale * back / factor : 0.f;
-            for (int d = 0; d < a.dim; d += 16) {
-                unsigned o[16] = {};
-                if (done && (which == 0 || varies)) {
-                    tmem_load16(o, lanes + (which == 0 ? F::kDv : F::kDk) + d);
-                    tmem_loaded();
-                    use_after(o);
-                }
-                if (store) store16<T>(which == 0 ? a.to2 : a.to, to_part, at, d, a.dim, o, f);
-                __syncwarp();
+        const long long all_rows = KEYS ? (long long)a.n_k * a.kv_heads : (long long)a.n_q * a.heads;
+        // KEYS: the first group writes dv and the second dk; else they share the columns
+        float *to_part = a.splits > 1 ? (KEYS && g == 0 ? a.part2 : a.part) + blockIdx.z * all_rows * a.dim : nullptr;
+        void *to = KEYS && g == 0 ? a.to2 : a.to;
+        const float by = KEYS && g == 0 ? back : a.scale * back / factor;
+        const bool some = done && (varies || (KEYS && g == 0));
+        for (int d = KEYS ? 0 : 16 * g; d < a.dim; d += KEYS ? 16 : 32) {
+            unsigned o[16] = {};
+            if (some) {
+                tmem_load16(o, lanes + (KEYS && g == 0 ? F::kSums2 : F::kSums) + d);
+                tmem_loaded();
+                use_after(o);
             }
+            if (store) store16<T>(to, to_part, row * a.dim, d, a.dim, o, some ? by : 0.f);
+            __syncwarp();
         }
     }
     if (steps > 0) {
         before_sync();
         __syncthreads();
         after_sync();
-        if (warp == 4 * G + 1) tmem_free(tmem, F::kColumns);
+        if (warp == 9) tmem_free(tmem, F::kColumns);
     }
 }
 
@@ -784,17 +659,12 @@ template <typename K> int launch(K kernel, dim3 grid, int threads, int smem, cud
     return HGC_OK;
 }
 
-template <typename T, int CHUNKS> int grad_queries_mma(const Args &a, const Maps &maps, cudaStream_t stream)
+template <typename T, int CHUNKS, bool KEYS> int grad_mma(const Args &a, const Maps &maps, cudaStream_t stream)
 {
-    using F = GradQueries<CHUNKS>;
-    const dim3 grid((unsigned)tile_count(a.n_q, kMmaRows / a.pack, a.n_events), a.heads / a.pack, a.splits);
-    return launch(grad_queries_mma_kernel<T, CHUNKS>, grid, kBlock, F::kSmem, stream, a, maps);
-}
-template <typename T, int CHUNKS> int grad_keys_mma(const Args &a, const Maps &maps, cudaStream_t stream)
-{
-    using F = GradKeys<CHUNKS>;
-    const dim3 grid((unsigned)tile_count(a.n_k, kMmaRows, a.n_events), a.kv_heads, a.splits);
-    return launch(grad_keys_mma_kernel<T, CHUNKS>, grid, F::kThreads, F::kSmem, stream, a, maps);
+    using F = Grad<CHUNKS, KEYS>;
+    const long long tiles = KEYS ? tile_count(a.n_k, kMmaRows, a.n_events) : tile_count(a.n_q, kMmaRows / a.pack, a.n_events);
+    return launch(grad_mma_kernel<T, CHUNKS, KEYS>, dim3((unsigned)tiles, KEYS ? a.kv_heads : a.heads / a.pack, a.splits), F::kThreads, F::kSmem, stream, a,
+                  maps);
 }
 
 template <typename T, int CHUNKS> int forward_mma(const Args &a, const Maps &maps, cudaStream_t stream)
@@ -822,29 +692,20 @@ int mma_forward(const Args &a, int dtype, cudaStream_t stream)
     return a.dim <= 64 ? forward_mma<__nv_bfloat16, 1>(a, maps, stream) : forward_mma<__nv_bfloat16, 2>(a, maps, stream);
 }
 
-int mma_grad_queries(const Args &a, int dtype, cudaStream_t stream)
+template <bool KEYS> static int grad(const Args &a, int dtype, cudaStream_t stream)
 {
     const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
+    const int rows_q = (KEYS ? kMmaGradStep : kMmaRows) / a.pack, rows_k = KEYS ? kMmaRows : kMmaGradStep;
     Maps maps;
-    if (const int rc = map_of(&maps.q, a.q, dtype, a.dim, a.heads, a.n_q, a.pack, kMmaRows / a.pack)) return rc;
-    if (const int rc = map_of(&maps.grad, grad, dtype, a.dim, a.heads, a.n_q, a.pack, kMmaRows / a.pack)) return rc;
-    if (const int rc = map_of(&maps.k, a.k, dtype, a.dim, a.kv_heads, a.n_k, 1, kMmaGradStep)) return rc;
-    if (const int rc = map_of(&maps.v, a.v, dtype, a.dim, a.kv_heads, a.n_k, 1, kMmaGradStep)) return rc;
-    if (dtype == HGC_FLOAT16) return a.dim <= 64 ? grad_queries_mma<__half, 1>(a, maps, stream) : grad_queries_mma<__half, 2>(a, maps, stream);
-    return a.dim <= 64 ? grad_queries_mma<__nv_bfloat16, 1>(a, maps, stream) : grad_queries_mma<__nv_bfloat16, 2>(a, maps, stream);
+    if (const int rc = map_of(&maps.q, a.q, dtype, a.dim, a.heads, a.n_q, a.pack, rows_q)) return rc;
+    if (const int rc = map_of(&maps.grad, grad, dtype, a.dim, a.heads, a.n_q, a.pack, rows_q)) return rc;
+    if (const int rc = map_of(&maps.k, a.k, dtype, a.dim, a.kv_heads, a.n_k, 1, rows_k)) return rc;
+    if (const int rc = map_of(&maps.v, a.v, dtype, a.dim, a.kv_heads, a.n_k, 1, rows_k)) return rc;
+    if (dtype == HGC_FLOAT16) return a.dim <= 64 ? grad_mma<__half, 1, KEYS>(a, maps, stream) : grad_mma<__half, 2, KEYS>(a, maps, stream);
+    return a.dim <= 64 ? grad_mma<__nv_bfloat16, 1, KEYS>(a, maps, stream) : grad_mma<__nv_bfloat16, 2, KEYS>(a, maps, stream);
 }
-
-int mma_grad_keys(const Args &a, int dtype, cudaStream_t stream)
-{
-    const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
-    Maps maps;
-    if (const int rc = map_of(&maps.q, a.q, dtype, a.dim, a.heads, a.n_q, a.pack, kMmaGradStep / a.pack)) return rc;
-    if (const int rc = map_of(&maps.grad, grad, dtype, a.dim, a.heads, a.n_q, a.pack, kMmaGradStep / a.pack)) return rc;
-    if (const int rc = map_of(&maps.k, a.k, dtype, a.dim, a.kv_heads, a.n_k, 1, kMmaRows)) return rc;
-    if (const int rc = map_of(&maps.v, a.v, dtype, a.dim, a.kv_heads, a.n_k, 1, kMmaRows)) return rc;
-    if (dtype == HGC_FLOAT16) return a.dim <= 64 ? grad_keys_mma<__half, 1>(a, maps, stream) : grad_keys_mma<__half, 2>(a, maps, stream);
-    return a.dim <= 64 ? grad_keys_mma<__nv_bfloat16, 1>(a, maps, stream) : grad_keys_mma<__nv_bfloat16, 2>(a, maps, stream);
-}
+int mma_grad_queries(const Args &a, int dtype, cudaStream_t stream) { return grad<false>(a, dtype, stream); }
+int mma_grad_keys(const Args &a, int dtype, cudaStream_t stream) { return grad<true>(a, dtype, stream); }
 
 }  // namespace attn
 }  // namespace hgc

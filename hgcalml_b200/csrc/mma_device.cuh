@@ -12,6 +12,16 @@ namespace mma {
 
 __device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 
+// One thread of a warp, the same one every time; all of the warp's lanes call this together.  Copies, products and their commits
+// are issued by the thread that it elects and by no other means: in a branch that is merely taken by one lane the assembler
+// cannot know that one thread issues, and operands that have to be uniform are gathered lane by lane.
+__device__ __forceinline__ bool elect()
+{
+    unsigned elected;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected) :: "memory");
+    return elected != 0;
+}
+
 // ----------------------------------------------------------------------------------------------------------- barriers
 __device__ __forceinline__ void barrier_init(unsigned bar, unsigned count)
 {
@@ -32,14 +42,9 @@ __device__ __forceinline__ void arrive_expect(unsigned bar, unsigned bytes)
 }
 
 // Waits end: after kPatience, or when another wait of the block has given up, the block's flag is set, every later wait returns
-// and no more copies or products are issued, so that the block runs to its end and frees its tensor memory.
-constexpr unsigned long long kPatience = 4000000000ull;  // ns
-__device__ __forceinline__ unsigned long long now()
-{
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
+// and no more copies or products are issued, so that the block runs to its end and frees its tensor memory.  The clock is looked at
+// only after many tries: a try sleeps until the barrier's phase ends or some time has passed.
+constexpr long long kPatience = 8000000000ll;  // cycles
 __device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity)
 {
     unsigned done;
@@ -47,18 +52,23 @@ __device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity)
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
+__device__ __forceinline__ bool wait_long(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
 {
-    if (try_wait(bar, parity)) return true;
-    const unsigned long long begin = now();
+    const long long begin = clock64();
     do {
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < 64; i++)
             if (try_wait(bar, parity)) return true;
         if (*gave_up) return false;
-    } while (now() - begin < kPatience);
+    } while (clock64() - begin < kPatience);
     *gave_up = 1;
     flag_status(status, HGC_STATUS_ITERATION_CAP);
     return false;
+}
+__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
+{
+    for (int i = 0; i < 16; i++)
+        if (try_wait(bar, parity)) return true;
+    return wait_long(bar, parity, gave_up, status);
 }
 // the same for a warp, whose lanes go on together
 __device__ __forceinline__ bool wait_warp(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
@@ -68,8 +78,8 @@ __device__ __forceinline__ bool wait_warp(unsigned bar, unsigned parity, volatil
 // A wait for what is under way whatever happened before.
 __device__ __forceinline__ void drain(unsigned bar, unsigned parity)
 {
-    const unsigned long long begin = now();
-    while (!try_wait(bar, parity) && now() - begin < kPatience) {}
+    const long long begin = clock64();
+    while (!try_wait(bar, parity) && clock64() - begin < kPatience) {}
 }
 
 // -------------------------------------------------------------------------------------------------------- tile copies
@@ -118,17 +128,24 @@ __device__ __forceinline__ void arrive_when_done(unsigned bar)
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// d[128 x n] (+)= a[128 rows] . b[n rows], both K-major, `steps` times 16 columns; tiles of 64 columns lie a_apart and b_apart bytes
-// behind each other.
-__device__ __forceinline__ void product_along(unsigned d, unsigned a, unsigned a_apart, unsigned b, unsigned b_apart, int steps, unsigned shape)
+// d[128 x n] = a[128 rows] . b[n rows], both K-major, over 16 `steps` columns; tiles of 64 columns lie A_APART and B_APART bytes
+// behind each other.  The thread that issues is a chain of its own, so that all it does per product is to add constants to the
+// operands.
+template <int CHUNKS, unsigned A_APART, unsigned B_APART>
+__device__ __forceinline__ void product_along(unsigned d, unsigned a, unsigned b, int steps, unsigned shape)
 {
-    for (int k = 0; k < steps; k++)
-        product(d, operand(a + (k >> 2) * a_apart + (k & 3) * 32, 16), operand(b + (k >> 2) * b_apart + (k & 3) * 32, 16), shape, k > 0);
+    const unsigned long long oa = operand(a, 16), ob = operand(b, 16);
+#pragma unroll
+    for (int k = 0; k < 4 * CHUNKS; k++)
+        if (k < steps) product(d, oa + (k / 4 * A_APART + k % 4 * 32) / 16, ob + (k / 4 * B_APART + k % 4 * 32) / 16, shape, k > 0);
 }
-// d[128 x columns] (+)= a[128 x 16 steps, in tensor memory] b[16 steps rows], tiles of 64 columns `apart` bytes behind each other
-__device__ __forceinline__ void product_over(unsigned d, unsigned a, unsigned b, unsigned apart, int steps, unsigned shape, bool add)
+// d[128 x columns] (+)= a[128 x 16 STEPS, in tensor memory] b[16 STEPS rows], tiles of 64 columns APART bytes behind each other
+template <int STEPS, unsigned APART>
+__device__ __forceinline__ void product_over(unsigned d, unsigned a, unsigned b, unsigned shape, bool add)
 {
-    for (int k = 0; k < steps; k++) product_from_tmem(d, a + 8 * k, operand(b + 2048 * k, apart), shape, add || k > 0);
+    const unsigned long long ob = operand(b, APART);
+#pragma unroll
+    for (int k = 0; k < STEPS; k++) product_from_tmem(d, a + 8 * k, ob + 2048 / 16 * k, shape, add || k > 0);
 }
 
 // ------------------------------------------------------------------------------------------------------ tensor memory
@@ -176,6 +193,38 @@ __device__ __forceinline__ float exp2_fast(float x)  // relative error 2^-22
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Pairs of floats: one instruction for both.
+typedef unsigned long long pair;
+__device__ __forceinline__ pair pair_of(float a, float b)
+{
+    pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts(pair a)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c)
+{
+    pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ pair add2(pair a, pair b)
+{
+    pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ pair mul2(pair a, pair b)
+{
+    pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 // two floats rounded to 16 bits, the first in the lower half
 template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
