@@ -516,7 +516,7 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
     p.splits = split_count(filled(n_q, m) * (heads / p.pack), steps_k, 4, 4);
     const int mma_tokens = kMmaRows / p.pack;
-    p.splits_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 4, 2);
+    p.splits_mma = split_count(filled(n_q, 2 * mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 2, 2);
     p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
     p.splits_q_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / kMmaGradStep, 4, 4);
     p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);

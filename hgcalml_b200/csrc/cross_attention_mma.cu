@@ -1,9 +1,7 @@
 // Attention between two ragged sets of rows on the tensor cores, for 16-bit types.
 //
-// A block has 128 rows of queries (tokens times the heads that share a key head) and takes them through the keys of their event.
-// Six warps: four hold a row of scores per lane and do the softmax, one copies keys and values, one issues the products.
-// Scores S = Q K^T, weights P (16 bits) and sums O = P V live in tensor memory, 256 columns, so that two blocks share a
-// multiprocessor and one's softmax runs under the other's products.
+// Blocks of twelve warps have a multiprocessor each.  Eight of them do the elementwise work on rows of tensor memory, four keep them
+// fed: copies, products of scores, products of sums, rows to clear.  They meet at barriers in shared memory only.
 #include <cuda.h>
 #include <atomic>
 
@@ -16,7 +14,6 @@ namespace {
 
 using namespace mma;
 
-constexpr int kBlock = 192;  // warps 0 to 3: rows; 4: copies; 5: products
 constexpr int kTile = 64 * 2;  // bytes of a row of a tile in shared memory
 
 struct Maps {
@@ -53,138 +50,195 @@ __device__ __forceinline__ void clear_unseen(unsigned tile, int chunks, const un
     }
 }
 
+// 16 columns of a row of a result
+template <typename T>
+__device__ __forceinline__ void store16(void *to, float *part, long long at, int d, int dim, const unsigned (&v)[16], float factor)
+{
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = __uint_as_float(v[i]) * factor;
+    if (part != nullptr) {
+        float4 *p = reinterpret_cast<float4 *>(part + at + d);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (d + 4 * i < dim) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    } else {
+        uint4 *p = reinterpret_cast<uint4 *>(static_cast<T *>(to) + at + d);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (d + 8 * i < dim)
+                p[i] = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]), pack2<T>(x[8 * i + 4], x[8 * i + 5]),
+                                  pack2<T>(x[8 * i + 6], x[8 * i + 7]));
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------- forward
+// A block has two tiles of 128 rows of queries, each with four warps that do its softmax (a row per lane), and takes them through
+// the keys of their event, kKeys a step.  Scores S = Q K^T and, in their place, weights P (16 bits) are in buffers of tensor memory
+// that the tiles use in turn, so that the next scores are done when a softmax ends; the sums O = P V lie beside them.  Four more warps
+// copy keys and values, issue scores, issue sums, and clear what must not be summed.
 template <int CHUNKS> struct Forward {
-    static constexpr int kKeys = CHUNKS == 1 ? 128 : 64;  // of a step
-    static constexpr int kStages = 2, kBarriers = 1 + 4 * kStages + 4;
-    static constexpr int kTileBytes = kKeys * kTile * CHUNKS;
-    static constexpr int kQueryBytes = kMmaRows * kTile * CHUNKS;
-    static constexpr int kSmem = kQueryBytes + 2 * kStages * kTileBytes;
-    // columns of tensor memory
-    static constexpr int kScores = 0, kWeights = kKeys, kOut = CHUNKS == 1 ? 192 : 128, kColumns = 256;
+    static constexpr int kKeys = CHUNKS == 1 ? 128 : 64, kStages = 5, kThreads = 384;
+    static constexpr int kTileBytes = kKeys * kTile * CHUNKS, kQueryBytes = kMmaRows * kTile * CHUNKS;
+    static constexpr int kBuffers = CHUNKS == 1 ? 3 : 4, kOut = kKeys * kBuffers, kColumns = 512;
+    static constexpr int kTiles = 2 * kQueryBytes + 2 * kStages * kTileBytes, kSmem = kTiles + 512;
+    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers + 2;
+    static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 512, "room");
 };
 
 template <typename T, int CHUNKS>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(Forward<CHUNKS>::kThreads, 1)
 forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps)
 {
     pdl_begin();
     using F = Forward<CHUNKS>;
-    constexpr int N = F::kKeys, W = N / 32;
+    constexpr int N = F::kKeys, W = N / 32, B = F::kBuffers;
     extern __shared__ __align__(1024) char s_raw[];
-    __shared__ __align__(8) unsigned long long s_bar[F::kBarriers];
-    __shared__ unsigned s_tmem;
-    __shared__ int s_gave_up;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int tokens = kMmaRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_splits(a, t, kBlock);
-    const Tile tile = find_tile(a.rs_q, a.n_q, a.n_events, tokens, blockIdx.x);
+    const int tokens = kMmaRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;  // tokens of one of the two tiles
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_splits(a, t, F::kThreads);
+    const Tile tile = find_tile(a.rs_q, a.n_q, a.n_events, 2 * tokens, blockIdx.x);
     if (tile.begin >= tile.end) return;
-    const int n_rows = (tile.end - tile.begin) * a.pack;
+    const int groups = tile.end - tile.begin > tokens ? 2 : 1;
     const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
     const int2 part = part_of(max(0, (keys.y - keys.x + N - 1) / N), blockIdx.z, a.splits);
     const int steps = part.y - part.x, first = keys.x + part.x * N;
+    // steps from this one on have keys that are masked, or of another event
+    const int dirty = a.mask != nullptr ? 0 : (keys.y - first) / N;
 
-    const unsigned s_q = smem_address(s_raw), s_k = s_q + F::kQueryBytes, s_v = s_k + F::kStages * F::kTileBytes;
-    const unsigned bar = smem_address(s_bar), q_full = bar, k_full = bar + 8, k_empty = k_full + 8 * F::kStages, v_full = k_empty + 8 * F::kStages,
-                   v_empty = v_full + 8 * F::kStages, s_full = v_empty + 8 * F::kStages, p_full = s_full + 8, o_full = p_full + 8,
-                   all_done = o_full + 8;
+    const unsigned s_q = smem_address(s_raw), s_k = s_q + 2 * F::kQueryBytes, s_v = s_k + F::kStages * F::kTileBytes;
+    const unsigned bar = s_q + F::kTiles, q_full = bar, scores_done = bar + 8, sums_done = scores_done + 8, full = sums_done + 8,
+                   empty = full + 8 * F::kStages, clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B,
+                   used = p_full + 8 * B, o_full = used + 8 * B;
+    unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + 8 * F::kBarriers);
+    volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
     if (steps > 0) {
         if (t == 0) {
-            for (int i = 0; i < F::kBarriers; i++) barrier_init(bar + 8 * i, bar + 8 * i == p_full ? 4 : 1);
+            for (int i = 0; i < F::kBarriers; i++) {
+                const unsigned at = bar + 8 * i;
+                barrier_init(at, at >= p_full && at < used ? 4 : 1);
+            }
             barrier_init_done();
-            s_gave_up = 0;
+            *gave_up = 0;
         }
-        if (warp == 5) tmem_alloc(&s_tmem, F::kColumns);
+        if (warp == 11) tmem_alloc(s_tmem, F::kColumns);
         before_sync();
         __syncthreads();
         after_sync();
     }
-    volatile int *gave_up = &s_gave_up;
-    const unsigned tmem = steps > 0 ? s_tmem : 0;
+    const unsigned tmem = steps > 0 ? *s_tmem : 0;
 
-    if (warp == 4) {
+    if (warp == 8) {
         if (steps > 0 && elect()) {
-            arrive_expect(q_full, CHUNKS * kTile * a.pack * tokens);
-            for (int c = 0; c < CHUNKS; c++) copy_box(s_q + c * kMmaRows * kTile, &maps.q, q_full, 64 * c, head0, tile.begin);
-            int k_copies = 0, v_copies = 0;
+            arrive_expect(q_full, groups * CHUNKS * kTile * a.pack * tokens);
+            for (int g = 0; g < groups; g++)
+                for (int c = 0; c < CHUNKS; c++)
+                    copy_box(s_q + g * F::kQueryBytes + c * kMmaRows * kTile, &maps.q, q_full, 64 * c, head0, tile.begin + g * tokens);
+            int copies = 0;
             for (int j = 0; j < steps; j++) {
                 const int stage = j % F::kStages;
-                const unsigned again = (j / F::kStages & 1) ^ 1;
-                if (j >= F::kStages && !wait(k_empty + 8 * stage, again, gave_up, a.status)) break;
-                arrive_expect(k_full + 8 * stage, F::kTileBytes);
-                for (int c = 0; c < CHUNKS; c++)
-                    copy_box(s_k + stage * F::kTileBytes + c * N * kTile, &maps.k, k_full + 8 * stage, 64 * c, kv, first + j * N);
-                k_copies++;
-                if (j >= F::kStages && !wait(v_empty + 8 * stage, again, gave_up, a.status)) break;
-                arrive_expect(v_full + 8 * stage, F::kTileBytes);
-                for (int c = 0; c < CHUNKS; c++)
-                    copy_box(s_v + stage * F::kTileBytes + c * N * kTile, &maps.v, v_full + 8 * stage, 64 * c, kv, first + j * N);
-                v_copies++;
+                if (j >= F::kStages && !wait(empty + 8 * stage, (j / F::kStages & 1) ^ 1, gave_up, a.status)) break;
+                arrive_expect(full + 8 * stage, 2 * F::kTileBytes);
+                for (int c = 0; c < CHUNKS; c++) {
+                    copy_box(s_k + stage * F::kTileBytes + c * N * kTile, &maps.k, full + 8 * stage, 64 * c, kv, first + j * N);
+                    copy_box(s_v + stage * F::kTileBytes + c * N * kTile, &maps.v, full + 8 * stage, 64 * c, kv, first + j * N);
+                }
+                copies++;
             }
             // no copy is under way when the block leaves
             drain(q_full, 0);
-            for (int j = max(0, k_copies - F::kStages); j < k_copies; j++) drain(k_full + 8 * (j % F::kStages), j / F::kStages & 1);
-            for (int j = max(0, v_copies - F::kStages); j < v_copies; j++) drain(v_full + 8 * (j % F::kStages), j / F::kStages & 1);
+            for (int j = max(0, copies - F::kStages); j < copies; j++) drain(full + 8 * (j % F::kStages), j / F::kStages & 1);
         }
         __syncwarp();
-    } else if (warp == 5) {
-        const int depth = (a.dim + 15) / 16;
-        const unsigned shape_s = shape<T>(N, false), shape_o = shape<T>(16 * depth, true);
-        // scores of step j
-        const auto scores = [&](int j) {
-            const int stage = j % F::kStages;
-            const bool ok = wait_warp(k_full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
-            after_sync();
-            if (ok && elect()) {
-                product_along<CHUNKS, kMmaRows * kTile, N * kTile>(tmem + F::kScores, s_q, s_k + stage * F::kTileBytes, depth, shape_s);
-                arrive_when_done(s_full);
-                arrive_when_done(k_empty + 8 * stage);
-            }
-            __syncwarp();
-        };
-        if (steps > 0 && wait_warp(q_full, 0, gave_up, a.status)) {
-            scores(0);
-            for (int j = 0; j < steps; j++) {
-                const int stage = j % F::kStages;
-                unsigned seen[W];
-                const bool all = seen_words<W>(seen, a.mask, first + j * N, keys.y - (first + j * N));
-                if (!wait_warp(v_full + 8 * stage, j / F::kStages & 1, gave_up, a.status)) break;
-                if (!all) {
-                    clear_unseen<W>(s_v + stage * F::kTileBytes, CHUNKS, seen);
-                    writes_before_products();
-                    __syncwarp();
+    } else if (warp == 9) {
+        if (steps > 0 && elect()) {
+            const int depth = (a.dim + 15) / 16;
+            const unsigned shape_s = shape<T>(N, false);
+            bool ok = wait(q_full, 0, gave_up, a.status);
+            int stage = 0, b = 0;
+            unsigned turn = 0, turn_b = 1;
+            for (int j = 0, i = 0; j < steps && ok; j++) {
+                ok = wait(full + 8 * stage, turn, gave_up, a.status);
+                for (int g = 0; g < groups && ok; g++, i++) {
+                    if (i >= B) ok = wait(used + 8 * b, turn_b, gave_up, a.status);
+                    after_sync();
+                    if (ok) {
+                        product_along<CHUNKS, kMmaRows * kTile, N * kTile>(tmem + N * b, s_q + g * F::kQueryBytes, s_k + stage * F::kTileBytes, depth, shape_s);
+                        arrive_when_done(s_full + 8 * b);
+                    }
+                    if (++b == B) b = 0, turn_b ^= 1;
                 }
-                if (!wait_warp(p_full, j & 1, gave_up, a.status)) break;
-                after_sync();
-                if (j + 1 < steps) scores(j + 1);
-                if (elect()) {
-                    product_over<N / 16, N * kTile>(tmem + F::kOut, tmem + F::kWeights, s_v + stage * F::kTileBytes, shape_o, j > 0);
-                    arrive_when_done(o_full);
-                    arrive_when_done(v_empty + 8 * stage);
+                if (++stage == F::kStages) stage = 0, turn ^= 1;
+            }
+            arrive_when_done(scores_done);  // no product is under way when the tensor memory is freed
+            drain(scores_done, 0);
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        if (steps > 0 && elect()) {
+            const unsigned shape_o = shape<T>((a.dim + 15) / 16 * 16, true);
+            int stage = 0, b = 0;
+            unsigned turn = 0, turn_b = 0;
+            bool ok = true;
+            for (int j = 0; j < steps && ok; j++) {
+                if (dirty < steps) ok = wait(clean + 8 * stage, turn, gave_up, a.status);
+                for (int g = 0; g < groups && ok; g++) {
+                    ok = wait(p_full + 8 * b, turn_b, gave_up, a.status);
+                    after_sync();
+                    if (ok) {
+                        product_over<N / 16, N * kTile>(tmem + F::kOut + 64 * CHUNKS * g, tmem + N * b, s_v + stage * F::kTileBytes, shape_o, j > 0);
+                        arrive_when_done(used + 8 * b);
+                        arrive_when_done(o_full + 8 * g);
+                    }
+                    if (++b == B) b = 0, turn_b ^= 1;
                 }
-                __syncwarp();
+                if (ok) arrive_when_done(empty + 8 * stage);
+                if (++stage == F::kStages) stage = 0, turn ^= 1;
             }
-            if (elect()) {  // no product is under way when the tensor memory is freed
-                arrive_when_done(all_done);
-                drain(all_done, 0);
-            }
+            arrive_when_done(sums_done);
+            drain(sums_done, 0);
+        }
+        __syncwarp();
+    } else if (warp == 11) {
+        // where there is anything to clear, every step passes through here: a wait tells only two rounds of a stage apart
+        for (int j = dirty < steps ? 0 : steps; j < steps; j++) {
+            const int stage = j % F::kStages, k0 = first + j * N;
+            unsigned seen[W];
+            const bool all = j < dirty || seen_words<W>(seen, a.mask, k0, keys.y - k0);
+            if (!wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)) break;
+            if (!all) clear_unseen<W>(s_v + stage * F::kTileBytes, CHUNKS, seen);
+            writes_before_products();
             __syncwarp();
+            if (lane == 0) arrive(clean + 8 * stage);
         }
     } else {
-        const unsigned rows = tmem + ((unsigned)warp << 21);  // lane 32 w of tensor memory
-        const bool idle = warp * 32 >= n_rows;                // none of the warp's rows counts
+        const int g = warp >> 2, r = t & 127;
+        const int n_rows = min(tokens, tile.end - tile.begin - g * tokens) * a.pack;
+        const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21), out = lanes + F::kOut + 64 * CHUNKS * g;
+        const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;  // idle: none of the warp's rows counts
         const float c = a.scale * kLog2e;
+        const pair c2 = pair_of(c, c);
         float top = -INFINITY, sum = 0.f;
-        for (int j = 0; j < steps; j++) {
-            unsigned seen[W];
-            const bool all = seen_words<W>(seen, a.mask, first + j * N, keys.y - (first + j * N));
-            if (!wait_warp(s_full, j & 1, gave_up, a.status)) break;
-            after_sync();
+        int b = g;
+        unsigned turn = 0, seen[W];
+        bool all = dirty > 0;
+        if (!all && g < groups && steps > 0) all = seen_words<W>(seen, a.mask, first, keys.y - first);
+        for (int j = 0; j < steps && g < groups; j++) {
+            const unsigned rows = lanes + N * b;
+            // whether the keys of the next step can be seen, asked for ahead of their time
+            unsigned char ahead[W];
+            const int next_key = first + (j + 1) * N, next_n = j + 1 < steps && j + 1 >= dirty ? keys.y - next_key : 0;
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                ahead[w] = 32 * w + lane < next_n ? a.mask == nullptr ? 1 : fresh(a.mask + next_key + 32 * w + lane) : 0;
+            if (!wait_warp(s_full + 8 * b, turn, gave_up, a.status)) break;
+            // every phase of the sums' barrier is waited for: here, where they are scaled, else when this step's weights are done
+            bool summed = j == 0;
             if (!idle) {
+                after_sync();
                 unsigned s[W][32];
 #pragma unroll
-                for (int w = 0; w < W; w++) tmem_load32(s[w], rows + F::kScores + 32 * w);
+                for (int w = 0; w < W; w++) tmem_load32(s[w], rows + 32 * w);
                 tmem_loaded();
 #pragma unroll
                 for (int w = 0; w < W; w++) use_after(s[w]);
@@ -199,85 +253,84 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
 #pragma unroll
                 for (int w = 0; w < W; w++)
 #pragma unroll
-                    for (int i = 0; i < 32; i++) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(s[w][i]));
+                    for (int i = 0; i < 32; i += 2)
+                        m[(i >> 1) & 3] = fmaxf(m[(i >> 1) & 3], fmaxf(__uint_as_float(s[w][i]), __uint_as_float(s[w][i + 1])));
                 const float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                if (j > 0 && !wait_warp(o_full, (j - 1) & 1, gave_up, a.status)) break;
-                // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that
-                // lose nothing in either type.
+                // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing in
+                // either type.
                 const bool grown = (next - top) * c > 8.f;
-                if (j == 0) top = next;
-                else if (__any_sync(0xffffffffu, grown)) {
+                if (j == 0) {
+                    top = next;
+                } else if (__any_sync(0xffffffffu, grown)) {
+                    if (!wait_warp(o_full + 8 * g, (j - 1) & 1, gave_up, a.status)) break;
+                    summed = true;
                     after_sync();
                     const float shrink = exp2_fast((top - (next == -INFINITY ? 0.f : next)) * c);
                     top = next;
                     sum *= shrink;
                     for (int d = 0; d < a.dim; d += 16) {
                         unsigned o[16];
-                        tmem_load16(o, rows + F::kOut + d);
+                        tmem_load16(o, out + d);
                         tmem_loaded();
                         use_after(o);
 #pragma unroll
                         for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-                        tmem_store16(rows + F::kOut + d, o);
+                        tmem_store16(out + d, o);
                     }
                 }
                 const float base = (top == -INFINITY ? 0.f : top) * c;
-                float part_sum[4] = {};
+                const pair base2 = pair_of(-base, -base);
+                pair sums[2] = {0, 0};
 #pragma unroll
                 for (int w = 0; w < W; w++) {
                     unsigned p[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float x = exp2_fast(fmaf(__uint_as_float(s[w][2 * i]), c, -base)), y = exp2_fast(fmaf(__uint_as_float(s[w][2 * i + 1]), c, -base));
-                        part_sum[i & 3] += x + y;
-                        p[i] = pack2<T>(x, y);
+                        const float2 x = parts(fma2(pair_of(__uint_as_float(s[w][2 * i]), __uint_as_float(s[w][2 * i + 1])), c2, base2));
+                        const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        sums[i & 1] = add2(sums[i & 1], pair_of(e.x, e.y));
+                        p[i] = pack2<T>(e.x, e.y);
                     }
-                    tmem_store16(rows + F::kWeights + 16 * w, p);
+                    tmem_store16(rows + 16 * w, p);
                 }
-                sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+                const float2 both = parts(add2(sums[0], sums[1]));
+                sum += both.x + both.y;
                 tmem_stored();
-            } else if (j > 0 && !wait_warp(o_full, (j - 1) & 1, gave_up, a.status)) {
-                break;
             }
+            if (!summed && !wait_warp(o_full + 8 * g, (j - 1) & 1, gave_up, a.status)) break;
             before_sync();
             __syncwarp();
-            if (lane == 0) arrive(p_full);
+            if (lane == 0) arrive(p_full + 8 * b);
+            if (j + 1 >= dirty) {
+                all = next_n >= N;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    seen[w] = __ballot_sync(0xffffffffu, ahead[w] != 0);
+                    all = all && seen[w] == 0xffffffffu;
+                }
+            }
+            b += groups;
+            if (b >= B) b -= B, turn ^= 1;
         }
-        const bool done = steps > 0 && wait_warp(o_full, (steps - 1) & 1, gave_up, a.status);
+        const bool done = steps > 0 && g < groups && wait_warp(sums_done, 0, gave_up, a.status);
         if (done) after_sync();
-        const int r = t;
-        const bool store = r < n_rows;
-        const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
+        const long long row = (long long)(tile.begin + g * tokens + r / a.pack) * a.heads + head0 + r % a.pack;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const long long all_rows = (long long)a.n_q * a.heads;
         if (store) {
             float *lse = a.splits > 1 ? a.part_lse + blockIdx.z * all_rows : a.lse;
             lse[row] = sum == 0.f ? -INFINITY : top * a.scale + logf(sum);
         }
-        if (!idle)
+        float *to_part = a.splits > 1 ? a.part + blockIdx.z * all_rows * a.dim : nullptr;
+        if (!idle && (done || a.splits == 1))  // a part without keys has no weight
             for (int d = 0; d < a.dim; d += 16) {
-                unsigned o[16];
+                unsigned o[16] = {};
                 if (done) {
-                    tmem_load16(o, rows + F::kOut + d);
+                    tmem_load16(o, out + d);
                     tmem_loaded();
                     use_after(o);
                 }
-                float v[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) v[i] = done ? __uint_as_float(o[i]) * inv : 0.f;
-                if (store && a.splits > 1 && done) {  // a part without keys has no weight
-                    float4 *to = reinterpret_cast<float4 *>(a.part + (blockIdx.z * all_rows + row) * a.dim + d);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (d + 4 * i < a.dim) to[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                } else if (store && a.splits == 1) {
-                    uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(a.to) + row * a.dim + d);
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        if (d + 8 * i < a.dim)
-                            to[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]), pack2<T>(v[8 * i + 4], v[8 * i + 5]),
-                                               pack2<T>(v[8 * i + 6], v[8 * i + 7]));
-                }
+                if (store) store16<T>(a.to, to_part, row * a.dim, d, a.dim, o, inv);
                 __syncwarp();
             }
     }
@@ -285,7 +338,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
         before_sync();
         __syncthreads();
         after_sync();
-        if (warp == 5) tmem_free(tmem, F::kColumns);
+        if (warp == 11) tmem_free(tmem, F::kColumns);
     }
 }
 
@@ -311,41 +364,21 @@ __device__ __forceinline__ void clear_rows(unsigned tile, int chunks, int tile_r
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" :: "r"(tile + c * tile_rows * kTile + i * 16), "r"(0) : "memory");
 }
 
-// 16 columns of a row of a gradient
-template <typename T>
-__device__ __forceinline__ void store16(void *to, float *part, long long at, int d, int dim, const unsigned (&v)[16], float factor)
-{
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = __uint_as_float(v[i]) * factor;
-    if (part != nullptr) {
-        float4 *p = reinterpret_cast<float4 *>(part + at + d);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (d + 4 * i < dim) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-    } else {
-        uint4 *p = reinterpret_cast<uint4 *>(static_cast<T *>(to) + at + d);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (d + 8 * i < dim)
-                p[i] = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]), pack2<T>(x[8 * i + 4], x[8 * i + 5]),
-                                  pack2<T>(x[8 * i + 6], x[8 * i + 7]));
-    }
-}
-
 // Both gradients are the same walk.  A block keeps 128 rows of two tensors (KEYS: keys and values, else queries and grad) and the
 // rows of the two others of the event pass by, 64 a step:
 //   KEYS: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q;  else S = Q K^T, dP = dO V^T, dQ += dS K
 // with a kept row per lane.  P and dS (16 bits) take the places of S and dP in tensor memory, from where they are an operand of the
 // sums.  One block has a multiprocessor and all 512 columns: the sums, and as many buffers for S and dP as there is room for, so
-// that two groups of four warps, which take the steps in turn, find the next step's scores done.
+// that two groups of four warps, which take the steps in turn, find the next step's scores done.  What bounds a step is how fast
+// products can be issued (about 36 cycles each, 12 or 16 a step) and the exponentials (512 cycles), so scores and sums are issued by a
+// thread each, that does nothing else, and rows that must not be summed over are cleared by a warp of their own.
 // (Two blocks of 256 columns, each with one buffer, waited for products two thirds of the time: 16k x 16k rows, 8 heads of 64, 3.2 ms.)
 template <int CHUNKS, bool KEYS> struct Grad {
-    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 320;
+    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 384;
     static constexpr int kTileBytes = kStep * kTile * CHUNKS, kKeptBytes = kMmaRows * kTile * CHUNKS;
     static constexpr int kBuffers = KEYS && CHUNKS == 2 ? 2 : 3, kSums = 128 * kBuffers, kSums2 = kSums + 64 * CHUNKS, kColumns = 512;
     static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 2 * 2 * kStep * 4, kSmem = kTiles + kStats + 256;
-    static constexpr int kBarriers = 2 + 2 * kStages + 3 * kBuffers;
+    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers;
     static_assert((KEYS ? kSums2 : kSums) + 64 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 256, "room");
 };
 
@@ -369,27 +402,27 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
     if (!KEYS && !varies) others.y = others.x;
     const int rows_a_step = KEYS ? tokens : N;
     const int2 part = part_of(max(0, (others.y - others.x + rows_a_step - 1) / rows_a_step), blockIdx.z, a.splits);
-    const int first_step = part.x * packs, steps = part.y * packs - first_step;
-    // first row (of a head, or packed heads) of a step
-    const auto row_of = [&](int j) { return others.x + (first_step + j) / packs * rows_a_step; };
-    const auto head_of = [&](int j) { return KEYS ? kv * a.group + (first_step + j) % packs * a.pack : kv; };
+    const int steps = (part.y - part.x) * packs, first_row = others.x + part.x * rows_a_step;
+    // Steps from this one on hold rows that must not be summed over: of another event, or keys that are masked.
+    const int whole = (others.y - others.x) / rows_a_step;  // steps, of one head
+    const int dirty = !KEYS && a.mask != nullptr ? 0 : max(0, (min(part.y, max(whole, part.x)) - part.x) * packs);
 
     const unsigned s_kept = smem_address(s_raw), s_kept2 = s_kept + F::kKeptBytes, s_step = s_kept2 + F::kKeptBytes,
                    s_step2 = s_step + F::kStages * F::kTileBytes;
-    const unsigned bar = s_kept + F::kTiles + F::kStats, kept_full = bar, all_done = bar + 8, full = all_done + 8, empty = full + 8 * F::kStages,
-                   s_full = empty + 8 * F::kStages, p_full = s_full + 8 * B, used = p_full + 8 * B;
+    const unsigned bar = s_kept + F::kTiles + F::kStats, kept_full = bar, scores_done = bar + 8, all_done = scores_done + 8, full = all_done + 8,
+                   empty = full + 8 * F::kStages, clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B, used = p_full + 8 * B;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + F::kStats + 8 * F::kBarriers);
     volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
     if (steps > 0) {
         if (t == 0) {
             for (int i = 0; i < F::kBarriers; i++) {
                 const unsigned at = bar + 8 * i;
-                barrier_init(at, at >= p_full && at < used ? 4 : 1);
+                barrier_init(at, at >= p_full && at < used ? 4 : at == kept_full ? 2 : 1);
             }
             barrier_init_done();
             *gave_up = 0;
         }
-        if (warp == 9) tmem_alloc(s_tmem, F::kColumns);
+        if (warp == 11) tmem_alloc(s_tmem, F::kColumns);
         before_sync();
         __syncthreads();
         after_sync();
@@ -404,16 +437,20 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
                 copy_box(s_kept + c * kMmaRows * kTile, KEYS ? &maps.k : &maps.q, kept_full, 64 * c, kept_head, tile.begin);
                 copy_box(s_kept2 + c * kMmaRows * kTile, KEYS ? &maps.v : &maps.grad, kept_full, 64 * c, kept_head, tile.begin);
             }
-            int copies = 0;
+            int copies = 0, row = first_row, p = 0;
             for (int j = 0; j < steps; j++) {
-                const int stage = j % F::kStages;
+                const int stage = j % F::kStages, head = KEYS ? kv * a.group + p * a.pack : kv;
                 if (j >= F::kStages && !wait(empty + 8 * stage, (j / F::kStages & 1) ^ 1, gave_up, a.status)) break;
                 arrive_expect(full + 8 * stage, KEYS ? 2 * CHUNKS * kTile * a.pack * tokens : 2 * F::kTileBytes);
                 for (int c = 0; c < CHUNKS; c++) {
-                    copy_box(s_step + stage * F::kTileBytes + c * N * kTile, KEYS ? &maps.q : &maps.k, full + 8 * stage, 64 * c, head_of(j), row_of(j));
-                    copy_box(s_step2 + stage * F::kTileBytes + c * N * kTile, KEYS ? &maps.grad : &maps.v, full + 8 * stage, 64 * c, head_of(j), row_of(j));
+                    copy_box(s_step + stage * F::kTileBytes + c * N * kTile, KEYS ? &maps.q : &maps.k, full + 8 * stage, 64 * c, head, row);
+                    copy_box(s_step2 + stage * F::kTileBytes + c * N * kTile, KEYS ? &maps.grad : &maps.v, full + 8 * stage, 64 * c, head, row);
                 }
                 copies++;
+                if (++p == packs) {
+                    p = 0;
+                    row += rows_a_step;
+                }
             }
             // no copy is under way when the block leaves
             drain(kept_full, 0);
@@ -421,78 +458,76 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         }
         __syncwarp();
     } else if (warp == 9) {
-        const int depth = (a.dim + 15) / 16;
-        const unsigned shape_s = shape<T>(N, false), shape_o = shape<T>(16 * depth, true);
-        const auto scores = [&](int j) {
-            const int stage = j % F::kStages;
+        if (steps > 0 && elect()) {
+            const int depth = (a.dim + 15) / 16;
+            const unsigned shape_s = shape<T>(N, false);
+            bool ok = wait(kept_full, 0, gave_up, a.status);
+            int stage = 0, b = 0;
+            unsigned turn = 0, turn_b = 1;  // of the stages; of the buffers, which are free at first
+            for (int j = 0; j < steps && ok; j++) {
+                ok = wait(full + 8 * stage, turn, gave_up, a.status);
+                if (dirty < steps) ok = ok && wait(clean + 8 * stage, turn, gave_up, a.status);
+                if (j >= B) ok = ok && wait(used + 8 * b, turn_b, gave_up, a.status);
+                after_sync();
+                if (ok) {
+                    const unsigned to = tmem + 128 * b;
+                    product_along<CHUNKS, kMmaRows * kTile, N * kTile>(to, s_kept, s_step + stage * F::kTileBytes, depth, shape_s);
+                    product_along<CHUNKS, kMmaRows * kTile, N * kTile>(to + 64, s_kept2, s_step2 + stage * F::kTileBytes, depth, shape_s);
+                    arrive_when_done(s_full + 8 * b);
+                }
+                if (++stage == F::kStages) stage = 0, turn ^= 1;
+                if (++b == B) b = 0, turn_b ^= 1;
+            }
+            arrive_when_done(scores_done);  // no product is under way when the tensor memory is freed
+            drain(scores_done, 0);
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        if (steps > 0 && elect()) {
+            const unsigned shape_o = shape<T>((a.dim + 15) / 16 * 16, true);
+            int stage = 0, b = 0;
+            unsigned turn_b = 0;
+            for (int j = 0; j < steps; j++) {
+                if (!wait(p_full + 8 * b, turn_b, gave_up, a.status)) break;
+                after_sync();
+                const unsigned from = tmem + 128 * b;
+                if (KEYS) product_over<N / 16, N * kTile>(tmem + F::kSums2, from, s_step2 + stage * F::kTileBytes, shape_o, j > 0);
+                product_over<N / 16, N * kTile>(tmem + F::kSums, from + 64, s_step + stage * F::kTileBytes, shape_o, j > 0);
+                arrive_when_done(used + 8 * b);
+                arrive_when_done(empty + 8 * stage);
+                if (++stage == F::kStages) stage = 0;
+                if (++b == B) b = 0, turn_b ^= 1;
+            }
+            arrive_when_done(all_done);
+            drain(all_done, 0);
+        }
+        __syncwarp();
+    } else if (warp == 11) {
+        if (KEYS && steps > 0 && a.pack * tokens < N) {  // rows that no copy writes
+            for (int i = 0; i < F::kStages; i++) {
+                clear_rows(s_step + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
+                clear_rows(s_step2 + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
+            }
+        }
+        writes_before_products();
+        __syncwarp();
+        if (lane == 0 && steps > 0) arrive(kept_full);
+        // Where there is anything to clear, every step passes through here: a wait tells only two rounds of a stage apart.
+        for (int j = dirty < steps ? 0 : steps; j < steps; j++) {
+            const int stage = j % F::kStages, row = first_row + j / packs * rows_a_step;
             const unsigned step = s_step + stage * F::kTileBytes, step2 = s_step2 + stage * F::kTileBytes;
-            bool ok;
-            if (KEYS) {
-                // rows of another event are not summed over, whatever they hold
-                const int n = min(tokens, others.y - row_of(j)) * a.pack;
-                ok = wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
-                if (ok && n < a.pack * tokens) {
-                    clear_rows(step, CHUNKS, N, n, a.pack * tokens);
-                    clear_rows(step2, CHUNKS, N, n, a.pack * tokens);
-                    writes_before_products();
-                    __syncwarp();
-                }
-            } else {
-                unsigned seen[W];
-                const bool all = seen_words<W>(seen, a.mask, row_of(j), others.y - row_of(j));
-                ok = wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status);
-                if (ok && !all) {
-                    clear_unseen<W>(step, CHUNKS, seen);
-                    writes_before_products();
-                    __syncwarp();
-                }
+            unsigned seen[W];
+            const bool all = KEYS || j < dirty || seen_words<W>(seen, a.mask, row, others.y - row);
+            if (!wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)) break;
+            if (KEYS && j >= dirty) {
+                clear_rows(step, CHUNKS, N, (others.y - row) * a.pack, a.pack * tokens);
+                clear_rows(step2, CHUNKS, N, (others.y - row) * a.pack, a.pack * tokens);
+            } else if (!all) {
+                clear_unseen<W>(step, CHUNKS, seen);
             }
-            after_sync();
-            if (ok && elect()) {
-                const unsigned to = tmem + 128 * (j % B);
-                product_along<CHUNKS, kMmaRows * kTile, N * kTile>(to, s_kept, step, depth, shape_s);
-                product_along<CHUNKS, kMmaRows * kTile, N * kTile>(to + 64, s_kept2, step2, depth, shape_s);
-                arrive_when_done(s_full + 8 * (j % B));
-            }
+            writes_before_products();
             __syncwarp();
-        };
-        if (steps > 0) {
-            if (KEYS && a.pack * tokens < N) {  // rows that no copy writes
-                for (int i = 0; i < F::kStages; i++) {
-                    clear_rows(s_step + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
-                    clear_rows(s_step2 + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
-                }
-                writes_before_products();
-                __syncwarp();
-            }
-            if (wait_warp(kept_full, 0, gave_up, a.status)) {
-                // With a buffer to spare, the scores for the buffer that was freed one step ago follow the sums of this one, and
-                // the tensor cores do not wait; with two buffers that would make the groups wait for each other.
-                constexpr int kLag = B > 2 ? 1 : 0;
-                for (int j = 0; j < min(B, steps); j++) scores(j);
-                for (int j = 0; j < steps; j++) {
-                    const int stage = j % F::kStages, b = j % B, freed = j - kLag;
-                    if (!wait_warp(p_full + 8 * b, j / B & 1, gave_up, a.status)) break;
-                    after_sync();
-                    if (elect()) {
-                        const unsigned from = tmem + 128 * b, step = s_step + stage * F::kTileBytes, step2 = s_step2 + stage * F::kTileBytes;
-                        if (KEYS) product_over<N / 16, N * kTile>(tmem + F::kSums2, from, step2, shape_o, j > 0);
-                        product_over<N / 16, N * kTile>(tmem + F::kSums, from + 64, step, shape_o, j > 0);
-                        arrive_when_done(used + 8 * b);
-                        arrive_when_done(empty + 8 * stage);
-                    }
-                    __syncwarp();
-                    if (freed >= 0 && freed + B < steps) {
-                        if (!wait_warp(used + 8 * (freed % B), freed / B & 1, gave_up, a.status)) break;
-                        scores(freed + B);
-                    }
-                }
-                if (elect()) {  // no product is under way when the tensor memory is freed
-                    arrive_when_done(all_done);
-                    drain(all_done, 0);
-                }
-                __syncwarp();
-            }
+            if (lane == 0) arrive(clean + 8 * stage);
         }
     } else {
         const int g = warp >> 2, r = t & 127;
@@ -513,25 +548,35 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             shift = pair_of(-stat.x, -stat.x);
             delta = pair_of(-stat.y * factor, -stat.y * factor);
         }
+        // KEYS: this thread's column of the next step
+        const int my_token = KEYS ? r / a.pack : 0, my_head = KEYS ? kv * a.group + r % a.pack : 0;
+        int token = first_row + my_token, p_next = 0;
+        const auto next_stats = [&](int ahead) {
+            for (p_next += ahead; p_next >= packs; p_next -= packs) token += rows_a_step;
+            return r < a.pack * tokens && token < others.y ? a.stats[(long long)token * a.heads + my_head + p_next * a.pack] : make_float2(INFINITY, 0.f);
+        };
+        float2 mine = make_float2(INFINITY, 0.f);
+        if (KEYS && g < steps) mine = next_stats(g);
+        int b = g, row_k = first_row + g * N;
+        unsigned turn = 0;
         for (int j = g; j < steps; j += 2) {
-            const unsigned rows = lanes + 128 * (j % B);
+            const unsigned rows = lanes + 128 * b;
             unsigned seen[W];
             bool all = true;
             if (KEYS) {
-                float2 mine = make_float2(INFINITY, 0.f);
-                const int q0 = row_of(j);
-                if (r < min(tokens, others.y - q0) * a.pack) mine = a.stats[(long long)(q0 + r / a.pack) * a.heads + head_of(j) + r % a.pack];
                 asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");  // the last step's have been read
                 if (r < N) {
                     stats[r] = -mine.x;
                     stats[N + r] = -mine.y * factor;
                 }
+                if (j + 2 < steps) mine = next_stats(2);
                 asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");
-            } else {
-                all = seen_words<W>(seen, a.mask, row_of(j), others.y - row_of(j));
+            } else if (j >= dirty) {
+                all = seen_words<W>(seen, a.mask, row_k, others.y - row_k);
             }
+            row_k += 2 * N;
             // if a wait gave up, on to the next step: the group's barriers count on all warps
-            if (wait_warp(s_full + 8 * (j % B), j / B & 1, gave_up, a.status) && !idle) {
+            if (wait_warp(s_full + 8 * b, turn, gave_up, a.status) && !idle) {
                 after_sync();
 #pragma unroll
                 for (int w = 0; w < W; w++) {
@@ -577,7 +622,9 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             }
             before_sync();
             __syncwarp();
-            if (lane == 0) arrive(p_full + 8 * (j % B));
+            if (lane == 0) arrive(p_full + 8 * b);
+            b += 2;
+            if (b >= B) b -= B, turn ^= 1;
         }
         const bool done = steps > 0 && wait_warp(all_done, 0, gave_up, a.status);
         if (done) after_sync();
@@ -603,7 +650,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         before_sync();
         __syncthreads();
         after_sync();
-        if (warp == 9) tmem_free(tmem, F::kColumns);
+        if (warp == 11) tmem_free(tmem, F::kColumns);
     }
 }
 
@@ -669,8 +716,8 @@ template <typename T, int CHUNKS, bool KEYS> int grad_mma(const Args &a, const M
 
 template <typename T, int CHUNKS> int forward_mma(const Args &a, const Maps &maps, cudaStream_t stream)
 {
-    const dim3 grid((unsigned)tile_count(a.n_q, kMmaRows / a.pack, a.n_events), a.heads / a.pack, a.splits);
-    return launch(forward_mma_kernel<T, CHUNKS>, grid, kBlock, Forward<CHUNKS>::kSmem, stream, a, maps);
+    const dim3 grid((unsigned)tile_count(a.n_q, 2 * (kMmaRows / a.pack), a.n_events), a.heads / a.pack, a.splits);
+    return launch(forward_mma_kernel<T, CHUNKS>, grid, Forward<CHUNKS>::kThreads, Forward<CHUNKS>::kSmem, stream, a, maps);
 }
 
 }  // namespace
