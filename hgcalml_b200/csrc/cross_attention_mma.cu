@@ -82,7 +82,7 @@ template <int CHUNKS> struct Forward {
     static constexpr int kTileBytes = kKeys * kTile * CHUNKS, kQueryBytes = kMmaRows * kTile * CHUNKS;
     static constexpr int kBuffers = CHUNKS == 1 ? 3 : 4, kOut = kKeys * kBuffers, kColumns = 512;
     static constexpr int kTiles = 2 * kQueryBytes + 2 * kStages * kTileBytes, kSmem = kTiles + 512;
-    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers + 2;
+    static constexpr int kBarriers = 4 + 3 * kStages + 3 * kBuffers + 2;
     static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 512, "room");
 };
 
@@ -107,7 +107,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
     const int dirty = a.mask != nullptr ? 0 : (keys.y - first) / N;
 
     const unsigned s_q = smem_address(s_raw), s_k = s_q + 2 * F::kQueryBytes, s_v = s_k + F::kStages * F::kTileBytes;
-    const unsigned bar = s_q + F::kTiles, q_full = bar, scores_done = bar + 8, sums_done = scores_done + 8, full = sums_done + 8,
+    const unsigned bar = s_q + F::kTiles, q_full = bar, scores_done = bar + 8, sums_done = scores_done + 8, go = sums_done + 8, full = go + 8,
                    empty = full + 8 * F::kStages, clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B,
                    used = p_full + 8 * B, o_full = used + 8 * B;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + 8 * F::kBarriers);
@@ -178,12 +178,15 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
         if (steps > 0 && elect()) {
             const unsigned shape_o = shape<T>((a.dim + 15) / 16 * 16, true);
             int stage = 0, b = 0;
-            unsigned turn = 0, turn_b = 0;
+            unsigned turn_b = 0;
             bool ok = true;
             for (int j = 0; j < steps && ok; j++) {
-                if (dirty < steps) ok = wait(clean + 8 * stage, turn, gave_up, a.status);
                 for (int g = 0; g < groups && ok; g++) {
                     ok = wait(p_full + 8 * b, turn_b, gave_up, a.status);
+                    if (g == 0 && j >= dirty && ok) {
+                        if (a.mask == nullptr) arrive(go);
+                        ok = wait(clean + 8 * stage, (j - dirty) / F::kStages & 1, gave_up, a.status);
+                    }
                     after_sync();
                     if (ok) {
                         product_over<N / 16, N * kTile>(tmem + F::kOut + 64 * CHUNKS * g, tmem + N * b, s_v + stage * F::kTileBytes, shape_o, j > 0);
@@ -193,22 +196,27 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     if (++b == B) b = 0, turn_b ^= 1;
                 }
                 if (ok) arrive_when_done(empty + 8 * stage);
-                if (++stage == F::kStages) stage = 0, turn ^= 1;
+                if (++stage == F::kStages) stage = 0;
             }
             arrive_when_done(sums_done);
             drain(sums_done, 0);
         }
         __syncwarp();
     } else if (warp == 11) {
-        // where there is anything to clear, every step passes through here: a wait tells only two rounds of a stage apart
-        for (int j = dirty < steps ? 0 : steps; j < steps; j++) {
+        // Masked keys may be in any step, and are cleared as the copies come in.  Else it is the event's last step alone, for which
+        // the sums ask: a warp that followed every step would cost them 5 %.
+        for (int j = dirty; j < steps; j++) {
             const int stage = j % F::kStages, k0 = first + j * N;
             unsigned seen[W];
-            const bool all = j < dirty || seen_words<W>(seen, a.mask, k0, keys.y - k0);
-            if (!wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)) break;
-            if (!all) clear_unseen<W>(s_v + stage * F::kTileBytes, CHUNKS, seen);
-            writes_before_products();
-            __syncwarp();
+            const bool all = seen_words<W>(seen, a.mask, k0, keys.y - k0);
+            if (!(a.mask != nullptr ? wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)
+                                    : wait_warp(go, (j - dirty) & 1, gave_up, a.status)))
+                break;
+            if (!all) {
+                clear_unseen<W>(s_v + stage * F::kTileBytes, CHUNKS, seen);
+                writes_before_products();
+                __syncwarp();
+            }
             if (lane == 0) arrive(clean + 8 * stage);
         }
     } else {
@@ -236,26 +244,33 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             bool summed = j == 0;
             if (!idle) {
                 after_sync();
-                unsigned s[W][32];
+                // The scores are read twice, 32 at a time: once for the maximum and once for the weights.  Two reads take 300 cycles of a
+                // step; all of a row in registers left no room to overlap anything with the exponentials.
+                unsigned s[2][32];
+                const auto load = [&](int w) { tmem_load32(s[w & 1], rows + 32 * w); };
+                const auto masked = [&](int w) {
 #pragma unroll
-                for (int w = 0; w < W; w++) tmem_load32(s[w], rows + 32 * w);
-                tmem_loaded();
+                    for (int i = 0; i < 32; i++)
+                        if (!((seen[w] >> i) & 1u)) s[w & 1][i] = 0xff800000u;
+                };
+                // WHOLE: all keys of the step can be seen
+                const auto maximum = [&](auto whole) {
+                    float m[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+                    load(0);
 #pragma unroll
-                for (int w = 0; w < W; w++) use_after(s[w]);
-                if (!all) {
+                    for (int w = 0; w < W; w++) {
+                        tmem_loaded();
+                        use_after(s[w & 1]);
+                        if (w + 1 < W) load(w + 1);
+                        if (!decltype(whole)::value) masked(w);
 #pragma unroll
-                    for (int w = 0; w < W; w++)
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (!((seen[w] >> i) & 1u)) s[w][i] = 0xff800000u;
-                }
-                float m[4] = {top, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int w = 0; w < W; w++)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        m[(i >> 1) & 3] = fmaxf(m[(i >> 1) & 3], fmaxf(__uint_as_float(s[w][i]), __uint_as_float(s[w][i + 1])));
-                const float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                        for (int i = 0; i < 32; i += 2)
+                            m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], __uint_as_float(s[w & 1][i]), __uint_as_float(s[w & 1][i + 1]));
+                    }
+                    load(0);
+                    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                };
+                const float next = all ? maximum(std::true_type{}) : maximum(std::false_type{});
                 // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing in
                 // either type.
                 const bool grown = (next - top) * c > 8.f;
@@ -281,18 +296,27 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 const float base = (top == -INFINITY ? 0.f : top) * c;
                 const pair base2 = pair_of(-base, -base);
                 pair sums[2] = {0, 0};
+                // The special function unit takes 8 cycles for a warp's exponentials; a quarter of them goes without it.
+                const auto weights = [&](auto whole) {
 #pragma unroll
-                for (int w = 0; w < W; w++) {
-                    unsigned p[16];
+                    for (int w = 0; w < W; w++) {
+                        tmem_loaded();
+                        use_after(s[w & 1]);
+                        if (w + 1 < W) load(w + 1);
+                        if (!decltype(whole)::value) masked(w);
+                        unsigned p[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float2 x = parts(fma2(pair_of(__uint_as_float(s[w][2 * i]), __uint_as_float(s[w][2 * i + 1])), c2, base2));
-                        const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                        sums[i & 1] = add2(sums[i & 1], pair_of(e.x, e.y));
-                        p[i] = pack2<T>(e.x, e.y);
+                        for (int i = 0; i < 16; i++) {
+                            const float2 x = parts(fma2(pair_of(__uint_as_float(s[w & 1][2 * i]), __uint_as_float(s[w & 1][2 * i + 1])), c2, base2));
+                            const float2 e = decltype(whole)::value && i % 4 == 3 ? exp2_arithmetic(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            sums[i & 1] = add2(sums[i & 1], pair_of(e.x, e.y));
+                            p[i] = pack2<T>(e.x, e.y);
+                        }
+                        tmem_store16(rows + 16 * w, p);
                     }
-                    tmem_store16(rows + 16 * w, p);
-                }
+                };
+                if (all) weights(std::true_type{});
+                else weights(std::false_type{});
                 const float2 both = parts(add2(sums[0], sums[1]));
                 sum += both.x + both.y;
                 tmem_stored();
@@ -377,9 +401,9 @@ template <int CHUNKS, bool KEYS> struct Grad {
     static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 384;
     static constexpr int kTileBytes = kStep * kTile * CHUNKS, kKeptBytes = kMmaRows * kTile * CHUNKS;
     static constexpr int kBuffers = KEYS && CHUNKS == 2 ? 2 : 3, kSums = 128 * kBuffers, kSums2 = kSums + 64 * CHUNKS, kColumns = 512;
-    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 2 * 2 * kStep * 4, kSmem = kTiles + kStats + 256;
-    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers;
-    static_assert((KEYS ? kSums2 : kSums) + 64 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 256, "room");
+    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 2 * 2 * kStep * 4, kSmem = kTiles + kStats + 512;
+    static constexpr int kBarriers = 4 + 3 * kStages + 3 * kBuffers;
+    static_assert((KEYS ? kSums2 : kSums) + 64 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 512, "room");
 };
 
 template <typename T, int CHUNKS, bool KEYS>
@@ -409,7 +433,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
 
     const unsigned s_kept = smem_address(s_raw), s_kept2 = s_kept + F::kKeptBytes, s_step = s_kept2 + F::kKeptBytes,
                    s_step2 = s_step + F::kStages * F::kTileBytes;
-    const unsigned bar = s_kept + F::kTiles + F::kStats, kept_full = bar, scores_done = bar + 8, all_done = scores_done + 8, full = all_done + 8,
+    const unsigned bar = s_kept + F::kTiles + F::kStats, kept_full = bar, scores_done = bar + 8, all_done = scores_done + 8, go = all_done + 8, full = go + 8,
                    empty = full + 8 * F::kStages, clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B, used = p_full + 8 * B;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + F::kStats + 8 * F::kBarriers);
     volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
@@ -466,7 +490,10 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             unsigned turn = 0, turn_b = 1;  // of the stages; of the buffers, which are free at first
             for (int j = 0; j < steps && ok; j++) {
                 ok = wait(full + 8 * stage, turn, gave_up, a.status);
-                if (dirty < steps) ok = ok && wait(clean + 8 * stage, turn, gave_up, a.status);
+                if (KEYS && j >= dirty && ok) {
+                    arrive(go);
+                    ok = wait(clean + 8 * stage, (j - dirty) / F::kStages & 1, gave_up, a.status);
+                }
                 if (j >= B) ok = ok && wait(used + 8 * b, turn_b, gave_up, a.status);
                 after_sync();
                 if (ok) {
@@ -489,6 +516,10 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             unsigned turn_b = 0;
             for (int j = 0; j < steps; j++) {
                 if (!wait(p_full + 8 * b, turn_b, gave_up, a.status)) break;
+                if (!KEYS && j >= dirty) {
+                    if (a.mask == nullptr) arrive(go);
+                    if (!wait(clean + 8 * stage, (j - dirty) / F::kStages & 1, gave_up, a.status)) break;
+                }
                 after_sync();
                 const unsigned from = tmem + 128 * b;
                 if (KEYS) product_over<N / 16, N * kTile>(tmem + F::kSums2, from, s_step2 + stage * F::kTileBytes, shape_o, j > 0);
@@ -512,14 +543,15 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         writes_before_products();
         __syncwarp();
         if (lane == 0 && steps > 0) arrive(kept_full);
-        // Where there is anything to clear, every step passes through here: a wait tells only two rounds of a stage apart.
-        for (int j = dirty < steps ? 0 : steps; j < steps; j++) {
+        for (int j = dirty; j < steps; j++) {
             const int stage = j % F::kStages, row = first_row + j / packs * rows_a_step;
             const unsigned step = s_step + stage * F::kTileBytes, step2 = s_step2 + stage * F::kTileBytes;
             unsigned seen[W];
-            const bool all = KEYS || j < dirty || seen_words<W>(seen, a.mask, row, others.y - row);
-            if (!wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)) break;
-            if (KEYS && j >= dirty) {
+            const bool all = KEYS || seen_words<W>(seen, a.mask, row, others.y - row);
+            if (!(!KEYS && a.mask != nullptr ? wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)
+                                             : wait_warp(go, (j - dirty) & 1, gave_up, a.status)))
+                break;
+            if (KEYS) {
                 clear_rows(step, CHUNKS, N, (others.y - row) * a.pack, a.pack * tokens);
                 clear_rows(step2, CHUNKS, N, (others.y - row) * a.pack, a.pack * tokens);
             } else if (!all) {
