@@ -244,8 +244,9 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             bool summed = j == 0;
             if (!idle) {
                 after_sync();
-                // The scores are read twice, 32 at a time: once for the maximum and once for the weights.  Two reads take 300 cycles of a
-                // step; all of a row in registers left no room to overlap anything with the exponentials.
+                // More than 64 scores are read twice, 32 at a time: once for the maximum and once for the weights.  Two reads take 300
+                // cycles of a step; all of a row in registers left no room to overlap anything with the exponentials.
+                constexpr bool kTwice = W > 2;
                 unsigned s[2][32];
                 const auto load = [&](int w) { tmem_load32(s[w & 1], rows + 32 * w); };
                 const auto masked = [&](int w) {
@@ -267,7 +268,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                         for (int i = 0; i < 32; i += 2)
                             m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], __uint_as_float(s[w & 1][i]), __uint_as_float(s[w & 1][i + 1]));
                     }
-                    load(0);
+                    if (kTwice) load(0);
                     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 };
                 const float next = all ? maximum(std::true_type{}) : maximum(std::false_type{});
@@ -300,10 +301,12 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 const auto weights = [&](auto whole) {
 #pragma unroll
                     for (int w = 0; w < W; w++) {
-                        tmem_loaded();
-                        use_after(s[w & 1]);
-                        if (w + 1 < W) load(w + 1);
-                        if (!decltype(whole)::value) masked(w);
+                        if (kTwice) {
+                            tmem_loaded();
+                            use_after(s[w & 1]);
+                            if (w + 1 < W) load(w + 1);
+                            if (!decltype(whole)::value) masked(w);
+                        }
                         unsigned p[16];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
