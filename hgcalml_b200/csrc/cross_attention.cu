@@ -516,7 +516,7 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
     p.splits = split_count(filled(n_q, m) * (heads / p.pack), steps_k, 4, 4);
     const int mma_tokens = kMmaRows / p.pack;
-    p.splits_mma = split_count(filled(n_q, 2 * mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 2, 2);
+    p.splits_mma = split_count(filled(n_q, 2 * mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 6, 4);
     p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
     p.splits_q_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / kMmaGradStep, 4, 4);
     p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);
@@ -525,11 +525,14 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 }
 
 struct ForwardBuffers {
+    int *counter = nullptr;
     float *part = nullptr, *part_lse = nullptr;
 };
 template <typename C> ForwardBuffers carve_forward(C &c, const Plan &p, int n_q, int heads, int dim)
 {
     ForwardBuffers b;
+    if constexpr (std::is_same_v<C, Carver>) b.counter = c.template take<int>(1);
+    else c.template take<int>(1);
     const int splits = p.splits > p.splits_mma ? p.splits : p.splits_mma;
     if (splits > 1) {
         const size_t rows = (size_t)splits * n_q * heads;
@@ -706,7 +709,7 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
                      workspace);
     Carver carver(workspace);
     const ForwardBuffers b = carve_forward(carver, p, n_q, n_heads, dim);
-    a.to = d_out; a.part = b.part; a.part_lse = b.part_lse;
+    a.to = d_out; a.part = b.part; a.part_lse = b.part_lse; a.counter = b.counter;
     return dtype == HGC_FLOAT32 ? forward_of<float>(a, p, dtype, stream)
          : dtype == HGC_FLOAT16 ? forward_of<__half>(a, p, dtype, stream) : forward_of<__nv_bfloat16>(a, p, dtype, stream);
 }

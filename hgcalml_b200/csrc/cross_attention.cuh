@@ -35,6 +35,7 @@ struct Args {
     float *part, *part2;           // the same of every part of a split, in float32
     float *part_lse;               // [splits, n_q, heads]
     const float *bounds;           // largest squared norms of the rows of grad and of v (half precision's backward pass)
+    int *counter;                  // of the tiles that the blocks of the forward pass take
     unsigned *status;
     int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits;
     float scale;

@@ -1,7 +1,8 @@
 // Attention between two ragged sets of rows on the tensor cores, for 16-bit types.
 //
-// Blocks of twelve warps have a multiprocessor each.  Eight of them do the elementwise work on rows of tensor memory, four keep them
-// fed: copies, products of scores, products of sums, rows to clear.  They meet at barriers in shared memory only.
+// Blocks of twenty warps have a multiprocessor each.  Sixteen of them do the elementwise work on rows of tensor memory (with eight,
+// each instruction of a warp waited for the one before, and none of the units was half busy), four keep them fed: copies, products
+// of scores, products of sums, rows to clear.  They meet at barriers in shared memory only.
 #include <cuda.h>
 #include <atomic>
 
@@ -50,323 +51,481 @@ __device__ __forceinline__ void clear_unseen(unsigned tile, int chunks, const un
     }
 }
 
-// 16 columns of a row of a result
+// Where the lanes' rows of a result begin.  Two lanes write a row together, 32 bytes of it: stores of 16 bytes to 32 rows each took
+// twice as long.
+struct Rows {
+    long long at, other;
+    bool store, store_other;
+    __device__ __forceinline__ Rows(long long begin, bool in) : at(begin), store(in)
+    {
+        other = __shfl_xor_sync(0xffffffffu, at, 1);
+        store_other = __shfl_xor_sync(0xffffffffu, (int)in, 1) != 0;
+    }
+};
+// 16 columns of a row of a result; all lanes of a warp call this.
 template <typename T>
-__device__ __forceinline__ void store16(void *to, float *part, long long at, int d, int dim, const unsigned (&v)[16], float factor)
+__device__ __forceinline__ void store16(void *to, float *part, const Rows &rows, int d, int dim, const unsigned (&v)[16], float factor)
 {
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) x[i] = __uint_as_float(v[i]) * factor;
     if (part != nullptr) {
-        float4 *p = reinterpret_cast<float4 *>(part + at + d);
+        float4 *p = reinterpret_cast<float4 *>(part + rows.at + d);
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (d + 4 * i < dim) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            if (rows.store && d + 4 * i < dim) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
     } else {
-        uint4 *p = reinterpret_cast<uint4 *>(static_cast<T *>(to) + at + d);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (d + 8 * i < dim)
-                p[i] = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]), pack2<T>(x[8 * i + 4], x[8 * i + 5]),
-                                  pack2<T>(x[8 * i + 6], x[8 * i + 7]));
+        uint4 a = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+        uint4 b = make_uint4(pack2<T>(x[8], x[9]), pack2<T>(x[10], x[11]), pack2<T>(x[12], x[13]), pack2<T>(x[14], x[15]));
+        // first the even lanes' rows: they keep their first 16 bytes and give away the second; then the odd ones'
+        const bool odd = lane_id() & 1;
+        const uint4 give = odd ? a : b;
+        const uint4 got = make_uint4(__shfl_xor_sync(0xffffffffu, give.x, 1), __shfl_xor_sync(0xffffffffu, give.y, 1),
+                                     __shfl_xor_sync(0xffffffffu, give.z, 1), __shfl_xor_sync(0xffffffffu, give.w, 1));
+        T *const base = static_cast<T *>(to) + d + (odd ? 8 : 0);
+        if (d + (odd ? 8 : 0) < dim) {
+            if (odd ? rows.store_other : rows.store) *reinterpret_cast<uint4 *>(base + (odd ? rows.other : rows.at)) = odd ? got : a;
+            if (odd ? rows.store : rows.store_other) *reinterpret_cast<uint4 *>(base + (odd ? rows.at : rows.other)) = odd ? b : got;
+        }
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------- forward
-// A block has two tiles of 128 rows of queries, each with four warps that do its softmax (a row per lane), and takes them through
-// the keys of their event, kKeys a step.  Scores S = Q K^T and, in their place, weights P (16 bits) are in buffers of tensor memory
-// that the tiles use in turn, so that the next scores are done when a softmax ends; the sums O = P V lie beside them.  Four more warps
-// copy keys and values, issue scores, issue sums, and clear what must not be summed.
+// A tile is twice 128 rows of queries of an event, each half with eight warps that do its softmax (half a row per lane); it goes
+// through the keys of the event, kKeys a step.  Scores S = Q K^T and, in their place, weights P (16 bits) are in buffers of tensor memory that
+// the halves use in turn, so that the next scores are done when a softmax ends; the sums O = P V lie beside them.  Four more warps
+// copy queries, keys and values, issue scores, issue sums, and clear what must not be summed.
+//
+// A block takes one tile after the other from a counter, and every warp goes on to the next tile as soon as its own part is done: copies
+// and scores of a tile run under the softmax and the results of the one before.  With a tile per block, 371k queries on 1152 keys
+// took 490 us, two thirds of them for starting and ending blocks.
 template <int CHUNKS> struct Forward {
-    static constexpr int kKeys = CHUNKS == 1 ? 128 : 64, kStages = 5, kThreads = 384;
-    static constexpr int kTileBytes = kKeys * kTile * CHUNKS, kQueryBytes = kMmaRows * kTile * CHUNKS;
-    static constexpr int kBuffers = CHUNKS == 1 ? 3 : 4, kOut = kKeys * kBuffers, kColumns = 512;
-    static constexpr int kTiles = 2 * kQueryBytes + 2 * kStages * kTileBytes, kSmem = kTiles + 512;
-    static constexpr int kBarriers = 4 + 3 * kStages + 3 * kBuffers + 2;
-    static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 512, "room");
+    static constexpr int kKeys = CHUNKS == 1 ? 128 : 64, kStages = 4, kQueries = CHUNKS == 1 ? 2 : 1, kThreads = 640;
+    static constexpr int kTileBytes = kKeys * kTile * CHUNKS, kHalfBytes = kMmaRows * kTile * CHUNKS, kQueryBytes = 2 * kHalfBytes;
+    static constexpr int kBuffers = CHUNKS == 1 ? 3 : 4, kOut = kKeys * kBuffers, kColumns = 512, kItems = 4;
+    static constexpr int kTiles = kQueries * kQueryBytes + 2 * kStages * kTileBytes;
+    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers + 2 * kQueries + 2 * kItems + 4 + 8;
+    static constexpr int kBias = 512, kMaxAt = kBias + kStages * kKeys * 4, kItemAt = kMaxAt + 2 * 3 * 2 * kMmaRows * 4,
+                         kSmem = kTiles + kItemAt + kItems * 48;  // behind the tiles
+    static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= kBias && kSmem <= 232448, "room");
+};
+
+// What the warps of a block have to know of a tile; steps < 0: there is none any more.
+struct Item {
+    int steps, first, keys_end, dirty;  // of keys; steps from `dirty` on have some that are masked, or of another event
+    int begin, end, head0, split;       // of queries
+};
+
+// Counts through rounds of N.
+template <int N> struct Ring {
+    int at = 0;
+    unsigned turn = 0;
+    __device__ __forceinline__ void go(int by)  // at most N
+    {
+        at += by;
+        if (at >= N) at -= N, turn ^= 1;
+    }
 };
 
 template <typename T, int CHUNKS>
 __global__ void __launch_bounds__(Forward<CHUNKS>::kThreads, 1)
-forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps)
+forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps, int n_tiles, int n_items)
 {
     pdl_begin();
     using F = Forward<CHUNKS>;
     constexpr int N = F::kKeys, W = N / 32, B = F::kBuffers;
     extern __shared__ __align__(1024) char s_raw[];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int tokens = kMmaRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;  // tokens of one of the two tiles
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_splits(a, t, F::kThreads);
-    const Tile tile = find_tile(a.rs_q, a.n_q, a.n_events, 2 * tokens, blockIdx.x);
-    if (tile.begin >= tile.end) return;
-    const int groups = tile.end - tile.begin > tokens ? 2 : 1;
-    const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
-    const int2 part = part_of(max(0, (keys.y - keys.x + N - 1) / N), blockIdx.z, a.splits);
-    const int steps = part.y - part.x, first = keys.x + part.x * N;
-    // steps from this one on have keys that are masked, or of another event
-    const int dirty = a.mask != nullptr ? 0 : (keys.y - first) / N;
+    const int tokens = kMmaRows / a.pack;  // of half a tile
+    if (blockIdx.x == 0) check_splits(a, t, F::kThreads);
 
-    const unsigned s_q = smem_address(s_raw), s_k = s_q + 2 * F::kQueryBytes, s_v = s_k + F::kStages * F::kTileBytes;
-    const unsigned bar = s_q + F::kTiles, q_full = bar, scores_done = bar + 8, sums_done = scores_done + 8, go = sums_done + 8, full = go + 8,
-                   empty = full + 8 * F::kStages, clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B,
-                   used = p_full + 8 * B, o_full = used + 8 * B;
+    const unsigned s_q = smem_address(s_raw), s_k = s_q + F::kQueries * F::kQueryBytes, s_v = s_k + F::kStages * F::kTileBytes;
+    const unsigned bar = s_q + F::kTiles, scores_done = bar, sums_done = bar + 8, go = bar + 16, full = bar + 24, empty = full + 8 * F::kStages,
+                   clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B, used = p_full + 8 * B,
+                   q_full = used + 8 * B, q_empty = q_full + 8 * F::kQueries, item_full = q_empty + 8 * F::kQueries,
+                   item_empty = item_full + 8 * F::kItems, o_full = item_empty + 8 * F::kItems, o_empty = o_full + 16, meet = o_empty + 16;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + 8 * F::kBarriers);
     volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
-    if (steps > 0) {
-        if (t == 0) {
-            for (int i = 0; i < F::kBarriers; i++) {
-                const unsigned at = bar + 8 * i;
-                barrier_init(at, at >= p_full && at < used ? 4 : 1);
-            }
-            barrier_init_done();
-            *gave_up = 0;
+    float *s_bias = reinterpret_cast<float *>(s_raw + F::kTiles + F::kBias);  // [kStages][kKeys], 0 or minus infinity
+    Item *s_item = reinterpret_cast<Item *>(s_raw + F::kTiles + F::kItemAt);
+    if (t == 0) {
+        for (int i = 0; i < F::kBarriers; i++) {
+            const unsigned at = bar + 8 * i;
+            // arrivals: a half's warps; or of an item, all that read it: sixteen of the halves, and three
+            barrier_init(at, at >= meet ? 2 : (at >= p_full && at < used) || at >= o_empty ? 8 : at >= item_empty && at < o_full ? 19 : 1);
         }
-        if (warp == 11) tmem_alloc(s_tmem, F::kColumns);
-        before_sync();
-        __syncthreads();
-        after_sync();
+        barrier_init_done();
+        *gave_up = 0;
     }
-    const unsigned tmem = steps > 0 ? *s_tmem : 0;
+    if (warp == 19) tmem_alloc(s_tmem, F::kColumns);
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const unsigned tmem = *s_tmem;
 
-    if (warp == 8) {
-        if (steps > 0 && elect()) {
-            arrive_expect(q_full, groups * CHUNKS * kTile * a.pack * tokens);
-            for (int g = 0; g < groups; g++)
-                for (int c = 0; c < CHUNKS; c++)
-                    copy_box(s_q + g * F::kQueryBytes + c * kMmaRows * kTile, &maps.q, q_full, 64 * c, head0, tile.begin + g * tokens);
-            int copies = 0;
-            for (int j = 0; j < steps; j++) {
-                const int stage = j % F::kStages;
-                if (j >= F::kStages && !wait(empty + 8 * stage, (j / F::kStages & 1) ^ 1, gave_up, a.status)) break;
-                arrive_expect(full + 8 * stage, 2 * F::kTileBytes);
-                for (int c = 0; c < CHUNKS; c++) {
-                    copy_box(s_k + stage * F::kTileBytes + c * N * kTile, &maps.k, full + 8 * stage, 64 * c, kv, first + j * N);
-                    copy_box(s_v + stage * F::kTileBytes + c * N * kTile, &maps.v, full + 8 * stage, 64 * c, kv, first + j * N);
+    if (warp == 16) {
+        Ring<F::kItems> item;
+        Ring<F::kStages> kv;
+        Ring<F::kQueries> q;
+        int k_copies = 0, q_copies = 0, taken = 0;
+        bool ok = true;
+        for (int next = blockIdx.x; ok;) {
+            // the next tile that has rows
+            Item it;
+            it.steps = -1;
+            while (next < n_items) {
+                const int rest = next / n_tiles, split = rest / (a.heads / a.pack);
+                const Tile tile = find_tile(a.rs_q, a.n_q, a.n_events, 2 * tokens, next - rest * n_tiles);
+                if (n_items > gridDim.x) {
+                    if (lane == 0) next = gridDim.x + atomicAdd(a.counter, 1);
+                    next = __shfl_sync(0xffffffffu, next, 0);
+                } else {
+                    next = n_items;
                 }
-                copies++;
+                if (tile.begin >= tile.end) continue;
+                const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
+                const int2 part = part_of(max(0, (keys.y - keys.x + N - 1) / N), split, a.splits);
+                it.steps = part.y - part.x;
+                it.first = keys.x + part.x * N;
+                it.keys_end = keys.y;
+                it.dirty = a.mask != nullptr ? 0 : min(it.steps, (keys.y - it.first) / N);
+                it.begin = tile.begin;
+                it.end = tile.end;
+                it.head0 = (rest - split * (a.heads / a.pack)) * a.pack;
+                it.split = split;
+                break;
             }
-            // no copy is under way when the block leaves
-            drain(q_full, 0);
-            for (int j = max(0, copies - F::kStages); j < copies; j++) drain(full + 8 * (j % F::kStages), j / F::kStages & 1);
+            if (taken >= F::kItems) ok = wait_warp(item_empty + 8 * item.at, item.turn ^ 1, gave_up, a.status);
+            if (!ok) break;
+            if (lane == 0) {
+                s_item[item.at] = it;
+                arrive(item_full + 8 * item.at);
+            }
+            __syncwarp();
+            item.go(1);
+            taken++;
+            if (it.steps < 0) break;
+            if (it.steps > 0 && elect()) {
+                const int groups = it.end - it.begin > tokens ? 2 : 1, kv_head = it.head0 / a.group;
+                if (q_copies >= F::kQueries) ok = wait(q_empty + 8 * q.at, q.turn ^ 1, gave_up, a.status);
+                if (ok) {
+                    arrive_expect(q_full + 8 * q.at, groups * CHUNKS * kTile * a.pack * tokens);
+                    for (int g = 0; g < groups; g++)
+                        for (int c = 0; c < CHUNKS; c++)
+                            copy_box(s_q + q.at * F::kQueryBytes + g * F::kHalfBytes + c * kMmaRows * kTile, &maps.q, q_full + 8 * q.at, 64 * c, it.head0,
+                                     it.begin + g * tokens);
+                    q_copies++;
+                    q.go(1);
+                }
+                for (int j = 0; j < it.steps && ok; j++) {
+                    if (k_copies >= F::kStages) ok = wait(empty + 8 * kv.at, kv.turn ^ 1, gave_up, a.status);
+                    if (!ok) break;
+                    arrive_expect(full + 8 * kv.at, 2 * F::kTileBytes);
+                    for (int c = 0; c < CHUNKS; c++) {
+                        copy_box(s_k + kv.at * F::kTileBytes + c * N * kTile, &maps.k, full + 8 * kv.at, 64 * c, kv_head, it.first + j * N);
+                        copy_box(s_v + kv.at * F::kTileBytes + c * N * kTile, &maps.v, full + 8 * kv.at, 64 * c, kv_head, it.first + j * N);
+                    }
+                    k_copies++;
+                    kv.go(1);
+                }
+            }
+            __syncwarp();  // the counts are the elected thread's, which is the same one every time
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (elect()) {  // no copy is under way when the block leaves
+            for (int i = 0; i < min(q_copies, F::kQueries); i++) {
+                if (--q.at < 0) q.at = F::kQueries - 1, q.turn ^= 1;
+                drain(q_full + 8 * q.at, q.turn);
+            }
+            for (int i = 0; i < min(k_copies, F::kStages); i++) {
+                if (--kv.at < 0) kv.at = F::kStages - 1, kv.turn ^= 1;
+                drain(full + 8 * kv.at, kv.turn);
+            }
         }
         __syncwarp();
-    } else if (warp == 9) {
-        if (steps > 0 && elect()) {
+    } else if (warp == 17) {
+        if (elect()) {
             const int depth = (a.dim + 15) / 16;
             const unsigned shape_s = shape<T>(N, false);
-            bool ok = wait(q_full, 0, gave_up, a.status);
-            int stage = 0, b = 0;
-            unsigned turn = 0, turn_b = 1;
-            for (int j = 0, i = 0; j < steps && ok; j++) {
-                ok = wait(full + 8 * stage, turn, gave_up, a.status);
-                for (int g = 0; g < groups && ok; g++, i++) {
-                    if (i >= B) ok = wait(used + 8 * b, turn_b, gave_up, a.status);
-                    after_sync();
-                    if (ok) {
-                        product_along<CHUNKS, kMmaRows * kTile, N * kTile>(tmem + N * b, s_q + g * F::kQueryBytes, s_k + stage * F::kTileBytes, depth, shape_s);
-                        arrive_when_done(s_full + 8 * b);
+            Ring<F::kItems> item;
+            Ring<F::kStages> kv;
+            Ring<F::kQueries> q;
+            Ring<B> buffer;
+            int scored = 0;
+            unsigned clean_turns = 0;  // a bit per stage: the round of its barrier
+            bool ok = true;
+            while (ok) {
+                ok = wait(item_full + 8 * item.at, item.turn, gave_up, a.status);
+                const Item it = s_item[item.at];
+                arrive(item_empty + 8 * item.at);
+                item.go(1);
+                if (!ok || it.steps < 0) break;
+                if (it.steps == 0) continue;
+                const int groups = it.end - it.begin > tokens ? 2 : 1;
+                ok = wait(q_full + 8 * q.at, q.turn, gave_up, a.status);
+                for (int j = 0; j < it.steps && ok; j++) {
+                    ok = wait(full + 8 * kv.at, kv.turn, gave_up, a.status);
+                    if (j >= it.dirty && ok) {
+                        if (a.mask == nullptr) arrive(go);
+                        ok = wait(clean + 8 * kv.at, clean_turns >> kv.at & 1, gave_up, a.status);
+                        clean_turns ^= 1u << kv.at;
                     }
-                    if (++b == B) b = 0, turn_b ^= 1;
+                    for (int g = 0; g < groups && ok; g++) {
+                        if (scored >= B) ok = wait(used + 8 * buffer.at, buffer.turn ^ 1, gave_up, a.status);
+                        after_sync();
+                        if (!ok) break;
+                        product_along<CHUNKS, kMmaRows * kTile, N * kTile>(tmem + N * buffer.at, s_q + q.at * F::kQueryBytes + g * F::kHalfBytes,
+                                                                           s_k + kv.at * F::kTileBytes, depth, shape_s);
+                        arrive_when_done(s_full + 8 * buffer.at);
+                        scored = min(scored + 1, B);
+                        buffer.go(1);
+                    }
+                    kv.go(1);
                 }
-                if (++stage == F::kStages) stage = 0, turn ^= 1;
+                if (ok) arrive_when_done(q_empty + 8 * q.at);
+                q.go(1);
             }
             arrive_when_done(scores_done);  // no product is under way when the tensor memory is freed
             drain(scores_done, 0);
         }
         __syncwarp();
-    } else if (warp == 10) {
-        if (steps > 0 && elect()) {
+    } else if (warp == 18) {
+        if (elect()) {
             const unsigned shape_o = shape<T>((a.dim + 15) / 16 * 16, true);
-            int stage = 0, b = 0;
-            unsigned turn_b = 0;
-            bool ok = true;
-            for (int j = 0; j < steps && ok; j++) {
-                for (int g = 0; g < groups && ok; g++) {
-                    ok = wait(p_full + 8 * b, turn_b, gave_up, a.status);
-                    if (g == 0 && j >= dirty && ok) {
-                        if (a.mask == nullptr) arrive(go);
-                        ok = wait(clean + 8 * stage, (j - dirty) / F::kStages & 1, gave_up, a.status);
-                    }
-                    after_sync();
-                    if (ok) {
-                        product_over<N / 16, N * kTile>(tmem + F::kOut + 64 * CHUNKS * g, tmem + N * b, s_v + stage * F::kTileBytes, shape_o, j > 0);
-                        arrive_when_done(used + 8 * b);
+            Ring<F::kItems> item;
+            Ring<F::kStages> kv;
+            Ring<B> buffer;
+            unsigned o_turn[2] = {1, 1};  // of the halves' sums, which are free at first
+            bool ok = true, o_used[2] = {false, false};
+            while (ok) {
+                ok = wait(item_full + 8 * item.at, item.turn, gave_up, a.status);
+                const Item it = s_item[item.at];
+                arrive(item_empty + 8 * item.at);
+                item.go(1);
+                if (!ok || it.steps < 0) break;
+                const int groups = it.end - it.begin > tokens ? 2 : 1;
+                for (int j = 0; j < it.steps && ok; j++) {
+                    for (int g = 0; g < groups && ok; g++) {
+                        ok = wait(p_full + 8 * buffer.at, buffer.turn, gave_up, a.status);
+                        if (j == 0 && ok) {  // the results of the tile before have been read
+                            if (o_used[g]) ok = wait(o_empty + 8 * g, o_turn[g], gave_up, a.status);
+                            o_used[g] = true;
+                            o_turn[g] ^= 1;
+                        }
+                        after_sync();
+                        if (!ok) break;
+                        product_over<N / 16, N * kTile>(tmem + F::kOut + 64 * CHUNKS * g, tmem + N * buffer.at, s_v + kv.at * F::kTileBytes, shape_o, j > 0);
+                        arrive_when_done(used + 8 * buffer.at);
                         arrive_when_done(o_full + 8 * g);
+                        buffer.go(1);
                     }
-                    if (++b == B) b = 0, turn_b ^= 1;
+                    if (ok) arrive_when_done(empty + 8 * kv.at);
+                    kv.go(1);
                 }
-                if (ok) arrive_when_done(empty + 8 * stage);
-                if (++stage == F::kStages) stage = 0;
             }
             arrive_when_done(sums_done);
             drain(sums_done, 0);
         }
         __syncwarp();
-    } else if (warp == 11) {
+    } else if (warp == 19) {
         // Masked keys may be in any step, and are cleared as the copies come in.  Else it is the event's last step alone, for which
-        // the sums ask: a warp that followed every step would cost them 5 %.
-        for (int j = dirty; j < steps; j++) {
-            const int stage = j % F::kStages, k0 = first + j * N;
-            unsigned seen[W];
-            const bool all = seen_words<W>(seen, a.mask, k0, keys.y - k0);
-            if (!(a.mask != nullptr ? wait_warp(full + 8 * stage, j / F::kStages & 1, gave_up, a.status)
-                                    : wait_warp(go, (j - dirty) & 1, gave_up, a.status)))
-                break;
-            if (!all) {
-                clear_unseen<W>(s_v + stage * F::kTileBytes, CHUNKS, seen);
-                writes_before_products();
+        // the scores ask: a warp that followed every step would cost the others 5 %.
+        Ring<F::kItems> item;
+        Ring<F::kStages> kv;
+        unsigned go_turn = 0;
+        bool ok = true;
+        while (ok) {
+            ok = wait_warp(item_full + 8 * item.at, item.turn, gave_up, a.status);
+            const Item it = s_item[item.at];
+            __syncwarp();
+            if (lane == 0) arrive(item_empty + 8 * item.at);
+            item.go(1);
+            if (!ok || it.steps < 0) break;
+            for (int j = 0; j < it.steps && ok; j++, kv.go(1)) {
+                if (j < it.dirty) continue;
+                const int k0 = it.first + j * N;
+                unsigned seen[W];
+                const bool all = seen_words<W>(seen, a.mask, k0, it.keys_end - k0);
+                if (a.mask != nullptr) {
+                    ok = wait_warp(full + 8 * kv.at, kv.turn, gave_up, a.status);
+                } else {
+                    ok = wait_warp(go, go_turn, gave_up, a.status);
+                    go_turn ^= 1;
+                }
+                if (!ok) break;
+                if (!all) {
+                    clear_unseen<W>(s_k + kv.at * F::kTileBytes, CHUNKS, seen);
+                    clear_unseen<W>(s_v + kv.at * F::kTileBytes, CHUNKS, seen);
+                    writes_before_products();
+                }
+#pragma unroll
+                for (int w = 0; w < W; w++) s_bias[kv.at * N + 32 * w + lane] = (seen[w] >> lane) & 1u ? 0.f : -INFINITY;
                 __syncwarp();
+                if (lane == 0) arrive(clean + 8 * kv.at);
             }
-            if (lane == 0) arrive(clean + 8 * stage);
         }
     } else {
-        const int g = warp >> 2, r = t & 127;
-        const int n_rows = min(tokens, tile.end - tile.begin - g * tokens) * a.pack;
+        const int g = warp >> 3, half = (warp >> 2) & 1, r = t & 127;  // the lane has row r of half tile g, and half of its columns
         const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21), out = lanes + F::kOut + 64 * CHUNKS * g;
-        const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;  // idle: none of the warp's rows counts
+        float *maxima = reinterpret_cast<float *>(s_raw + F::kTiles + F::kMaxAt) + g * 3 * 2 * kMmaRows;  // [two in turn, and the sums][halves][rows]
+        const unsigned meeting = meet + 8 * (g * 4 + (warp & 3));  // of the two warps that share rows
+        unsigned meet_turn = 0;
+        bool ok = true;
+        const auto exchange = [&](float *both_halves, float mine) {
+            both_halves[half * kMmaRows + r] = mine;
+            __syncwarp();
+            if (lane == 0) arrive(meeting);
+            ok = wait_warp(meeting, meet_turn, gave_up, a.status) && ok;
+            meet_turn ^= 1;
+            return both_halves[(half ^ 1) * kMmaRows + r];
+        };
+        constexpr int V = W / 2;
         const float c = a.scale * kLog2e;
         const pair c2 = pair_of(c, c);
-        float top = -INFINITY, sum = 0.f;
-        int b = g;
-        unsigned turn = 0, seen[W];
-        bool all = dirty > 0;
-        if (!all && g < groups && steps > 0) all = seen_words<W>(seen, a.mask, first, keys.y - first);
-        for (int j = 0; j < steps && g < groups; j++) {
-            const unsigned rows = lanes + N * b;
-            // whether the keys of the next step can be seen, asked for ahead of their time
-            unsigned char ahead[W];
-            const int next_key = first + (j + 1) * N, next_n = j + 1 < steps && j + 1 >= dirty ? keys.y - next_key : 0;
-#pragma unroll
-            for (int w = 0; w < W; w++)
-                ahead[w] = 32 * w + lane < next_n ? a.mask == nullptr ? 1 : fresh(a.mask + next_key + 32 * w + lane) : 0;
-            if (!wait_warp(s_full + 8 * b, turn, gave_up, a.status)) break;
-            // every phase of the sums' barrier is waited for: here, where they are scaled, else when this step's weights are done
-            bool summed = j == 0;
-            if (!idle) {
-                after_sync();
-                // More than 64 scores are read twice, 32 at a time: once for the maximum and once for the weights.  Two reads take 300
-                // cycles of a step; all of a row in registers left no room to overlap anything with the exponentials.
-                constexpr bool kTwice = W > 2;
-                unsigned s[2][32];
-                const auto load = [&](int w) { tmem_load32(s[w & 1], rows + 32 * w); };
-                const auto masked = [&](int w) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (!((seen[w] >> i) & 1u)) s[w & 1][i] = 0xff800000u;
-                };
-                // WHOLE: all keys of the step can be seen
-                const auto maximum = [&](auto whole) {
-                    float m[4] = {top, -INFINITY, -INFINITY, -INFINITY};
-                    load(0);
-#pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        tmem_loaded();
-                        use_after(s[w & 1]);
-                        if (w + 1 < W) load(w + 1);
-                        if (!decltype(whole)::value) masked(w);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], __uint_as_float(s[w & 1][i]), __uint_as_float(s[w & 1][i + 1]));
-                    }
-                    if (kTwice) load(0);
-                    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                };
-                const float next = all ? maximum(std::true_type{}) : maximum(std::false_type{});
-                // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing in
-                // either type.
-                const bool grown = (next - top) * c > 8.f;
-                if (j == 0) {
-                    top = next;
-                } else if (__any_sync(0xffffffffu, grown)) {
-                    if (!wait_warp(o_full + 8 * g, (j - 1) & 1, gave_up, a.status)) break;
-                    summed = true;
-                    after_sync();
-                    const float shrink = exp2_fast((top - (next == -INFINITY ? 0.f : next)) * c);
-                    top = next;
-                    sum *= shrink;
-                    for (int d = 0; d < a.dim; d += 16) {
-                        unsigned o[16];
-                        tmem_load16(o, out + d);
-                        tmem_loaded();
-                        use_after(o);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-                        tmem_store16(out + d, o);
-                    }
+        Ring<F::kItems> item;
+        Ring<F::kStages> kv;
+        Ring<B> buffer;
+        unsigned o_turn = 0, clean_turns = 0;
+        while (ok) {
+            ok = wait_warp(item_full + 8 * item.at, item.turn, gave_up, a.status);
+            const Item it = s_item[item.at];
+            __syncwarp();
+            if (lane == 0) arrive(item_empty + 8 * item.at);
+            item.go(1);
+            if (!ok || it.steps < 0) break;
+            const int groups = it.end - it.begin > tokens ? 2 : 1;
+            const int n_rows = min(tokens, it.end - it.begin - g * tokens) * a.pack;
+            const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;  // idle: none of the warp's rows counts
+            float top = -INFINITY, sum = 0.f;
+            if (groups == 2 && g == 1 && it.steps > 0) buffer.go(1);  // this half's place among the two
+            for (int j = 0; j < it.steps; j++, kv.go(1)) {
+                const bool whole_step = j < it.dirty;
+                const unsigned clean_turn = clean_turns >> kv.at & 1;
+                if (!whole_step) clean_turns ^= 1u << kv.at;
+                if (g >= groups) {  // the other half's buffers
+                    buffer.go(1);
+                    continue;
                 }
-                const float base = (top == -INFINITY ? 0.f : top) * c;
-                const pair base2 = pair_of(-base, -base);
-                pair sums[2] = {0, 0};
-                // The special function unit takes 8 cycles for a warp's exponentials; a quarter of them goes without it.
-                const auto weights = [&](auto whole) {
+                const unsigned rows = lanes + N * buffer.at + half * (N / 2);
+                ok = wait_warp(s_full + 8 * buffer.at, buffer.turn, gave_up, a.status) && ok;
+                if (!whole_step) ok = wait_warp(clean + 8 * kv.at, clean_turn, gave_up, a.status) && ok;
+                // every phase of the sums' barrier is waited for: here, where they are scaled, else when this step's weights are done
+                bool summed = j == 0;
+                if (!idle) {
+                    after_sync();
+                    // The scores are read twice, 32 at a time: once for the maximum and once for the weights.  The loops stay loops: unrolled
+                    // and in a second form for masked keys they were more instructions than the caches hold.
+                    unsigned s[32];
+                    const float *bias = s_bias + kv.at * N + half * (N / 2);
+                    const auto read = [&](int w) {
+                        tmem_load32(s, rows + 32 * w);
+                        tmem_loaded();
+                        use_after(s);
+                        if (whole_step) return;
 #pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        if (kTwice) {
-                            tmem_loaded();
-                            use_after(s[w & 1]);
-                            if (w + 1 < W) load(w + 1);
-                            if (!decltype(whole)::value) masked(w);
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 add = *reinterpret_cast<const float4 *>(bias + 32 * w + i);
+                            s[i] = __float_as_uint(__uint_as_float(s[i]) + add.x);
+                            s[i + 1] = __float_as_uint(__uint_as_float(s[i + 1]) + add.y);
+                            s[i + 2] = __float_as_uint(__uint_as_float(s[i + 2]) + add.z);
+                            s[i + 3] = __float_as_uint(__uint_as_float(s[i + 3]) + add.w);
                         }
+                    };
+                    float m[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int w = 0; w < V; w++) {
+                        read(w);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    }
+                    float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                    next = fmaxf(next, exchange(maxima + (j & 1) * 2 * kMmaRows, next));
+                    // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing
+                    // in either type.
+                    const bool grown = (next - top) * c > 8.f;
+                    if (j == 0) {
+                        top = next;
+                    } else if (__any_sync(0xffffffffu, grown)) {
+                        ok = wait_warp(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
+                        summed = true;
+                        after_sync();
+                        const float shrink = exp2_fast((top - (next == -INFINITY ? 0.f : next)) * c);
+                        top = next;
+                        sum *= shrink;
+                        for (int d = 16 * half; d < a.dim; d += 32) {
+                            unsigned o[16];
+                            tmem_load16(o, out + d);
+                            tmem_loaded();
+                            use_after(o);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                            tmem_store16(out + d, o);
+                        }
+                    }
+                    const float base = (top == -INFINITY ? 0.f : top) * c;
+                    const pair base2 = pair_of(-base, -base);
+                    pair sums[2] = {0, 0};
+                    // The special function unit takes 8 cycles for a warp's exponentials; a quarter of them goes without it.  (There, a masked
+                    // key gets 2^-126: its row of values is zero, and a sum of nothing else is told by its maximum.)
+#pragma unroll 1
+                    for (int w = 0; w < V; w++) {
+                        if (V > 1) read(w);
                         unsigned p[16];
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float2 x = parts(fma2(pair_of(__uint_as_float(s[w & 1][2 * i]), __uint_as_float(s[w & 1][2 * i + 1])), c2, base2));
-                            const float2 e = decltype(whole)::value && i % 4 == 3 ? exp2_arithmetic(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            const float2 x = parts(fma2(pair_of(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, base2));
+                            const float2 e = i % 4 == 3 ? exp2_arithmetic(x) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
                             sums[i & 1] = add2(sums[i & 1], pair_of(e.x, e.y));
                             p[i] = pack2<T>(e.x, e.y);
                         }
                         tmem_store16(rows + 16 * w, p);
                     }
-                };
-                if (all) weights(std::true_type{});
-                else weights(std::false_type{});
-                const float2 both = parts(add2(sums[0], sums[1]));
-                sum += both.x + both.y;
-                tmem_stored();
-            }
-            if (!summed && !wait_warp(o_full + 8 * g, (j - 1) & 1, gave_up, a.status)) break;
-            before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(p_full + 8 * b);
-            if (j + 1 >= dirty) {
-                all = next_n >= N;
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    seen[w] = __ballot_sync(0xffffffffu, ahead[w] != 0);
-                    all = all && seen[w] == 0xffffffffu;
+                    const float2 both = parts(add2(sums[0], sums[1]));
+                    sum += both.x + both.y;
+                    tmem_stored();
                 }
-            }
-            b += groups;
-            if (b >= B) b -= B, turn ^= 1;
-        }
-        const bool done = steps > 0 && g < groups && wait_warp(sums_done, 0, gave_up, a.status);
-        if (done) after_sync();
-        const long long row = (long long)(tile.begin + g * tokens + r / a.pack) * a.heads + head0 + r % a.pack;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const long long all_rows = (long long)a.n_q * a.heads;
-        if (store) {
-            float *lse = a.splits > 1 ? a.part_lse + blockIdx.z * all_rows : a.lse;
-            lse[row] = sum == 0.f ? -INFINITY : top * a.scale + logf(sum);
-        }
-        float *to_part = a.splits > 1 ? a.part + blockIdx.z * all_rows * a.dim : nullptr;
-        if (!idle && (done || a.splits == 1))  // a part without keys has no weight
-            for (int d = 0; d < a.dim; d += 16) {
-                unsigned o[16] = {};
-                if (done) {
-                    tmem_load16(o, out + d);
-                    tmem_loaded();
-                    use_after(o);
-                }
-                if (store) store16<T>(a.to, to_part, row * a.dim, d, a.dim, o, inv);
+                if (!summed) ok = wait_warp(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
+                o_turn ^= 1;
+                before_sync();
                 __syncwarp();
+                if (lane == 0) arrive(p_full + 8 * buffer.at);
+                buffer.go(groups == 1 || (g == 1 && j == it.steps - 1) ? 1 : 2);
             }
+            if (g >= groups) continue;
+            const bool done = it.steps > 0 && ok && wait_warp(o_full + 8 * g, o_turn ^ 1, gave_up, a.status);
+            if (done) after_sync();
+            const long long row = (long long)(it.begin + g * tokens + r / a.pack) * a.heads + it.head0 + r % a.pack;
+            if (it.steps > 0 && !idle) sum += exchange(maxima + 2 * 2 * kMmaRows, sum);
+            const bool none = top == -INFINITY;  // no key was seen
+            const float inv = none ? 0.f : 1.f / sum;
+            const long long all_rows = (long long)a.n_q * a.heads;
+            if (store && half == 0) {
+                float *lse = a.splits > 1 ? a.part_lse + it.split * all_rows : a.lse;
+                lse[row] = none ? -INFINITY : top * a.scale + logf(sum);
+            }
+            float *to_part = a.splits > 1 ? a.part + it.split * all_rows * a.dim : nullptr;
+            if (!idle && (done || a.splits == 1)) {  // a part without keys has no weight
+                const Rows to(row * a.dim, store);
+                for (int d = 16 * half; d < a.dim; d += 32) {
+                    unsigned o[16] = {};
+                    if (done) {
+                        tmem_load16(o, out + d);
+                        tmem_loaded();
+                        use_after(o);
+                    }
+                    store16<T>(a.to, to_part, to, d, a.dim, o, inv);
+                }
+            }
+            if (it.steps > 0) {
+                before_sync();
+                __syncwarp();
+                if (lane == 0) arrive(o_empty + 8 * g);
+            }
+        }
     }
-    if (steps > 0) {
-        before_sync();
-        __syncthreads();
-        after_sync();
-        if (warp == 11) tmem_free(tmem, F::kColumns);
-    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    if (warp == 19) tmem_free(tmem, F::kColumns);
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
@@ -401,10 +560,10 @@ __device__ __forceinline__ void clear_rows(unsigned tile, int chunks, int tile_r
 // thread each, that does nothing else, and rows that must not be summed over are cleared by a warp of their own.
 // (Two blocks of 256 columns, each with one buffer, waited for products two thirds of the time: 16k x 16k rows, 8 heads of 64, 3.2 ms.)
 template <int CHUNKS, bool KEYS> struct Grad {
-    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 384;
+    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 640;
     static constexpr int kTileBytes = kStep * kTile * CHUNKS, kKeptBytes = kMmaRows * kTile * CHUNKS;
     static constexpr int kBuffers = KEYS && CHUNKS == 2 ? 2 : 3, kSums = 128 * kBuffers, kSums2 = kSums + 64 * CHUNKS, kColumns = 512;
-    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 2 * 2 * kStep * 4, kSmem = kTiles + kStats + 512;
+    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 16 * 2 * 32 * 4, kSmem = kTiles + kStats + 512;
     static constexpr int kBarriers = 4 + 3 * kStages + 3 * kBuffers;
     static_assert((KEYS ? kSums2 : kSums) + 64 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 512, "room");
 };
@@ -444,19 +603,19 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         if (t == 0) {
             for (int i = 0; i < F::kBarriers; i++) {
                 const unsigned at = bar + 8 * i;
-                barrier_init(at, at >= p_full && at < used ? 4 : at == kept_full ? 2 : 1);
+                barrier_init(at, at >= p_full && at < used ? 8 : at == kept_full ? 2 : 1);
             }
             barrier_init_done();
             *gave_up = 0;
         }
-        if (warp == 11) tmem_alloc(s_tmem, F::kColumns);
+        if (warp == 19) tmem_alloc(s_tmem, F::kColumns);
         before_sync();
         __syncthreads();
         after_sync();
     }
     const unsigned tmem = steps > 0 ? *s_tmem : 0;
 
-    if (warp == 8) {
+    if (warp == 16) {
         if (steps > 0 && elect()) {
             const int kept_head = KEYS ? kv : blockIdx.y * a.pack;
             arrive_expect(kept_full, KEYS ? 2 * F::kKeptBytes : 2 * CHUNKS * kTile * a.pack * tokens);
@@ -484,7 +643,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             for (int j = max(0, copies - F::kStages); j < copies; j++) drain(full + 8 * (j % F::kStages), j / F::kStages & 1);
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         if (steps > 0 && elect()) {
             const int depth = (a.dim + 15) / 16;
             const unsigned shape_s = shape<T>(N, false);
@@ -512,7 +671,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             drain(scores_done, 0);
         }
         __syncwarp();
-    } else if (warp == 10) {
+    } else if (warp == 18) {
         if (steps > 0 && elect()) {
             const unsigned shape_o = shape<T>((a.dim + 15) / 16 * 16, true);
             int stage = 0, b = 0;
@@ -536,7 +695,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             drain(all_done, 0);
         }
         __syncwarp();
-    } else if (warp == 11) {
+    } else if (warp == 19) {
         if (KEYS && steps > 0 && a.pack * tokens < N) {  // rows that no copy writes
             for (int i = 0; i < F::kStages; i++) {
                 clear_rows(s_step + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
@@ -565,13 +724,15 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             if (lane == 0) arrive(clean + 8 * stage);
         }
     } else {
-        const int g = warp >> 2, r = t & 127;
+        // the lane has row r in every other step, beginning with step g, and half of its columns
+        const int g = warp >> 3, half = (warp >> 2) & 1, r = t & 127;
         const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21);
         const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;
         const float scale = a.scale * kLog2e, factor = slope_factor<T>(a);
         const pair c = pair_of(scale, scale), f = pair_of(factor, factor);
-        // KEYS: of the columns, in shared memory, negative, first the exponents' and then the slopes'.  Else of this lane's row.
-        float *stats = reinterpret_cast<float *>(s_raw + F::kTiles) + g * 2 * N;
+        // KEYS: of the columns, in the warp's own shared memory, negative, first the exponents' and then the slopes'.  Else of this
+        // lane's row.
+        float *stats = reinterpret_cast<float *>(s_raw + F::kTiles) + warp * 2 * 32;
         const long long row = KEYS ? ((long long)(tile.begin + r) * a.kv_heads + kv)
                                    : (long long)(tile.begin + r / a.pack) * a.heads + blockIdx.y * a.pack + r % a.pack;
         pair shift = 0, delta = 0;
@@ -583,76 +744,70 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             shift = pair_of(-stat.x, -stat.x);
             delta = pair_of(-stat.y * factor, -stat.y * factor);
         }
-        // KEYS: this thread's column of the next step
-        const int my_token = KEYS ? r / a.pack : 0, my_head = KEYS ? kv * a.group + r % a.pack : 0;
+        // KEYS: the lane asks for a column of the next step
+        const int column = 32 * half + lane, my_token = KEYS ? column / a.pack : 0, my_head = KEYS ? kv * a.group + column % a.pack : 0;
         int token = first_row + my_token, p_next = 0;
         const auto next_stats = [&](int ahead) {
             for (p_next += ahead; p_next >= packs; p_next -= packs) token += rows_a_step;
-            return r < a.pack * tokens && token < others.y ? a.stats[(long long)token * a.heads + my_head + p_next * a.pack] : make_float2(INFINITY, 0.f);
+            return column < a.pack * tokens && token < others.y ? a.stats[(long long)token * a.heads + my_head + p_next * a.pack] : make_float2(INFINITY, 0.f);
         };
         float2 mine = make_float2(INFINITY, 0.f);
         if (KEYS && g < steps) mine = next_stats(g);
         int b = g, row_k = first_row + g * N;
         unsigned turn = 0;
         for (int j = g; j < steps; j += 2) {
-            const unsigned rows = lanes + 128 * b;
+            const unsigned rows = lanes + 128 * b + 32 * half;
             unsigned seen[W];
             bool all = true;
             if (KEYS) {
-                asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");  // the last step's have been read
-                if (r < N) {
-                    stats[r] = -mine.x;
-                    stats[N + r] = -mine.y * factor;
-                }
+                __syncwarp();
+                stats[lane] = -mine.x;
+                stats[32 + lane] = -mine.y * factor;
                 if (j + 2 < steps) mine = next_stats(2);
-                asm volatile("bar.sync %0, 128;" :: "r"(1 + g) : "memory");
+                __syncwarp();
             } else if (j >= dirty) {
                 all = seen_words<W>(seen, a.mask, row_k, others.y - row_k);
             }
             row_k += 2 * N;
-            // if a wait gave up, on to the next step: the group's barriers count on all warps
             if (wait_warp(s_full + 8 * b, turn, gave_up, a.status) && !idle) {
                 after_sync();
+                unsigned s[32], d[32], p[16], q[16];
+                tmem_load32(s, rows);
+                tmem_load32(d, rows + 64);
+                tmem_loaded();
+                use_after(s);
+                use_after(d);
 #pragma unroll
-                for (int w = 0; w < W; w++) {
-                    unsigned s[32], d[32], p[16], q[16];
-                    tmem_load32(s, rows + 32 * w);
-                    tmem_load32(d, rows + 64 + 32 * w);
-                    tmem_loaded();
-                    use_after(s);
-                    use_after(d);
+                for (int i = 0; i < 32; i += 4) {
+                    pair x[2] = {shift, shift}, y[2] = {delta, delta};
+                    if (KEYS) {
+                        const ulonglong2 sx = *reinterpret_cast<const ulonglong2 *>(stats + i);
+                        const ulonglong2 sy = *reinterpret_cast<const ulonglong2 *>(stats + 32 + i);
+                        x[0] = sx.x; x[1] = sx.y; y[0] = sy.x; y[1] = sy.y;
+                    }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        pair x[2] = {shift, shift}, y[2] = {delta, delta};
+                    for (int h = 0; h < 2; h++) {
+                        const int at = i + 2 * h;
+                        const float2 e = parts(fma2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c, x[h]));
+                        const float2 w2 = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                        const pair dp = pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1]));
+                        const float2 slope = parts(mul2(pair_of(w2.x, w2.y), kScaled ? fma2(dp, f, y[h]) : add2(dp, y[h])));
                         if (KEYS) {
-                            const ulonglong2 sx = *reinterpret_cast<const ulonglong2 *>(stats + 32 * w + i);
-                            const ulonglong2 sy = *reinterpret_cast<const ulonglong2 *>(stats + N + 32 * w + i);
-                            x[0] = sx.x; x[1] = sx.y; y[0] = sy.x; y[1] = sy.y;
-                        }
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int at = i + 2 * h;
-                            const float2 e = parts(fma2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c, x[h]));
-                            const float2 w2 = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                            const pair dp = pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1]));
-                            const float2 slope = parts(mul2(pair_of(w2.x, w2.y), kScaled ? fma2(dp, f, y[h]) : add2(dp, y[h])));
-                            if (KEYS) {
-                                p[at / 2] = pack2<T>(w2.x, w2.y) & seen_row;
-                                q[at / 2] = pack2<T>(slope.x, slope.y) & seen_row;
-                            } else {
-                                q[at / 2] = pack2<T>(slope.x, slope.y);
-                            }
+                            p[at / 2] = pack2<T>(w2.x, w2.y) & seen_row;
+                            q[at / 2] = pack2<T>(slope.x, slope.y) & seen_row;
+                        } else {
+                            q[at / 2] = pack2<T>(slope.x, slope.y);
                         }
                     }
-                    if (!KEYS && !all) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            q[i] &= ((seen[w] >> (2 * i)) & 1u ? 0x0000ffffu : 0u) | ((seen[w] >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
-                    }
-                    // in place: these columns have been read, by the lanes that own their rows
-                    if (KEYS) tmem_store16(rows + 16 * w, p);
-                    tmem_store16(rows + 64 + 16 * w, q);
                 }
+                if (!KEYS && !all) {
+                    const unsigned word = half ? seen[1] : seen[0];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) q[i] &= ((word >> (2 * i)) & 1u ? 0x0000ffffu : 0u) | ((word >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+                }
+                // in place: this lane has read these columns
+                if (KEYS) tmem_store16(rows, p);
+                tmem_store16(rows + 64, q);
                 tmem_stored();
             }
             before_sync();
@@ -665,27 +820,27 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         if (done) after_sync();
         const float back = exp2f(-Range<T>::kShift);
         const long long all_rows = KEYS ? (long long)a.n_k * a.kv_heads : (long long)a.n_q * a.heads;
-        // KEYS: the first group writes dv and the second dk; else they share the columns
+        // KEYS: the first group writes dv and the second dk; else they share the columns, as the halves do
         float *to_part = a.splits > 1 ? (KEYS && g == 0 ? a.part2 : a.part) + blockIdx.z * all_rows * a.dim : nullptr;
         void *to = KEYS && g == 0 ? a.to2 : a.to;
         const float by = KEYS && g == 0 ? back : a.scale * back / factor;
         const bool some = done && (varies || (KEYS && g == 0));
-        for (int d = KEYS ? 0 : 16 * g; d < a.dim; d += KEYS ? 16 : 32) {
+        const Rows place(row * a.dim, store);
+        for (int d = KEYS ? 16 * half : 16 * (2 * g + half); d < a.dim; d += KEYS ? 32 : 64) {
             unsigned o[16] = {};
             if (some) {
                 tmem_load16(o, lanes + (KEYS && g == 0 ? F::kSums2 : F::kSums) + d);
                 tmem_loaded();
                 use_after(o);
             }
-            if (store) store16<T>(to, to_part, row * a.dim, d, a.dim, o, some ? by : 0.f);
-            __syncwarp();
+            store16<T>(to, to_part, place, d, a.dim, o, some ? by : 0.f);
         }
     }
     if (steps > 0) {
         before_sync();
         __syncthreads();
         after_sync();
-        if (warp == 11) tmem_free(tmem, F::kColumns);
+        if (warp == 19) tmem_free(tmem, F::kColumns);
     }
 }
 
@@ -733,10 +888,11 @@ bool rows_fit(const Strided &s)
     return (reinterpret_cast<uintptr_t>(s.p) & 15u) == 0 && s.row > 0 && s.head > 0 && s.row % 8 == 0 && s.head % 8 == 0 && s.row < most && s.head < most;
 }
 
-template <typename K> int launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const Args &a, const Maps &maps)
+template <typename K, typename... More>
+int launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const Args &a, const Maps &maps, More... more)
 {
     HGC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    HGC_CUDA_TRY(launch_pdl(kernel, grid, threads, smem, stream, a, maps));
+    HGC_CUDA_TRY(launch_pdl(kernel, grid, threads, smem, stream, a, maps, more...));
     HGC_LAUNCH_CHECK();
     return HGC_OK;
 }
@@ -751,8 +907,11 @@ template <typename T, int CHUNKS, bool KEYS> int grad_mma(const Args &a, const M
 
 template <typename T, int CHUNKS> int forward_mma(const Args &a, const Maps &maps, cudaStream_t stream)
 {
-    const dim3 grid((unsigned)tile_count(a.n_q, 2 * (kMmaRows / a.pack), a.n_events), a.heads / a.pack, a.splits);
-    return launch(forward_mma_kernel<T, CHUNKS>, grid, Forward<CHUNKS>::kThreads, Forward<CHUNKS>::kSmem, stream, a, maps);
+    const long long tiles = tile_count(a.n_q, 2 * (kMmaRows / a.pack), a.n_events), items = tiles * (a.heads / a.pack) * a.splits;
+    if (items > 0x7fffffff) return HGC_ERR_UNSUPPORTED;
+    const int blocks = items < sm_count() ? (int)items : sm_count();
+    if (items > blocks) HGC_CUDA_TRY(cudaMemsetAsync(a.counter, 0, sizeof(int), stream));
+    return launch(forward_mma_kernel<T, CHUNKS>, blocks, Forward<CHUNKS>::kThreads, Forward<CHUNKS>::kSmem, stream, a, maps, (int)tiles, (int)items);
 }
 
 }  // namespace

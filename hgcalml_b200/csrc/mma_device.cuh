@@ -139,13 +139,14 @@ __device__ __forceinline__ void product_along(unsigned d, unsigned a, unsigned b
     for (int k = 0; k < 4 * CHUNKS; k++)
         if (k < steps) product(d, oa + (k / 4 * A_APART + k % 4 * 32) / 16, ob + (k / 4 * B_APART + k % 4 * 32) / 16, shape, k > 0);
 }
-// d[128 x columns] (+)= a[128 x 16 STEPS, in tensor memory] b[16 STEPS rows], tiles of 64 columns APART bytes behind each other
+// d[128 x columns] (+)= a[128 x 16 STEPS] b[16 STEPS rows], tiles of 64 columns APART bytes behind each other.  a is in tensor
+// memory, its halves where the 32-bit values were that they come from: the second one begins 8 STEPS columns behind the first.
 template <int STEPS, unsigned APART>
 __device__ __forceinline__ void product_over(unsigned d, unsigned a, unsigned b, unsigned shape, bool add)
 {
     const unsigned long long ob = operand(b, APART);
 #pragma unroll
-    for (int k = 0; k < STEPS; k++) product_from_tmem(d, a + 8 * k, ob + 2048 / 16 * k, shape, add || k > 0);
+    for (int k = 0; k < STEPS; k++) product_from_tmem(d, a + 8 * k + (2 * k >= STEPS ? 4 * STEPS : 0), ob + 2048 / 16 * k, shape, add || k > 0);
 }
 
 // ------------------------------------------------------------------------------------------------------ tensor memory
