@@ -194,7 +194,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 it.split = split;
                 break;
             }
-            if (taken >= F::kItems) ok = wait_warp(item_empty + 8 * item.at, item.turn ^ 1, gave_up, a.status);
+            if (taken >= F::kItems) ok = wait_warp<true>(item_empty + 8 * item.at, item.turn ^ 1, gave_up, a.status);
             if (!ok) break;
             if (lane == 0) {
                 s_item[item.at] = it;
@@ -334,7 +334,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
         unsigned go_turn = 0;
         bool ok = true;
         while (ok) {
-            ok = wait_warp(item_full + 8 * item.at, item.turn, gave_up, a.status);
+            ok = wait_warp<true>(item_full + 8 * item.at, item.turn, gave_up, a.status);
             const Item it = s_item[item.at];
             __syncwarp();
             if (lane == 0) arrive(item_empty + 8 * item.at);
@@ -346,9 +346,9 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 unsigned seen[W];
                 const bool all = seen_words<W>(seen, a.mask, k0, it.keys_end - k0);
                 if (a.mask != nullptr) {
-                    ok = wait_warp(full + 8 * kv.at, kv.turn, gave_up, a.status);
+                    ok = wait_warp<true>(full + 8 * kv.at, kv.turn, gave_up, a.status);
                 } else {
-                    ok = wait_warp(go, go_turn, gave_up, a.status);
+                    ok = wait_warp<true>(go, go_turn, gave_up, a.status);
                     go_turn ^= 1;
                 }
                 if (!ok) break;
@@ -374,7 +374,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             both_halves[half * kMmaRows + r] = mine;
             __syncwarp();
             if (lane == 0) arrive(meeting);
-            ok = wait_warp(meeting, meet_turn, gave_up, a.status) && ok;
+            ok = wait_warp<true>(meeting, meet_turn, gave_up, a.status) && ok;
             meet_turn ^= 1;
             return both_halves[(half ^ 1) * kMmaRows + r];
         };
@@ -386,7 +386,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
         Ring<B> buffer;
         unsigned o_turn = 0, clean_turns = 0;
         while (ok) {
-            ok = wait_warp(item_full + 8 * item.at, item.turn, gave_up, a.status);
+            ok = wait_warp<true>(item_full + 8 * item.at, item.turn, gave_up, a.status);
             const Item it = s_item[item.at];
             __syncwarp();
             if (lane == 0) arrive(item_empty + 8 * item.at);
@@ -406,8 +406,8 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     continue;
                 }
                 const unsigned rows = lanes + N * buffer.at + half * (N / 2);
-                ok = wait_warp(s_full + 8 * buffer.at, buffer.turn, gave_up, a.status) && ok;
-                if (!whole_step) ok = wait_warp(clean + 8 * kv.at, clean_turn, gave_up, a.status) && ok;
+                ok = wait_warp<true>(s_full + 8 * buffer.at, buffer.turn, gave_up, a.status) && ok;
+                if (!whole_step) ok = wait_warp<true>(clean + 8 * kv.at, clean_turn, gave_up, a.status) && ok;
                 // every phase of the sums' barrier is waited for: here, where they are scaled, else when this step's weights are done
                 bool summed = j == 0;
                 if (!idle) {
@@ -418,8 +418,6 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     const float *bias = s_bias + kv.at * N + half * (N / 2);
                     const auto read = [&](int w) {
                         tmem_load32(s, rows + 32 * w);
-                        tmem_loaded();
-                        use_after(s);
                         if (whole_step) return;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
@@ -445,7 +443,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     if (j == 0) {
                         top = next;
                     } else if (__any_sync(0xffffffffu, grown)) {
-                        ok = wait_warp(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
+                        ok = wait_warp<true>(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
                         summed = true;
                         after_sync();
                         const float shrink = exp2_fast((top - (next == -INFINITY ? 0.f : next)) * c);
@@ -454,8 +452,6 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                         for (int d = 16 * half; d < a.dim; d += 32) {
                             unsigned o[16];
                             tmem_load16(o, out + d);
-                            tmem_loaded();
-                            use_after(o);
 #pragma unroll
                             for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
                             tmem_store16(out + d, o);
@@ -483,7 +479,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     sum += both.x + both.y;
                     tmem_stored();
                 }
-                if (!summed) ok = wait_warp(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
+                if (!summed) ok = wait_warp<true>(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
                 o_turn ^= 1;
                 before_sync();
                 __syncwarp();
@@ -491,7 +487,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 buffer.go(groups == 1 || (g == 1 && j == it.steps - 1) ? 1 : 2);
             }
             if (g >= groups) continue;
-            const bool done = it.steps > 0 && ok && wait_warp(o_full + 8 * g, o_turn ^ 1, gave_up, a.status);
+            const bool done = it.steps > 0 && ok && wait_warp<true>(o_full + 8 * g, o_turn ^ 1, gave_up, a.status);
             if (done) after_sync();
             const long long row = (long long)(it.begin + g * tokens + r / a.pack) * a.heads + it.head0 + r % a.pack;
             if (it.steps > 0 && !idle) sum += exchange(maxima + 2 * 2 * kMmaRows, sum);
@@ -509,8 +505,6 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     unsigned o[16] = {};
                     if (done) {
                         tmem_load16(o, out + d);
-                        tmem_loaded();
-                        use_after(o);
                     }
                     store16<T>(a.to, to_part, to, d, a.dim, o, inv);
                 }
@@ -560,10 +554,10 @@ __device__ __forceinline__ void clear_rows(unsigned tile, int chunks, int tile_r
 // thread each, that does nothing else, and rows that must not be summed over are cleared by a warp of their own.
 // (Two blocks of 256 columns, each with one buffer, waited for products two thirds of the time: 16k x 16k rows, 8 heads of 64, 3.2 ms.)
 template <int CHUNKS, bool KEYS> struct Grad {
-    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 640;
+    static constexpr int kStep = kMmaGradStep, kStages = CHUNKS == 1 ? 6 : 4, kThreads = 384;
     static constexpr int kTileBytes = kStep * kTile * CHUNKS, kKeptBytes = kMmaRows * kTile * CHUNKS;
     static constexpr int kBuffers = KEYS && CHUNKS == 2 ? 2 : 3, kSums = 128 * kBuffers, kSums2 = kSums + 64 * CHUNKS, kColumns = 512;
-    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 16 * 2 * 32 * 4, kSmem = kTiles + kStats + 512;
+    static constexpr int kTiles = 2 * kKeptBytes + 2 * kStages * kTileBytes, kStats = 8 * 2 * kStep * 4, kSmem = kTiles + kStats + 512;
     static constexpr int kBarriers = 4 + 3 * kStages + 3 * kBuffers;
     static_assert((KEYS ? kSums2 : kSums) + 64 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= 512, "room");
 };
@@ -603,19 +597,19 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         if (t == 0) {
             for (int i = 0; i < F::kBarriers; i++) {
                 const unsigned at = bar + 8 * i;
-                barrier_init(at, at >= p_full && at < used ? 8 : at == kept_full ? 2 : 1);
+                barrier_init(at, at >= p_full && at < used ? 4 : at == kept_full ? 2 : 1);
             }
             barrier_init_done();
             *gave_up = 0;
         }
-        if (warp == 19) tmem_alloc(s_tmem, F::kColumns);
+        if (warp == 11) tmem_alloc(s_tmem, F::kColumns);
         before_sync();
         __syncthreads();
         after_sync();
     }
     const unsigned tmem = steps > 0 ? *s_tmem : 0;
 
-    if (warp == 16) {
+    if (warp == 8) {
         if (steps > 0 && elect()) {
             const int kept_head = KEYS ? kv : blockIdx.y * a.pack;
             arrive_expect(kept_full, KEYS ? 2 * F::kKeptBytes : 2 * CHUNKS * kTile * a.pack * tokens);
@@ -643,7 +637,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             for (int j = max(0, copies - F::kStages); j < copies; j++) drain(full + 8 * (j % F::kStages), j / F::kStages & 1);
         }
         __syncwarp();
-    } else if (warp == 17) {
+    } else if (warp == 9) {
         if (steps > 0 && elect()) {
             const int depth = (a.dim + 15) / 16;
             const unsigned shape_s = shape<T>(N, false);
@@ -671,7 +665,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             drain(scores_done, 0);
         }
         __syncwarp();
-    } else if (warp == 18) {
+    } else if (warp == 10) {
         if (steps > 0 && elect()) {
             const unsigned shape_o = shape<T>((a.dim + 15) / 16 * 16, true);
             int stage = 0, b = 0;
@@ -695,7 +689,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             drain(all_done, 0);
         }
         __syncwarp();
-    } else if (warp == 19) {
+    } else if (warp == 11) {
         if (KEYS && steps > 0 && a.pack * tokens < N) {  // rows that no copy writes
             for (int i = 0; i < F::kStages; i++) {
                 clear_rows(s_step + i * F::kTileBytes, CHUNKS, N, a.pack * tokens, N);
@@ -724,15 +718,14 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             if (lane == 0) arrive(clean + 8 * stage);
         }
     } else {
-        // the lane has row r in every other step, beginning with step g, and half of its columns
-        const int g = warp >> 3, half = (warp >> 2) & 1, r = t & 127;
+        const int g = warp >> 2, r = t & 127;  // the lane has row r in every other step, beginning with step g
         const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21);
         const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;
         const float scale = a.scale * kLog2e, factor = slope_factor<T>(a);
         const pair c = pair_of(scale, scale), f = pair_of(factor, factor);
         // KEYS: of the columns, in the warp's own shared memory, negative, first the exponents' and then the slopes'.  Else of this
         // lane's row.
-        float *stats = reinterpret_cast<float *>(s_raw + F::kTiles) + warp * 2 * 32;
+        float *stats = reinterpret_cast<float *>(s_raw + F::kTiles) + warp * 2 * N;
         const long long row = KEYS ? ((long long)(tile.begin + r) * a.kv_heads + kv)
                                    : (long long)(tile.begin + r / a.pack) * a.heads + blockIdx.y * a.pack + r % a.pack;
         pair shift = 0, delta = 0;
@@ -744,26 +737,39 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             shift = pair_of(-stat.x, -stat.x);
             delta = pair_of(-stat.y * factor, -stat.y * factor);
         }
-        // KEYS: the lane asks for a column of the next step
-        const int column = 32 * half + lane, my_token = KEYS ? column / a.pack : 0, my_head = KEYS ? kv * a.group + column % a.pack : 0;
-        int token = first_row + my_token, p_next = 0;
+        // KEYS: the lane asks for two columns of the next step
+        int token[2], head[2], p_next = 0;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            token[w] = first_row + (KEYS ? (32 * w + lane) / a.pack : 0);
+            head[w] = KEYS ? kv * a.group + (32 * w + lane) % a.pack : 0;
+        }
+        float2 mine[W];
         const auto next_stats = [&](int ahead) {
-            for (p_next += ahead; p_next >= packs; p_next -= packs) token += rows_a_step;
-            return column < a.pack * tokens && token < others.y ? a.stats[(long long)token * a.heads + my_head + p_next * a.pack] : make_float2(INFINITY, 0.f);
+            for (p_next += ahead; p_next >= packs; p_next -= packs) {
+                token[0] += rows_a_step;
+                token[1] += rows_a_step;
+            }
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                mine[w] = 32 * w + lane < a.pack * tokens && token[w] < others.y
+                    ? a.stats[(long long)token[w] * a.heads + head[w] + p_next * a.pack] : make_float2(INFINITY, 0.f);
         };
-        float2 mine = make_float2(INFINITY, 0.f);
-        if (KEYS && g < steps) mine = next_stats(g);
+        if (KEYS && g < steps) next_stats(g);
         int b = g, row_k = first_row + g * N;
         unsigned turn = 0;
         for (int j = g; j < steps; j += 2) {
-            const unsigned rows = lanes + 128 * b + 32 * half;
+            const unsigned rows = lanes + 128 * b;
             unsigned seen[W];
             bool all = true;
             if (KEYS) {
                 __syncwarp();
-                stats[lane] = -mine.x;
-                stats[32 + lane] = -mine.y * factor;
-                if (j + 2 < steps) mine = next_stats(2);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    stats[32 * w + lane] = -mine[w].x;
+                    stats[N + 32 * w + lane] = -mine[w].y * factor;
+                }
+                if (j + 2 < steps) next_stats(2);
                 __syncwarp();
             } else if (j >= dirty) {
                 all = seen_words<W>(seen, a.mask, row_k, others.y - row_k);
@@ -771,43 +777,42 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             row_k += 2 * N;
             if (wait_warp(s_full + 8 * b, turn, gave_up, a.status) && !idle) {
                 after_sync();
-                unsigned s[32], d[32], p[16], q[16];
-                tmem_load32(s, rows);
-                tmem_load32(d, rows + 64);
-                tmem_loaded();
-                use_after(s);
-                use_after(d);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    pair x[2] = {shift, shift}, y[2] = {delta, delta};
-                    if (KEYS) {
-                        const ulonglong2 sx = *reinterpret_cast<const ulonglong2 *>(stats + i);
-                        const ulonglong2 sy = *reinterpret_cast<const ulonglong2 *>(stats + 32 + i);
-                        x[0] = sx.x; x[1] = sx.y; y[0] = sy.x; y[1] = sy.y;
-                    }
+                for (int w = 0; w < W; w++) {
+                    unsigned s[32], d[32], p[16], q[16];
+                    tmem_load32(s, rows + 32 * w, d, rows + 64 + 32 * w);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int at = i + 2 * h;
-                        const float2 e = parts(fma2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c, x[h]));
-                        const float2 w2 = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                        const pair dp = pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1]));
-                        const float2 slope = parts(mul2(pair_of(w2.x, w2.y), kScaled ? fma2(dp, f, y[h]) : add2(dp, y[h])));
+                    for (int i = 0; i < 32; i += 4) {
+                        pair x[2] = {shift, shift}, y[2] = {delta, delta};
                         if (KEYS) {
-                            p[at / 2] = pack2<T>(w2.x, w2.y) & seen_row;
-                            q[at / 2] = pack2<T>(slope.x, slope.y) & seen_row;
-                        } else {
-                            q[at / 2] = pack2<T>(slope.x, slope.y);
+                            const ulonglong2 sx = *reinterpret_cast<const ulonglong2 *>(stats + 32 * w + i);
+                            const ulonglong2 sy = *reinterpret_cast<const ulonglong2 *>(stats + N + 32 * w + i);
+                            x[0] = sx.x; x[1] = sx.y; y[0] = sy.x; y[1] = sy.y;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int at = i + 2 * h;
+                            const float2 e = parts(fma2(pair_of(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), c, x[h]));
+                            const float2 w2 = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            const pair dp = pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1]));
+                            const float2 slope = parts(mul2(pair_of(w2.x, w2.y), kScaled ? fma2(dp, f, y[h]) : add2(dp, y[h])));
+                            if (KEYS) {
+                                p[at / 2] = pack2<T>(w2.x, w2.y) & seen_row;
+                                q[at / 2] = pack2<T>(slope.x, slope.y) & seen_row;
+                            } else {
+                                q[at / 2] = pack2<T>(slope.x, slope.y);
+                            }
                         }
                     }
-                }
-                if (!KEYS && !all) {
-                    const unsigned word = half ? seen[1] : seen[0];
+                    if (!KEYS && !all) {
+                        const unsigned word = w ? seen[1] : seen[0];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) q[i] &= ((word >> (2 * i)) & 1u ? 0x0000ffffu : 0u) | ((word >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+                        for (int i = 0; i < 16; i++) q[i] &= ((word >> (2 * i)) & 1u ? 0x0000ffffu : 0u) | ((word >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
+                    }
+                    // in place: this lane has read these columns
+                    if (KEYS) tmem_store16(rows + 32 * w, p);
+                    tmem_store16(rows + 64 + 32 * w, q);
                 }
-                // in place: this lane has read these columns
-                if (KEYS) tmem_store16(rows, p);
-                tmem_store16(rows + 64, q);
                 tmem_stored();
             }
             before_sync();
@@ -820,18 +825,16 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         if (done) after_sync();
         const float back = exp2f(-Range<T>::kShift);
         const long long all_rows = KEYS ? (long long)a.n_k * a.kv_heads : (long long)a.n_q * a.heads;
-        // KEYS: the first group writes dv and the second dk; else they share the columns, as the halves do
+        // KEYS: the first group writes dv and the second dk; else they share the columns
         float *to_part = a.splits > 1 ? (KEYS && g == 0 ? a.part2 : a.part) + blockIdx.z * all_rows * a.dim : nullptr;
         void *to = KEYS && g == 0 ? a.to2 : a.to;
         const float by = KEYS && g == 0 ? back : a.scale * back / factor;
         const bool some = done && (varies || (KEYS && g == 0));
         const Rows place(row * a.dim, store);
-        for (int d = KEYS ? 16 * half : 16 * (2 * g + half); d < a.dim; d += KEYS ? 32 : 64) {
+        for (int d = KEYS ? 0 : 16 * g; d < a.dim; d += KEYS ? 16 : 32) {
             unsigned o[16] = {};
             if (some) {
                 tmem_load16(o, lanes + (KEYS && g == 0 ? F::kSums2 : F::kSums) + d);
-                tmem_loaded();
-                use_after(o);
             }
             store16<T>(to, to_part, place, d, a.dim, o, some ? by : 0.f);
         }
@@ -840,7 +843,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         before_sync();
         __syncthreads();
         after_sync();
-        if (warp == 19) tmem_free(tmem, F::kColumns);
+        if (warp == 11) tmem_free(tmem, F::kColumns);
     }
 }
 

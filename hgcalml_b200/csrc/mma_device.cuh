@@ -52,8 +52,10 @@ __device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity)
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool wait_long(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
+__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
 {
+    for (int i = 0; i < 16; i++)
+        if (try_wait(bar, parity)) return true;
     const long long begin = clock64();
     do {
         for (int i = 0; i < 64; i++)
@@ -64,16 +66,20 @@ __device__ __forceinline__ bool wait_long(unsigned bar, unsigned parity, volatil
     flag_status(status, HGC_STATUS_ITERATION_CAP);
     return false;
 }
-__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
+static __device__ __noinline__ bool wait_out_of_line(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
 {
-    for (int i = 0; i < 16; i++)
-        if (try_wait(bar, parity)) return true;
-    return wait_long(bar, parity, gave_up, status);
+    return wait(bar, parity, gave_up, status);
 }
-// the same for a warp, whose lanes go on together
+// For a warp, whose lanes go on together.  LITTLE: with few instructions here, for code that the instruction caches hardly hold
+// (forward pass 1.05 -> 0.91 ms at 16k x 16k rows, 8 heads of 64); without it the sums and scores are issued sooner (backward pass
+// 2.07 -> 1.84).
+template <bool LITTLE = false>
 __device__ __forceinline__ bool wait_warp(unsigned bar, unsigned parity, volatile int *gave_up, unsigned *status)
 {
-    return __all_sync(0xffffffffu, wait(bar, parity, gave_up, status));
+    bool done;
+    if (LITTLE) done = try_wait(bar, parity) || wait_out_of_line(bar, parity, gave_up, status);
+    else done = wait(bar, parity, gave_up, status);
+    return __all_sync(0xffffffffu, done);
 }
 // A wait for what is under way whatever happened before.
 __device__ __forceinline__ void drain(unsigned bar, unsigned parity)
@@ -162,18 +168,34 @@ __device__ __forceinline__ void tmem_free(unsigned address, unsigned columns)
 }
 #define HGC_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
 #define HGC_R16(v, i) HGC_R4(v, i), HGC_R4(v, i + 4), HGC_R4(v, i + 8), HGC_R4(v, i + 12)
+// the same where an input follows that must not share a register with what is written first
+#define HGC_E4(v, i) "=&r"(v[i]), "=&r"(v[i + 1]), "=&r"(v[i + 2]), "=&r"(v[i + 3])
+#define HGC_E16(v, i) HGC_E4(v, i), HGC_E4(v, i + 4), HGC_E4(v, i + 8), HGC_E4(v, i + 12)
 #define HGC_S4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
 #define HGC_S16(v, i) HGC_S4(v, i), HGC_S4(v, i + 4), HGC_S4(v, i + 8), HGC_S4(v, i + 12)
-// A lane's row of 32 or 16 columns.  Warp w of a group of four reaches rows 32 w .. 32 w + 31.
+// A lane's row of 32 or 16 columns.  Warp w of a group of four reaches rows 32 w .. 32 w + 31.  A load and the wait for it are one
+// statement: in between, its registers are written at any time, and the compiler, to which they are values that are there already,
+// may have moved these values elsewhere and given the registers to something else.  (Loads and waits apart from each other faulted
+// in some builds of the kernels for wide heads, at no fixed place.)
+#define HGC_LD32 "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
 __device__ __forceinline__ void tmem_load32(unsigned (&v)[32], unsigned address)
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
-                 "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+    asm volatile(HGC_LD32 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
+                 "%25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
                  : HGC_R16(v, 0), HGC_R16(v, 16) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(unsigned (&v)[32], unsigned address, unsigned (&w)[32], unsigned address2)
+{
+    asm volatile(HGC_LD32 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
+                 "%25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+                 HGC_LD32 "{%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, "
+                 "%55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : HGC_E16(v, 0), HGC_E16(v, 16), HGC_E16(w, 0), HGC_E16(w, 16) : "r"(address), "r"(address2) : "memory");
 }
 __device__ __forceinline__ void tmem_load16(unsigned (&v)[16], unsigned address)
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
                  : HGC_R16(v, 0) : "r"(address) : "memory");
 }
 __device__ __forceinline__ void tmem_store16(unsigned address, const unsigned (&v)[16])
@@ -181,12 +203,6 @@ __device__ __forceinline__ void tmem_store16(unsigned address, const unsigned (&
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  :: "r"(address), HGC_S16(v, 0) : "memory");
 }
-// What was loaded may be used: the registers pass through, so that no use of them moves ahead of the wait.
-#define HGC_P4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
-#define HGC_P16(v, i) HGC_P4(v, i), HGC_P4(v, i + 4), HGC_P4(v, i + 8), HGC_P4(v, i + 12)
-__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void use_after(unsigned (&v)[32]) { asm volatile("" : HGC_P16(v, 0), HGC_P16(v, 16) :: "memory"); }
-__device__ __forceinline__ void use_after(unsigned (&v)[16]) { asm volatile("" : HGC_P16(v, 0) :: "memory"); }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_fast(float x)  // relative error 2^-22
