@@ -18,13 +18,17 @@ namespace hgc {
 namespace {
 
 constexpr int kMaxDim = 128;
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 32;  // rows of a block, whose angles are kept
+constexpr int kThreads = 256, kBlocksPerSm = 4;
+constexpr int kMaxTokens = 64;  // rows of a block, whose angles are kept
 
+// Where the partner of a column is.  The small numbers: that many columns further on in the same lane, for axes of few columns.
 enum Pairs {
-    kNeighbours,  // columns 2 i and 2 i + 1: in one lane
-    kHalves,      // columns i and i + pairs, whole vectors apart: in two lanes
-    kAnywhere     // through shared memory
+    kNeighbours = 1,  // columns 2 i and 2 i + 1
+    kTwoOn = 2,
+    kFourOn = 4,
+    kHalves = 16,     // columns i and i + pairs, whole vectors apart: in two lanes
+    kBothHalves = 17, // columns i and i + pairs, all that there are: a lane has a vector of either half
+    kAnywhere = 18    // through shared memory
 };
 
 struct Set {
@@ -38,7 +42,7 @@ struct Set {
 struct Call {
     Set set[2];
     double turns[kMaxDim / 2];  // turns per unit of position
-    int dim, rotary, axes, pairs, position_type, interleaved, lanes_log2;
+    int dim, rotary, axes, pairs, axis_factor, position_type, interleaved, lanes_log2;
     float eps;
 };
 
@@ -51,40 +55,87 @@ template <> __device__ __forceinline__ float rounded<float>(float v) { return v;
 template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V columns from one address; a whole 16-byte vector, or one column
+// V columns at one address; a whole 16-byte vector, or one column
 template <typename T, int V> struct Vec { alignas(V == 1 ? sizeof(T) : 16) T v[V]; };
 
-template <typename T, int V>
-__device__ __forceinline__ void load(float (&to)[V], const T *__restrict__ from, bool in)
+// two columns at a time where they come in 32 bits
+__device__ __forceinline__ float2 two(unsigned v, __nv_bfloat16) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+__device__ __forceinline__ float2 two(unsigned v, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+__device__ __forceinline__ unsigned both(float a, float b, __nv_bfloat16)
 {
-    Vec<T, V> q = {};
-    if (in) q = *reinterpret_cast<const Vec<T, V> *>(from);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&r);
+}
+__device__ __forceinline__ unsigned both(float a, float b, __half)
+{
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&r);
+}
+template <typename T, int V>
+__device__ __forceinline__ void to_floats(float (&to)[V], const Vec<T, V> &from)
+{
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(&from);
+        const unsigned u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < V; i++) to[i] = in ? as_float(q.v[i]) : 0.f;
+        for (int i = 0; i < 4; i++) {
+            const float2 f = two(u[i], T{});
+            to[2 * i] = f.x;
+            to[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) to[i] = as_float(from.v[i]);
+    }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store(T *__restrict__ to, const float (&from)[V])
 {
-    Vec<T, V> q;
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        *reinterpret_cast<uint4 *>(to) = make_uint4(both(from[0], from[1], T{}), both(from[2], from[3], T{}), both(from[4], from[5], T{}),
+                                                    both(from[6], from[7], T{}));
+    } else {
+        Vec<T, V> q;
 #pragma unroll
-    for (int i = 0; i < V; i++) q.v[i] = rounded<T>(from[i]);
-    *reinterpret_cast<Vec<T, V> *>(to) = q;
+        for (int i = 0; i < V; i++) q.v[i] = rounded<T>(from[i]);
+        *reinterpret_cast<Vec<T, V> *>(to) = q;
+    }
 }
 
-// The angles of rows [first, first + n) of a set: (cos, sin) of every pair of columns.
-__device__ __forceinline__ void angles(const Call &c, const Set &s, int first, int n, float2 *__restrict__ table)
+// Where the angle of a pair is in a row's part of the table.  Lanes read two angles at a time, 16 bytes; kept in the order of the
+// lanes these do not meet in the same banks.
+template <int V, Pairs P> __device__ __forceinline__ int place(int pair, int n_pairs)
 {
-    const int pairs = c.rotary / 2;
-    for (int i = threadIdx.x; i < n * pairs; i += kThreads) {
-        const int token = i / pairs, p = i - token * pairs, axis = p / c.pairs;
+    constexpr int A = P == kHalves || P == kBothHalves ? V : V / 2;  // angles of a lane
+    if constexpr (P == kAnywhere || A < 4) return pair;
+    else return pair < n_pairs / A * A ? (pair % A / 2 * (n_pairs / A) + pair / A) * 2 + pair % 2 : pair;
+}
+// The angles of rows [first, first + n) of a set: (cos, sin) of every pair of columns.  The whole turns go in double: what is left is
+// exact to 2^-53 of the position's turns.
+template <typename T, int V, Pairs P>
+__device__ __forceinline__ void angles(const Call &c, const Set &s, const double *__restrict__ turns, int first, int n, float2 *__restrict__ table)
+{
+    const int pairs = c.rotary / 2, step_t = kThreads / pairs, step_p = kThreads - step_t * pairs;
+    int token = threadIdx.x / pairs, p = threadIdx.x - token * pairs;
+    while (token < n) {
+        const int axis = p * c.axis_factor >> 16;  // p / c.pairs
         const long long at = (long long)(first + token) * c.axes + axis;
         const double x = c.position_type == HGC_POSITION_FLOAT32 ? (double)static_cast<const float *>(s.positions)[at]
                        : c.position_type == HGC_POSITION_INT32 ? (double)static_cast<const int *>(s.positions)[at]
                                                                : (double)static_cast<const long long *>(s.positions)[at];
-        const double t = x * c.turns[p - axis * c.pairs];
+        const double turn = turns[p - axis * c.pairs];
         float2 cs;
-        sincospif(2.f * (float)(t - rint(t)), &cs.y, &cs.x);
-        table[i] = cs;
+        const float part = (float)fma(x, turn, -rint(x * turn));
+        if constexpr (sizeof(T) == 4) {
+            sincospif(2.f * part, &cs.y, &cs.x);
+        } else {  // off by 2^-20 at most, where results are rounded to 2^-11 or less
+            cs.y = __sinf(6.283185307f * part);
+            cs.x = __cosf(6.283185307f * part);
+        }
+        table[token * pairs + place<V, P>(p, pairs)] = cs;
+        token += step_t;
+        p += step_p;
+        if (p >= pairs) { p -= pairs; token++; }
     }
 }
 
@@ -93,6 +144,8 @@ template <int V, int E, Pairs P> struct Columns {
     int column[E];       // first of V, or -1
     int pair[E];         // its angle in a row of the table (kNeighbours, kHalves: that of the first column)
     bool turned[E];
+    int at, step;        // where the lane's first two angles are, and from there to its next two
+    bool whole;          // all of its columns turn
     int partner_lane;    // kHalves
     float sign;          // kHalves: of the sine
 
@@ -100,14 +153,16 @@ template <int V, int E, Pairs P> struct Columns {
     {
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int d = (lane_in_row + lanes * e) * V;
+            const int d = P == kBothHalves ? lane_in_row * V + c.pairs * e : (lane_in_row + lanes * e) * V;
             column[e] = d < c.dim ? d : -1;
             turned[e] = d < c.rotary;
             pair[e] = 0;
         }
+        whole = column[0] >= 0 && column[0] + V <= c.rotary;
         partner_lane = lane_id();
         sign = 0.f;
-        if constexpr (P == kNeighbours) pair[0] = column[0] / 2;
+        if constexpr (P == kBothHalves) pair[0] = lane_in_row * V;
+        if constexpr (P < kHalves) pair[0] = max(column[0], 0) / 2;  // a lane's columns hold whole axes, or neighbours
         if constexpr (P == kHalves) {
             const int span = 2 * c.pairs, axis = max(column[0], 0) / span, off = max(column[0], 0) - axis * span;
             const bool second = off >= c.pairs;
@@ -115,6 +170,11 @@ template <int V, int E, Pairs P> struct Columns {
             sign = second ? 1.f : -1.f;
             if (turned[0] && column[0] >= 0) partner_lane += (second ? -c.pairs : c.pairs) / V;
         }
+        constexpr int A = P == kHalves || P == kBothHalves ? V : V / 2;
+        const int n_pairs = c.rotary / 2;
+        const bool in_order = A < 4 || pair[0] >= n_pairs / A * A;
+        at = in_order ? pair[0] : pair[0] / A * 2;
+        step = in_order ? 2 : n_pairs / A * 2;
     }
 };
 
@@ -123,26 +183,37 @@ template <int V, int E, Pairs P>
 __device__ __forceinline__ void turn(float (&v)[E][V], const Columns<V, E, P> &k, const Call &c, const float2 *__restrict__ table, float direction,
                                      float *__restrict__ row_buffer)
 {
-    if constexpr (P == kNeighbours) {
+    if constexpr (P < kHalves) {
+        // pair j of the lane: columns (j / P) 2 P + j % P and P further on
         if (k.turned[0] && k.column[0] >= 0) {
 #pragma unroll
-            for (int i = 0; i < V; i += 2) {
-                if (k.column[0] + i >= c.rotary) break;
-                const float2 cs = table[k.pair[0] + i / 2];
-                const float a = v[0][i], b = v[0][i + 1], sn = cs.y * direction;
-                v[0][i] = a * cs.x - b * sn;
-                v[0][i + 1] = b * cs.x + a * sn;
+            for (int j = 0; j < V / 2; j++) {
+                const int first = j / P * (2 * P) + j % P;
+                if (!k.whole && k.column[0] + first >= c.rotary) break;
+                const float2 cs = table[k.at + j / 2 * k.step + j % 2];
+                const float a = v[0][first], b = v[0][first + P], sine = cs.y * direction;
+                v[0][first] = a * cs.x - b * sine;
+                v[0][first + P] = b * cs.x + a * sine;
             }
+        }
+    } else if constexpr (P == kBothHalves) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float2 cs = table[k.at + i / 2 * k.step + i % 2];
+            const float a = v[0][i], b = v[1][i], sine = cs.y * direction;
+            v[0][i] = a * cs.x - b * sine;
+            v[1][i] = b * cs.x + a * sine;
         }
     } else if constexpr (P == kHalves) {
         float other[V];
 #pragma unroll
         for (int i = 0; i < V; i++) other[i] = __shfl_sync(0xffffffffu, v[0][i], k.partner_lane);
         if (k.turned[0] && k.column[0] >= 0) {
+            const float sign = direction * k.sign;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float2 cs = table[k.pair[0] + i];
-                v[0][i] = v[0][i] * cs.x + other[i] * (cs.y * direction * k.sign);
+                const float2 cs = table[k.at + i / 2 * k.step + i % 2];
+                v[0][i] = v[0][i] * cs.x + other[i] * (cs.y * sign);
             }
         }
     } else {
@@ -176,25 +247,36 @@ __device__ __forceinline__ void turn(float (&v)[E][V], const Columns<V, E, P> &k
 
 __device__ __forceinline__ float row_sum(float v, int lanes)
 {
-    for (int w = lanes >> 1; w > 0; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1)
+        if (w < lanes) v += __shfl_xor_sync(0xffffffffu, v, w);
     return v;
 }
 
-// A block has the rows of some tokens, with all their heads; BACKWARD: and, of the set, every blocks-th such group, so that
-// the sums for the gradient of the weights stay in registers.
+// A block has the rows of some tokens, with all their heads, kRows for every group of lanes that share a row; all of them are asked
+// for before the angles are worked out, which takes as long as they are on their way.  It goes on with every blocks-th such group of
+// tokens: what a block works out about its columns would cost as much as four rows of every lane do, and in the backward pass the
+// sums for the gradient of the weights stay in registers.
+constexpr int kRows = 2;
+// blocks that a multiprocessor has registers for
+template <int E, Pairs P, bool BACKWARD> constexpr int kResident = P == kAnywhere || (E > 1 && BACKWARD) ? 2 : BACKWARD || E > 1 ? 3 : kBlocksPerSm;
 template <typename T, int V, int E, Pairs P, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kResident<E, P, BACKWARD>)
 norm_rotate_kernel(const __grid_constant__ Call c)
 {
     pdl_begin();
     extern __shared__ __align__(16) float s_mem[];
     const bool second = (int)blockIdx.x >= c.set[0].blocks;
-    const Set &s = c.set[second];
+    const Set s = c.set[second];
     const int block = blockIdx.x - (second ? c.set[0].blocks : 0);
     float2 *s_table = reinterpret_cast<float2 *>(s_mem);
     const int lanes = 1 << c.lanes_log2, lane_in_row = threadIdx.x & (lanes - 1), sub = threadIdx.x >> c.lanes_log2, subs = kThreads >> c.lanes_log2;
     float *row_buffer = s_mem + s.tokens * c.rotary + sub * c.dim;  // kAnywhere
     const Columns<V, E, P> k(c, lane_in_row, lanes);
+    const bool turns = c.rotary > 0 && s.positions != nullptr;
+    __shared__ double s_turns[kMaxDim / 2];  // lanes that ask the arguments for different ones are served one after the other
+    if (turns && threadIdx.x < c.pairs) s_turns[threadIdx.x] = c.turns[threadIdx.x];
+    __syncthreads();
     float w[E][V], dw[E][V];
 #pragma unroll
     for (int e = 0; e < E; e++) {
@@ -206,65 +288,87 @@ norm_rotate_kernel(const __grid_constant__ Call c)
                                                                               : as_float(static_cast<const T *>(s.weight)[k.column[e] + i]);
         }
     }
-    const int groups = (s.n + s.tokens - 1) / s.tokens;
+    const int groups = (s.n + s.tokens - 1) / s.tokens, token0 = sub / s.heads, head0 = sub - token0 * s.heads;
+    const int step_t = subs / s.heads, step_h = subs - step_t * s.heads;
     const float inv_dim = 1.f / (float)c.dim;
     for (int group = block; group < groups; group += s.blocks) {
         const int first = group * s.tokens, n = min(s.tokens, s.n - first), rows = n * s.heads;
-        if (c.rotary > 0 && s.positions != nullptr) {
-            if (BACKWARD) __syncthreads();
-            angles(c, s, first, n, s_table);
-            __syncthreads();
-        }
-        int token = sub / s.heads, head = sub - token * s.heads;
-        const int step_t = subs / s.heads, step_h = subs - step_t * s.heads;
-        for (int base = 0; base < rows; base += subs) {
-            const bool valid = base + sub < rows;
-            const long long at = (long long)(first + token) * s.row + head * s.head;
-            const long long dense = ((long long)(first + token) * s.heads + head) * c.dim;
-            float x[E][V], g[E][V], sum = 0.f;
+        if (turns && group != block) __syncthreads();  // the last group's angles have been read
+        bool angles_due = turns;
+        int token = token0, head = head0;
+        for (int base = 0; base < rows; base += kRows * subs) {
+            Vec<T, V> x_in[kRows][E], g_in[BACKWARD ? kRows : 1][E];
+            int token_of[kRows];
+            long long dense[kRows];
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool in = valid && k.column[e] >= 0;
-                load<T, V>(x[e], static_cast<const T *>(s.x) + (in ? at + k.column[e] : 0), in);
-                if (BACKWARD) load<T, V>(g[e], static_cast<const T *>(s.grad) + (in ? dense + k.column[e] : 0), in);
-#pragma unroll
-                for (int i = 0; i < V; i++) sum = fmaf(x[e][i], x[e][i], sum);
-            }
-            const float r = 1.f / sqrtf(row_sum(sum, lanes) * inv_dim + c.eps);
-            const float2 *table = s_table + (valid ? token : 0) * (c.rotary / 2);
-            const bool turns = c.rotary > 0 && s.positions != nullptr;
-            T *to = static_cast<T *>(s.y) + dense;
-            if (!BACKWARD) {
-#pragma unroll
-                for (int e = 0; e < E; e++)
-#pragma unroll
-                    for (int i = 0; i < V; i++) x[e][i] = x[e][i] * r * w[e][i];
-                if (turns) turn<V, E, P>(x, k, c, table, 1.f, row_buffer);
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (valid && k.column[e] >= 0) store<T, V>(to + k.column[e], x[e]);
-            } else {
-                if (turns) turn<V, E, P>(g, k, c, table, -1.f, row_buffer);
-                float dot = 0.f;
-#pragma unroll
-                for (int e = 0; e < E; e++)
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        if (valid) dw[e][i] = fmaf(g[e][i], x[e][i] * r, dw[e][i]);
-                        g[e][i] *= w[e][i];
-                        dot = fmaf(g[e][i], x[e][i], dot);
-                    }
-                const float mean = row_sum(dot, lanes) * inv_dim * r * r;
+            for (int j = 0; j < kRows; j++) {
+                const bool valid = base + j * subs + sub < rows;
+                token_of[j] = valid ? token : -1;
+                dense[j] = ((long long)(first + token) * s.heads + head) * c.dim;
+                const T *x = static_cast<const T *>(s.x) + (long long)(first + token) * s.row + head * s.head;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
+                    x_in[j][e] = Vec<T, V>{};
+                    if (valid && k.column[e] >= 0) x_in[j][e] = *reinterpret_cast<const Vec<T, V> *>(x + k.column[e]);
+                    if constexpr (BACKWARD) {
+                        g_in[j][e] = Vec<T, V>{};
+                        if (valid && k.column[e] >= 0) g_in[j][e] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(s.grad) + dense[j] + k.column[e]);
+                    }
+                }
+                token += step_t;
+                head += step_h;
+                if (head >= s.heads) { head -= s.heads; token++; }
+            }
+            if (angles_due) {
+                angles<T, V, P>(c, s, s_turns, first, n, s_table);
+                __syncthreads();
+                angles_due = false;
+            }
 #pragma unroll
-                    for (int i = 0; i < V; i++) g[e][i] = r * (g[e][i] - x[e][i] * mean);
-                    if (valid && k.column[e] >= 0) store<T, V>(to + k.column[e], g[e]);
+            for (int j = 0; j < kRows; j++) {
+                if (base + j * subs >= rows) break;  // for all lanes alike
+                const bool valid = token_of[j] >= 0;
+                float x[E][V], sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; e++) to_floats<T, V>(x[e], x_in[j][e]);
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int i = 0; i < V; i++) sum = fmaf(x[e][i], x[e][i], sum);
+                const float r = rsqrtf(row_sum(sum, lanes) * inv_dim + c.eps);
+                const float2 *table = s_table + (valid ? token_of[j] : 0) * (c.rotary / 2);
+                T *to = static_cast<T *>(s.y) + dense[j];
+                if constexpr (!BACKWARD) {
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int i = 0; i < V; i++) x[e][i] = x[e][i] * r * w[e][i];
+                    if (turns) turn<V, E, P>(x, k, c, table, 1.f, row_buffer);
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if (valid && k.column[e] >= 0) store<T, V>(to + k.column[e], x[e]);
+                } else {
+                    float g[E][V], dot = 0.f;
+#pragma unroll
+                    for (int e = 0; e < E; e++) to_floats<T, V>(g[e], g_in[j][e]);
+                    if (turns) turn<V, E, P>(g, k, c, table, -1.f, row_buffer);
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int i = 0; i < V; i++) {
+                            if (valid) dw[e][i] = fmaf(g[e][i], x[e][i] * r, dw[e][i]);
+                            g[e][i] *= w[e][i];
+                            dot = fmaf(g[e][i], x[e][i], dot);
+                        }
+                    const float mean = row_sum(dot, lanes) * inv_dim * r * r;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) g[e][i] = r * (g[e][i] - x[e][i] * mean);
+                        if (valid && k.column[e] >= 0) store<T, V>(to + k.column[e], g[e]);
+                    }
                 }
             }
-            token += step_t;
-            head += step_h;
-            if (head >= s.heads) { head -= s.heads; token++; }
         }
     }
     if (BACKWARD && s.weight_part != nullptr) {
@@ -324,17 +428,25 @@ int log2_up(int n)
     return b;
 }
 
-// Blocks that a set's gradient is summed in: enough to fill the chip.
-int gradient_blocks(int n, int heads)
-{
-    const long long rows = (long long)n * heads, most = 4LL * sm_count();
-    const long long want = (rows + 31) / 32;
-    return (int)(want < most ? want : most);
-}
+// Blocks that a set's gradient is summed in, at most.
+int gradient_blocks(int n) { return (int)(n < kBlocksPerSm * (long long)sm_count() + 1 ? n : kBlocksPerSm * sm_count() + 1); }
 
 template <typename T, int V, int E, Pairs P, bool BACKWARD>
-int run(const Call &c, cudaStream_t stream)
+int run(Call &c, cudaStream_t stream)
 {
+    // As many blocks as the chip holds at a time, shared by the sets according to their work: an angle takes about as long as four
+    // elements, and is worked out once for all heads (8 and 2 heads of 64, blocks shared by rows 409 us, by work 253).
+    long long groups[2], room = kResident<E, P, BACKWARD> * (long long)sm_count();
+    double work[2];
+    for (int i = 0; i < 2; i++) {
+        const Set &s = c.set[i];
+        groups[i] = s.n > 0 ? div_up(s.n, s.tokens) : 0;
+        work[i] = (double)s.n * ((double)s.heads * c.dim + (s.positions != nullptr ? 2. * c.rotary : 0.));
+    }
+    for (int i = 0; i < 2; i++) {
+        const long long share = groups[0] + groups[1] <= room ? groups[i] : (long long)(work[i] / (work[0] + work[1]) * (double)(room - 1)) + 1;
+        c.set[i].blocks = (int)(share < groups[i] ? share : groups[i]);
+    }
     const int subs = kThreads >> c.lanes_log2;
     const int tokens = c.set[0].tokens > c.set[1].tokens ? c.set[0].tokens : c.set[1].tokens;
     size_t smem = sizeof(float) * (size_t)(tokens * c.rotary + (P == kAnywhere ? subs * c.dim : 0));
@@ -354,7 +466,9 @@ int run_type(Call &c, cudaStream_t stream)
     for (const Set &s : c.set)
         if (s.n > 0)
             whole = whole && aligned16(s.x) && aligned16(s.y) && s.row % V == 0 && s.head % V == 0 && (!BACKWARD || aligned16(s.grad));
-    c.lanes_log2 = whole ? log2_up(c.dim / V) : 5;
+    // a vector of either half to a lane, where the lanes of a row are then a power of two and all columns turn together
+    const bool both = whole && !c.interleaved && c.axes == 1 && c.rotary == c.dim && c.dim % (2 * V) == 0 && (c.dim & (c.dim - 1)) == 0;
+    c.lanes_log2 = both ? log2_up(c.dim / V) - 1 : whole ? log2_up(c.dim / V) : 5;
     const int subs = kThreads >> c.lanes_log2;
     for (Set &s : c.set) {
         // about four rows for every group of lanes, which share the angles; fewer where that leaves multiprocessors without a block
@@ -362,13 +476,15 @@ int run_type(Call &c, cudaStream_t stream)
         const int each = even < 1 ? 1 : even > 4 ? 4 : (int)even;
         const int tokens = s.heads > 0 ? each * subs / s.heads : 1;
         s.tokens = tokens < 1 ? 1 : tokens > kMaxTokens ? kMaxTokens : tokens;
-        const int groups = s.n > 0 ? div_up(s.n, s.tokens) : 0;
-        if (BACKWARD) s.blocks = groups < s.blocks ? groups : s.blocks;
-        else s.blocks = groups;
     }
     if (!whole) return run<T, 1, kMaxDim / 32, kAnywhere, BACKWARD>(c, stream);
+    if (both) return run<T, V, 2, kBothHalves, BACKWARD>(c, stream);
     if (c.interleaved) return run<T, V, 1, kNeighbours, BACKWARD>(c, stream);
     if (c.rotary == 0 || c.pairs % V == 0) return run<T, V, 1, kHalves, BACKWARD>(c, stream);
+    if (c.pairs == 1) return run<T, V, 1, kNeighbours, BACKWARD>(c, stream);
+    if (c.pairs == 2) return run<T, V, 1, kTwoOn, BACKWARD>(c, stream);
+    if constexpr (V == 8)
+        if (c.pairs == 4) return run<T, V, 1, kFourOn, BACKWARD>(c, stream);
     return run<T, V, 1, kAnywhere, BACKWARD>(c, stream);
 }
 
@@ -403,6 +519,7 @@ Call call_of(const hgc_norm_rotate_rows *sets, int n_sets, int dim, int rotary_d
     c.dim = dim; c.rotary = rotary_dim; c.axes = n_axes; c.pairs = rotary_dim / (2 * n_axes);
     c.position_type = position_type; c.interleaved = interleaved; c.eps = eps;
     if (c.pairs > 0) {
+        c.axis_factor = 65536 / c.pairs + 1;  // exact for the up to 64 pairs of a row
         const double ratio = pow(base, -1. / c.pairs);
         double f = 0.15915494309189533577;  // turns of a radian
         for (int i = 0; i < c.pairs; i++, f *= ratio) c.turns[i] = f;
@@ -440,7 +557,7 @@ extern "C" size_t hgc_norm_rotate_grad_workspace_bytes(const hgc_norm_rotate_row
     Sizer z;
     for (int i = 0; i < n_sets; i++) {
         if (sets[i].n < 0 || sets[i].n_heads < 1) return 0;
-        z.take<float>((size_t)gradient_blocks(sets[i].n, sets[i].n_heads) * dim);
+        z.take<float>((size_t)gradient_blocks(sets[i].n) * dim);
     }
     return z.used;
 }
@@ -457,8 +574,7 @@ extern "C" int hgc_norm_rotate_grad(const hgc_norm_rotate_rows *sets, int n_sets
     bool join = false;
     for (int i = 0; i < n_sets; i++) {
         Set &s = c.set[i];
-        s.blocks = gradient_blocks(s.n, s.heads);
-        float *part = carver.take<float>((size_t)s.blocks * dim);
+        float *part = carver.take<float>((size_t)gradient_blocks(s.n) * dim);
         s.weight_part = sets[i].d_grad_weight ? part : nullptr;
         j.part[i] = part;
         j.to[i] = sets[i].d_grad_weight;

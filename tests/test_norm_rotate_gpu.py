@@ -76,7 +76,9 @@ def inputs(n, heads, dim, dtype, axes, kind, dev, seed):
 @pytest.mark.parametrize("dtype", ["float", "half", "bfloat"])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dim,rotary,axes", [(64, 64, 0), (32, 32, 4), (22, 12, 3), (128, 128, 1), (128, 64, 2), (8, 8, 1), (2, 2, 0), (96, 32, 2),
-                                             (72, 64, 0), (1, 0, 0), (127, 126, 3), (40, 24, 1), (16, 16, 1)])
+                                             (72, 64, 0), (1, 0, 0), (127, 126, 3), (40, 24, 1), (16, 16, 1)] + [
+                             # axes of few columns, which end inside a 16-byte vector
+                             (16, 4, 1), (32, 12, 3), (8, 6, 3), (64, 20, 5), (24, 8, 4), (16, 6, 1), (128, 8, 1)])
 def test_forward_and_backward(cuda, dtype, interleaved, dim, rotary, axes):
     from hgcalml_b200.norm_rotate_op import NormRotate
     kinds = [torch.float32, torch.int32, torch.int64]
@@ -236,3 +238,15 @@ def test_more_rows_than_the_chip_holds(cuda, dtype):
     for i, name in enumerate(("y", "dx", "dw")):
         assert_near(got[2 * i].detach(), want_q[i], "queries " + name)
         assert_near(got[2 * i + 1].detach(), want_k[i], "keys " + name)
+
+
+def test_without_an_eps(cuda):
+    """Nothing but the rows' own squares under the root; groups of lanes that have no row divide by zero, which is no one's concern."""
+    from hgcalml_b200.norm_rotate_op import NormRotate
+    x, w, pos, grad = inputs(7, 3, 64, "bfloat", 1, torch.float32, cuda, 11)
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    y, _ = NormRotate(leaves[0], None, leaves[1], None, pos, eps=0.)
+    dx, dw = torch.autograd.grad(y, leaves, grad)
+    want = reference(x.detach(), w.detach(), pos, 64, False, 10000., 0., grad)
+    for got, ref, name in zip((y.detach(), dx, dw), want, ("y", "dx", "dw")):
+        assert_near(got, ref, name)
