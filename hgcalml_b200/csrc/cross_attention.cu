@@ -86,30 +86,69 @@ template <int DP> __device__ __forceinline__ int column(int tx, int c)
     return tx * V + c / V * (16 * V) + c % V;
 }
 
-// Rows [begin, begin + n) of one head as floats; what is not there, and the keys that cannot be seen, are zeros, whatever the
-// memory holds: a weight of zero would not make up for an infinity.
+// Rows of one head as floats; what is not there, and the keys that cannot be seen, are zeros, whatever the memory holds: a weight of
+// zero would not make up for an infinity.  In float32 the copies are asynchronous, in pieces of 16, 8 or 4 bytes as the rows allow
+// (copied() waits for all but the last `ahead` groups); other types are converted on their way.
+template <typename T> __device__ __forceinline__ int piece_of(const Strided &s, int dim)
+{
+    if (sizeof(T) != 4) return 1;
+    const unsigned long long all = reinterpret_cast<unsigned long long>(s.p) | (unsigned long long)(s.row * 4) | (unsigned long long)(s.head * 4) |
+                                   (unsigned long long)(dim * 4);
+    return (all & 15u) == 0 ? 4 : (all & 7u) == 0 ? 2 : 1;
+}
+template <int N> __device__ __forceinline__ void copy_async(float *dst, const float *src, bool in)  // zeros where not `in`
+{
+    const unsigned to = (unsigned)__cvta_generic_to_shared(dst);
+    if constexpr (N == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" :: "r"(to), "l"(src), "r"(in ? 4 * N : 0), "n"(4 * N) : "memory");
+}
+template <int AHEAD> __device__ __forceinline__ void copied() { asm volatile("cp.async.wait_group %0;" :: "n"(AHEAD) : "memory"); }
+__device__ __forceinline__ void end_of_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// `place(r)`: where row r begins, or a negative number
+template <typename T, int DP, int N, typename Place>
+__device__ __forceinline__ void copy_rows(float *__restrict__ dst, const T *__restrict__ p, int dim, Place place)
+{
+    constexpr int W = DP / N;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kRows * W; i += kThreads) {
+        const int r = i / W, d = i % W * N;
+        const long long at = place(r);
+        const bool in = at >= 0 && d < dim;
+        if constexpr (sizeof(T) == 4) copy_async<N>(dst + r * kPitch<DP> + d, p + (in ? at + d : 0), in);
+        else dst[r * kPitch<DP> + d] = in ? to_float(p[at + d]) : 0.f;
+    }
+}
+template <typename T, int DP, typename Place>
+__device__ __forceinline__ void load_rows(float *__restrict__ dst, const Strided &s, int piece, int dim, Place place)
+{
+    const T *p = static_cast<const T *>(s.p);
+    if constexpr (sizeof(T) == 4) {
+        if (piece == 4) return copy_rows<T, DP, 4>(dst, p, dim, place);
+        if (piece == 2) return copy_rows<T, DP, 2>(dst, p, dim, place);
+    }
+    copy_rows<T, DP, 1>(dst, p, dim, place);
+}
+// keys that can be seen, of those of a step
+__device__ __forceinline__ void load_seen(unsigned char *seen, const unsigned char *mask, int begin, int n)
+{
+    if (threadIdx.x < kRows) seen[threadIdx.x] = (int)threadIdx.x < n && (mask == nullptr || mask[begin + threadIdx.x] != 0);
+}
 template <typename T, int DP>
-__device__ __forceinline__ void load_keys(float *__restrict__ dst, const Strided &s, int head, int begin, int n, int dim,
-                                          const unsigned char *__restrict__ mask)
+__device__ __forceinline__ void load_keys(float *__restrict__ dst, const Strided &s, int piece, int head, int begin, int dim, const unsigned char *seen)
 {
-    const T *__restrict__ p = static_cast<const T *>(s.p) + head * s.head;
-    for (int i = threadIdx.x; i < kRows * DP; i += kThreads) {
-        const int r = i / DP, d = i % DP;
-        const bool in = r < n && d < dim && (mask == nullptr || fresh(mask + begin + r) != 0);
-        dst[r * kPitch<DP> + d] = in ? to_float(p[(long long)(begin + r) * s.row + d]) : 0.f;
-    }
+    load_rows<T, DP>(dst, s, piece, dim, [&](int r) { return seen[r] ? (long long)(begin + r) * s.row + (long long)head * s.head : -1ll; });
 }
-// Rows of a tile of queries: row r is head r % pack of token r / pack.
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void load_queries(float *__restrict__ dst, const Strided &s, int head0, int begin, int n, int pack, int dim)
+// row r of a tile of queries is head r % pack of token r / pack
+template <typename T, int DP>
+__device__ __forceinline__ void load_queries(float *__restrict__ dst, const Strided &s, int piece, int head0, int begin, int n, int pack, int dim)
 {
-    const T *__restrict__ p = static_cast<const T *>(s.p);
-    for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
-        const int r = i / DP, d = i % DP;
-        dst[r * kPitch<DP> + d] = r < n && d < dim
-            ? to_float(p[(long long)(begin + r / pack) * s.row + (long long)(head0 + r % pack) * s.head + d]) : 0.f;
-    }
+    load_rows<T, DP>(dst, s, piece, dim, [&](int r) {
+        return r < n ? (long long)(begin + r / pack) * s.row + (long long)(head0 + r % pack) * s.head : -1ll;
+    });
 }
+// Narrow heads: the next step's rows are on their way during this one.  Wide ones have no room for that; there are other blocks.
+template <int DP> constexpr int kStages = DP == 32 ? 2 : 1;
 
 // The block's tile, found by the first warp; blocks of one call that have nothing to do leave here.
 __device__ __forceinline__ Tile block_tile(const int *rs, int n, int n_events, int rows)
@@ -133,8 +172,10 @@ forward_kernel(const __grid_constant__ Args a)
     pdl_begin();
     constexpr int M = 16 * TM, P = kPitch<DP>, C = DP / 16;
     extern __shared__ __align__(16) float s_mem[];
-    float *s_q = s_mem, *s_k = s_q + M * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P;
-    __shared__ unsigned char s_seen[kRows];
+    static_assert(M == kRows, "tiles of queries are copied as tiles of keys are");
+    constexpr int S = kStages<DP>;
+    float *s_q = s_mem, *s_k = s_q + M * P, *s_v = s_k + S * kRows * P, *s_p = s_v + S * kRows * P;
+    __shared__ unsigned char s_seen_all[S][kRows];
     const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
     const int tokens = M / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_splits(a, t, kThreads);
@@ -143,7 +184,19 @@ forward_kernel(const __grid_constant__ Args a)
     const int n_rows = (tile.end - tile.begin) * a.pack;
     const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
     const int2 part = part_of(max(0, (keys.y - keys.x + kRows - 1) / kRows), blockIdx.z, a.splits);
-    load_queries<T, DP, M>(s_q, a.q, head0, tile.begin, n_rows, a.pack, a.dim);
+    load_queries<T, DP>(s_q, a.q, piece_of<T>(a.q, a.dim), head0, tile.begin, n_rows, a.pack, a.dim);
+    const int piece_k = piece_of<T>(a.k, a.dim), piece_v = piece_of<T>(a.v, a.dim);
+    const auto load = [&](int step) {  // with a barrier inside
+        const int at = step % S, k0 = keys.x + step * kRows;
+        if (step < part.y) load_seen(s_seen_all[at], a.mask, k0, min(kRows, keys.y - k0));
+        __syncthreads();
+        if (step < part.y) {
+            load_keys<T, DP>(s_k + at * kRows * P, a.k, piece_k, kv, k0, a.dim, s_seen_all[at]);
+            load_keys<T, DP>(s_v + at * kRows * P, a.v, piece_v, kv, k0, a.dim, s_seen_all[at]);
+        }
+        end_of_copies();
+    };
+    if (S > 1) load(part.x);
     const float c = a.scale * kLog2e;
     float o[TM][C], m[TM], l[TM];
 #pragma unroll
@@ -154,14 +207,14 @@ forward_kernel(const __grid_constant__ Args a)
         for (int j = 0; j < C; j++) o[i][j] = 0.f;
     }
     for (int step = part.x; step < part.y; step++) {
-        const int k0 = keys.x + step * kRows, n = min(kRows, keys.y - k0);
+        __syncthreads();  // the buffers that are filled now have been read
+        load(step + S - 1);
+        copied<S - 1>();
         __syncthreads();
-        load_keys<T, DP>(s_k, a.k, kv, k0, n, a.dim, a.mask);
-        load_keys<T, DP>(s_v, a.v, kv, k0, n, a.dim, a.mask);
-        if (t < kRows) s_seen[t] = t < n && (a.mask == nullptr || a.mask[k0 + t] != 0);
-        __syncthreads();
+        const float *k_now = s_k + step % S * kRows * P, *v_now = s_v + step % S * kRows * P;
+        const unsigned char *s_seen = s_seen_all[step % S];
         float s[TM][4] = {};
-        dots<DP, TM>(s, s_q, s_k, ty, tx);
+        dots<DP, TM>(s, s_q, k_now, ty, tx);
 #pragma unroll
         for (int i = 0; i < TM; i++) {
             float top = -INFINITY;
@@ -187,7 +240,7 @@ forward_kernel(const __grid_constant__ Args a)
             for (int j = 0; j < C; j++) o[i][j] *= shrink;
         }
         __syncthreads();
-        weighted_rows<DP, TM>(o, s_p, s_v, ty, tx);
+        weighted_rows<DP, TM>(o, s_p, v_now, ty, tx);
     }
 #pragma unroll
     for (int i = 0; i < TM; i++) {
@@ -310,8 +363,9 @@ grad_queries_kernel(const __grid_constant__ Args a)
     pdl_begin();
     constexpr int P = kPitch<DP>, C = DP / 16;
     extern __shared__ __align__(16) float s_mem[];
-    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P;
-    __shared__ unsigned char s_seen[kRows];
+    constexpr int S = kStages<DP>;
+    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + S * kRows * P, *s_p = s_v + S * kRows * P;
+    __shared__ unsigned char s_seen_all[S][kRows];
     const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
     const int tokens = kRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
     const Tile tile = block_tile(a.rs_q, a.n_q, a.n_events, tokens);
@@ -321,8 +375,20 @@ grad_queries_kernel(const __grid_constant__ Args a)
     if (tile.event < a.n_events && a.visible[tile.event] < 2) keys.y = keys.x;
     const int2 part = part_of(max(0, (keys.y - keys.x + kRows - 1) / kRows), blockIdx.z, a.splits);
     const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
-    load_queries<T, DP, kRows>(s_q, a.q, head0, tile.begin, n_rows, a.pack, a.dim);
-    load_queries<T, DP, kRows>(s_g, grad, head0, tile.begin, n_rows, a.pack, a.dim);
+    load_queries<T, DP>(s_q, a.q, piece_of<T>(a.q, a.dim), head0, tile.begin, n_rows, a.pack, a.dim);
+    load_queries<T, DP>(s_g, grad, piece_of<T>(grad, a.dim), head0, tile.begin, n_rows, a.pack, a.dim);
+    const int piece_k = piece_of<T>(a.k, a.dim), piece_v = piece_of<T>(a.v, a.dim);
+    const auto load = [&](int step) {  // with a barrier inside
+        const int at = step % S, k0 = keys.x + step * kRows;
+        if (step < part.y) load_seen(s_seen_all[at], a.mask, k0, min(kRows, keys.y - k0));
+        __syncthreads();
+        if (step < part.y) {
+            load_keys<T, DP>(s_k + at * kRows * P, a.k, piece_k, kv, k0, a.dim, s_seen_all[at]);
+            load_keys<T, DP>(s_v + at * kRows * P, a.v, piece_v, kv, k0, a.dim, s_seen_all[at]);
+        }
+        end_of_copies();
+    };
+    if (S > 1) load(part.x);
     const float c = a.scale * kLog2e;
     float dq[4][C] = {}, lse[4], delta[4];
 #pragma unroll
@@ -334,15 +400,15 @@ grad_queries_kernel(const __grid_constant__ Args a)
         delta[i] = stat.y;
     }
     for (int step = part.x; step < part.y; step++) {
-        const int k0 = keys.x + step * kRows, n = min(kRows, keys.y - k0);
+        __syncthreads();  // the buffers that are filled now have been read
+        load(step + S - 1);
+        copied<S - 1>();
         __syncthreads();
-        load_keys<T, DP>(s_k, a.k, kv, k0, n, a.dim, a.mask);
-        load_keys<T, DP>(s_v, a.v, kv, k0, n, a.dim, a.mask);
-        if (t < kRows) s_seen[t] = t < n && (a.mask == nullptr || a.mask[k0 + t] != 0);
-        __syncthreads();
+        const float *k_now = s_k + step % S * kRows * P, *v_now = s_v + step % S * kRows * P;
+        const unsigned char *s_seen = s_seen_all[step % S];
         float s[4][4] = {}, dp[4][4] = {};
-        dots<DP, 4>(s, s_q, s_k, ty, tx);
-        dots<DP, 4>(dp, s_g, s_v, ty, tx);
+        dots<DP, 4>(s, s_q, k_now, ty, tx);
+        dots<DP, 4>(dp, s_g, v_now, ty, tx);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -352,7 +418,7 @@ grad_queries_kernel(const __grid_constant__ Args a)
                 s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
             }
         __syncthreads();
-        weighted_rows<DP, 4>(dq, s_p, s_k, ty, tx);
+        weighted_rows<DP, 4>(dq, s_p, k_now, ty, tx);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -378,9 +444,11 @@ grad_keys_kernel(const __grid_constant__ Args a)
     pdl_begin();
     constexpr int P = kPitch<DP>, C = DP / 16;
     extern __shared__ __align__(16) float s_mem[];
-    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P,
+    constexpr int S = kStages<DP>;
+    float *s_q = s_mem, *s_g = s_q + S * kRows * P, *s_k = s_g + S * kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P,
           *s_d = s_p + kRows * kPitchP;
-    __shared__ float2 s_stats[kRows];
+    __shared__ float2 s_stats_all[S][kRows];
+    __shared__ unsigned char s_seen[kRows];
     const int t = threadIdx.x, ty = t >> 4, tx = t & 15, kv = blockIdx.y;
     const Tile tile = block_tile(a.rs_k, a.n_k, a.n_events, kRows);
     if (tile.begin >= tile.end) return;
@@ -390,30 +458,42 @@ grad_keys_kernel(const __grid_constant__ Args a)
     const int2 part = part_of(blocks, blockIdx.z, a.splits);
     const bool varies = tile.event < a.n_events && a.visible[tile.event] > 1;
     const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
-    load_keys<T, DP>(s_k, a.k, kv, tile.begin, n_keys, a.dim, a.mask);
-    load_keys<T, DP>(s_v, a.v, kv, tile.begin, n_keys, a.dim, a.mask);
+    load_seen(s_seen, a.mask, tile.begin, n_keys);
+    __syncthreads();
+    load_keys<T, DP>(s_k, a.k, piece_of<T>(a.k, a.dim), kv, tile.begin, a.dim, s_seen);
+    load_keys<T, DP>(s_v, a.v, piece_of<T>(a.v, a.dim), kv, tile.begin, a.dim, s_seen);
+    const int piece_q = piece_of<T>(a.q, a.dim), piece_g = piece_of<T>(grad, a.dim);
+    const auto load = [&](int step) {
+        if (step < part.y * packs) {
+            const int at = step % S, q0 = queries.x + step / packs * tokens, head0 = kv * a.group + step % packs * a.pack;
+            const int n = min(tokens, queries.y - q0) * a.pack;
+            load_queries<T, DP>(s_q + at * kRows * P, a.q, piece_q, head0, q0, n, a.pack, a.dim);
+            load_queries<T, DP>(s_g + at * kRows * P, grad, piece_g, head0, q0, n, a.pack, a.dim);
+            if (t < kRows)
+                s_stats_all[at][t] = t < n ? a.stats[(long long)(q0 + t / a.pack) * a.heads + head0 + t % a.pack] : make_float2(INFINITY, 0.f);
+        }
+        end_of_copies();
+    };
+    if (S > 1) load(part.x * packs);
     const float c = a.scale * kLog2e;
     float dk[4][C] = {}, dv[4][C] = {};
     bool seen[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int r = ty + 16 * i;
-        seen[i] = r < n_keys && (a.mask == nullptr || a.mask[tile.begin + r] != 0);
+        seen[i] = s_seen[r];
     }
     for (int step = part.x * packs; step < part.y * packs; step++) {
-        const int q0 = queries.x + step / packs * tokens, head0 = kv * a.group + step % packs * a.pack;
-        const int n = min(tokens, queries.y - q0) * a.pack;
+        const int n = min(tokens, queries.y - (queries.x + step / packs * tokens)) * a.pack;
+        __syncthreads();  // the buffers that are filled now have been read
+        load(step + S - 1);
+        copied<S - 1>();
         __syncthreads();
-        load_queries<T, DP, kRows>(s_q, a.q, head0, q0, n, a.pack, a.dim);
-        load_queries<T, DP, kRows>(s_g, grad, head0, q0, n, a.pack, a.dim);
-        if (t < kRows) {
-            const long long row = (long long)(q0 + t / a.pack) * a.heads + head0 + t % a.pack;
-            s_stats[t] = t < n ? a.stats[row] : make_float2(INFINITY, 0.f);
-        }
-        __syncthreads();
+        const float *q_now = s_q + step % S * kRows * P, *g_now = s_g + step % S * kRows * P;
+        const float2 *s_stats = s_stats_all[step % S];
         float s[4][4] = {}, dp[4][4] = {};
-        dots<DP, 4>(s, s_k, s_q, ty, tx);
-        dots<DP, 4>(dp, s_v, s_g, ty, tx);
+        dots<DP, 4>(s, s_k, q_now, ty, tx);
+        dots<DP, 4>(dp, s_v, g_now, ty, tx);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -424,8 +504,8 @@ grad_keys_kernel(const __grid_constant__ Args a)
                 s_d[(ty + 16 * i) * kPitchP + tx + 16 * j] = in && varies ? p * (dp[i][j] - s_stats[tx + 16 * j].y) : 0.f;
             }
         __syncthreads();
-        weighted_rows<DP, 4>(dv, s_p, s_g, ty, tx);
-        weighted_rows<DP, 4>(dk, s_d, s_q, ty, tx);
+        weighted_rows<DP, 4>(dv, s_p, g_now, ty, tx);
+        weighted_rows<DP, 4>(dk, s_d, q_now, ty, tx);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -579,7 +659,7 @@ template <typename C> BackwardBuffers carve_backward(C &c, const Plan &p, int n_
 template <typename T, int DP> int run_forward(const Args &a, const Plan &p, cudaStream_t stream)
 {
     constexpr int M = 16 * kForwardTM;
-    const size_t smem = sizeof(float) * ((M + 2 * kRows) * kPitch<DP> + M * kPitchP);
+    const size_t smem = sizeof(float) * ((M + 2 * kStages<DP> * kRows) * kPitch<DP> + M * kPitchP);
     return launch(forward_kernel<T, DP, kForwardTM>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a);
 }
 
@@ -594,12 +674,12 @@ template <typename T> int join_gradient(const Args &a, long long n, cudaStream_t
 
 template <typename T, int DP> int run_grad_queries(const Args &a, const Plan &p, cudaStream_t stream)
 {
-    const size_t smem = sizeof(float) * (4 * kRows * kPitch<DP> + kRows * kPitchP);
+    const size_t smem = sizeof(float) * ((2 + 2 * kStages<DP>) * kRows * kPitch<DP> + kRows * kPitchP);
     return launch(grad_queries_kernel<T, DP>, dim3((unsigned)p.tiles_q64, a.heads / a.pack, a.splits), smem, stream, a);
 }
 template <typename T, int DP> int run_grad_keys(const Args &a, const Plan &p, cudaStream_t stream)
 {
-    const size_t smem = sizeof(float) * (4 * kRows * kPitch<DP> + 2 * kRows * kPitchP);
+    const size_t smem = sizeof(float) * ((2 + 2 * kStages<DP>) * kRows * kPitch<DP> + 2 * kRows * kPitchP);
     return launch(grad_keys_kernel<T, DP>, dim3((unsigned)p.tiles_k, a.kv_heads, a.splits), smem, stream, a);
 }
 
