@@ -8,6 +8,7 @@
 // A row without keys has o = 0, and -inf for the logarithm of its sum.  Gradients of shared key heads are summed inside the
 // kernel and parts of a split are joined in their order: no atomics, so results do not change from run to run.
 #include "cross_attention.cuh"
+#include "mma_device.cuh"
 
 namespace hgc {
 namespace attn {
@@ -21,64 +22,74 @@ constexpr int kPitchP = kRows + 4;
 // at once.
 template <int DP> constexpr int kPitch = DP + 4;
 
-// acc[i][j] += a[ty + 16 i] . b[tx + 16 j]
+// acc[i][j] += a[ty + 16 i] . b[tx + 16 j].  Two columns at a time, whose sums are joined at the end: half the instructions.
 template <int DP, int TM>
 __device__ __forceinline__ void dots(float (&acc)[TM][4], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
 {
     constexpr int P = kPitch<DP>;
+    mma::pair sum[TM][4] = {};
 #pragma unroll 2
     for (int d = 0; d < DP; d += 4) {
-        float4 y[4];
+        ulonglong2 y[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) y[j] = *reinterpret_cast<const float4 *>(b + (tx + 16 * j) * P + d);
+        for (int j = 0; j < 4; j++) y[j] = *reinterpret_cast<const ulonglong2 *>(b + (tx + 16 * j) * P + d);
 #pragma unroll
         for (int i = 0; i < TM; i++) {
-            const float4 x = *reinterpret_cast<const float4 *>(a + (ty + 16 * i) * P + d);
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(a + (ty + 16 * i) * P + d);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                acc[i][j] = fmaf(x.x, y[j].x, acc[i][j]);
-                acc[i][j] = fmaf(x.y, y[j].y, acc[i][j]);
-                acc[i][j] = fmaf(x.z, y[j].z, acc[i][j]);
-                acc[i][j] = fmaf(x.w, y[j].w, acc[i][j]);
+                sum[i][j] = mma::fma2(x.x, y[j].x, sum[i][j]);
+                sum[i][j] = mma::fma2(x.y, y[j].y, sum[i][j]);
             }
         }
     }
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 halves = mma::parts(sum[i][j]);
+            acc[i][j] += halves.x + halves.y;
+        }
 }
 
 // acc[i][c] += sum_k a[ty + 16 i][k] b[k][column c of tx]; columns tx * V + 16 V g + v
 template <int DP> constexpr int kVec = DP / 16 < 4 ? DP / 16 : 4;
 template <int DP, int TM>
-__device__ __forceinline__ void weighted_rows(float (&acc)[TM][DP / 16], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
+__device__ __forceinline__ void weighted_rows(mma::pair (&acc)[TM][DP / 32], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
 {
     constexpr int P = kPitch<DP>, V = kVec<DP>, C = DP / 16;
 #pragma unroll 2
     for (int k = 0; k < kRows; k += 4) {
-        float y[4][C];
+        mma::pair y[4][C / 2];
 #pragma unroll
         for (int kk = 0; kk < 4; kk++)
 #pragma unroll
             for (int c = 0; c < C; c += V) {
                 const float *from = b + (k + kk) * P + tx * V + c * 16;
                 if constexpr (V == 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(from);
-                    y[kk][c] = q.x; y[kk][c + 1] = q.y; y[kk][c + 2] = q.z; y[kk][c + 3] = q.w;
+                    const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(from);
+                    y[kk][c / 2] = q.x;
+                    y[kk][c / 2 + 1] = q.y;
                 } else {
-                    const float2 q = *reinterpret_cast<const float2 *>(from);
-                    y[kk][c] = q.x; y[kk][c + 1] = q.y;
+                    y[kk][c / 2] = *reinterpret_cast<const mma::pair *>(from);
                 }
             }
 #pragma unroll
         for (int i = 0; i < TM; i++) {
             const float4 x = *reinterpret_cast<const float4 *>(a + (ty + 16 * i) * kPitchP + k);
+            const mma::pair w[4] = {mma::pair_of(x.x, x.x), mma::pair_of(x.y, x.y), mma::pair_of(x.z, x.z), mma::pair_of(x.w, x.w)};
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                acc[i][c] = fmaf(x.x, y[0][c], acc[i][c]);
-                acc[i][c] = fmaf(x.y, y[1][c], acc[i][c]);
-                acc[i][c] = fmaf(x.z, y[2][c], acc[i][c]);
-                acc[i][c] = fmaf(x.w, y[3][c], acc[i][c]);
-            }
+            for (int c = 0; c < C / 2; c++)
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) acc[i][c] = mma::fma2(w[kk], y[kk][c], acc[i][c]);
         }
     }
+}
+// value j of the pairs
+template <int N> __device__ __forceinline__ float value_of(const mma::pair (&acc)[N], int j)
+{
+    const float2 v = mma::parts(acc[j / 2]);
+    return j % 2 ? v.y : v.x;
 }
 template <int DP> __device__ __forceinline__ int column(int tx, int c)
 {
@@ -198,13 +209,14 @@ forward_kernel(const __grid_constant__ Args a)
     };
     if (S > 1) load(part.x);
     const float c = a.scale * kLog2e;
-    float o[TM][C], m[TM], l[TM];
+    mma::pair o[TM][C / 2];
+    float m[TM], l[TM];
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < C; j++) o[i][j] = 0.f;
+        for (int j = 0; j < C / 2; j++) o[i][j] = 0;
     }
     for (int step = part.x; step < part.y; step++) {
         __syncthreads();  // the buffers that are filled now have been read
@@ -237,7 +249,7 @@ forward_kernel(const __grid_constant__ Args a)
             }
             l[i] = l[i] * shrink + sum;  // of this thread's columns
 #pragma unroll
-            for (int j = 0; j < C; j++) o[i][j] *= shrink;
+            for (int j = 0; j < C / 2; j++) o[i][j] = mma::mul2(o[i][j], mma::pair_of(shrink, shrink));
         }
         __syncthreads();
         weighted_rows<DP, TM>(o, s_p, v_now, ty, tx);
@@ -258,8 +270,8 @@ forward_kernel(const __grid_constant__ Args a)
         for (int j = 0; j < C; j++) {
             const int d = column<DP>(tx, j);
             if (d >= a.dim) continue;
-            if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = o[i][j] * inv;
-            else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(o[i][j] * inv);
+            if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = value_of(o[i], j) * inv;
+            else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(value_of(o[i], j) * inv);
         }
     }
 }
@@ -293,12 +305,13 @@ join_forward_kernel(const float *__restrict__ part, const float *__restrict__ pa
 // ------------------------------------------------------------------------------------------------------------ backward
 // What both gradients go by.  The first `n_count` blocks: the keys of an event that can be seen, counted up to two; with one key
 // the weights do not depend on the scores, so the gradients of q and k are zero and not what is left of two sums that cancel.
-// The next `n_rows` blocks, a warp per row of the queries: what its exponents are less by (log2 of its sum, less `shift`; infinity
+// The next `n_rows` blocks, for every row of the queries: what its exponents are less by (log2 of its sum, less `shift`; infinity
 // without keys) and delta.  bounds: the largest squared norm of the rows of grad there, and of v in the blocks that follow.
+constexpr int kRowsALane = 4;
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ stats, int *__restrict__ visible, float *__restrict__ bounds, float shift,
-                        int n_count, int n_rows)
+                        int n_count, int n_rows, int lanes_log2)
 {
     pdl_begin();
     const int t = threadIdx.x;
@@ -316,42 +329,84 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
     }
     block -= n_count;
     float norm = 0.f;
-    if (block < n_rows) {
-        const long long row = (long long)block * (kThreads / 32) + (t >> 5);
-        if (row < (long long)a.n_q * a.heads) {
-            const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ grad = static_cast<const T *>(a.grad);
-            float sum = 0.f;
-            for (int d = lane_id(); d < a.dim; d += 32) {
-                const float g = to_float(grad[row * a.dim + d]);
-                sum = fmaf(to_float(out[row * a.dim + d]), g, sum);
-                norm = fmaf(g, g, norm);
-            }
+    // 2^lanes_log2 lanes have a row, 16 bytes each, or all 32 of them single columns; four rows a lane are on their way at a time
+    const bool whole = lanes_log2 >= 0;
+    const int lanes = whole ? 1 << lanes_log2 : 32, lane = t & (lanes - 1), subs = kThreads / lanes;
+    constexpr int V = 16 / sizeof(T);
+    struct alignas(16) Vec { T v[V]; };
+    const bool of_queries = block < n_rows;
+    const long long all = of_queries ? (long long)a.n_q * a.heads : (long long)a.n_k * a.kv_heads;
+    const long long first = (long long)(of_queries ? block : block - n_rows) * (subs * kRowsALane) + t / lanes;
+    const int known = of_queries ? split_at(a.rs_q, a.n_events, a.n_q) : split_at(a.rs_k, a.n_events, a.n_k);  // rows of some event
+    const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ grad = static_cast<const T *>(a.grad);
+    float sum[kRowsALane], square[kRowsALane];
+    if (whole) {
+        Vec x[kRowsALane], y[kRowsALane];
 #pragma unroll
-            for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-            if (lane_id() == 0) {
-                const float lse = a.lse[row];
-                stats[row] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e - shift, sum);
+        for (int i = 0; i < kRowsALane; i++) {
+            const long long row = first + (long long)i * subs;
+            const bool in = row < all && lane * V < a.dim;
+            x[i] = y[i] = Vec{};
+            if (in && of_queries) {
+                x[i] = *reinterpret_cast<const Vec *>(out + row * a.dim + lane * V);
+                y[i] = *reinterpret_cast<const Vec *>(grad + row * a.dim + lane * V);
+            } else if (in) {
+                const int key = (int)(row / a.kv_heads);
+                y[i] = *reinterpret_cast<const Vec *>(static_cast<const T *>(a.v.p) + key * a.v.row + (row - (long long)key * a.kv_heads) * a.v.head + lane * V);
             }
-            if (row / a.heads >= split_at(a.rs_q, a.n_events, a.n_q)) norm = 0.f;  // behind the last event: of no one's concern
+        }
+#pragma unroll
+        for (int i = 0; i < kRowsALane; i++) {
+            sum[i] = square[i] = 0.f;
+#pragma unroll
+            for (int d = 0; d < V; d++) {
+                const float g = to_float(y[i].v[d]);
+                sum[i] = fmaf(to_float(x[i].v[d]), g, sum[i]);
+                square[i] = fmaf(g, g, square[i]);
+            }
         }
     } else {
-        const long long row = (long long)(block - n_rows) * (kThreads / 32) + (t >> 5);
-        const int key = (int)(row / a.kv_heads), head = (int)(row - (long long)key * a.kv_heads);
-        if (row < (long long)a.n_k * a.kv_heads && key < split_at(a.rs_k, a.n_events, a.n_k) && (a.mask == nullptr || a.mask[key] != 0)) {
-            const T *__restrict__ v = static_cast<const T *>(a.v.p) + key * a.v.row + head * a.v.head;
-            for (int d = lane_id(); d < a.dim; d += 32) norm = fmaf(to_float(v[d]), to_float(v[d]), norm);
+#pragma unroll
+        for (int i = 0; i < kRowsALane; i++) {
+            const long long row = first + (long long)i * subs;
+            sum[i] = square[i] = 0.f;
+            for (int d = lane; d < a.dim && row < all; d += 32) {
+                const int key = of_queries ? 0 : (int)(row / a.kv_heads);
+                const float g = of_queries ? to_float(grad[row * a.dim + d])
+                                           : to_float(static_cast<const T *>(a.v.p)[key * a.v.row + (row - (long long)key * a.kv_heads) * a.v.head + d]);
+                if (of_queries) sum[i] = fmaf(to_float(out[row * a.dim + d]), g, sum[i]);
+                square[i] = fmaf(g, g, square[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsALane; i++) {
+        const long long row = first + (long long)i * subs;
+        for (int w = lanes >> 1; w > 0; w >>= 1) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], w);
+            square[i] += __shfl_xor_sync(0xffffffffu, square[i], w);
+        }
+        if (row >= all) continue;
+        if (of_queries && lane == 0) {
+            const float lse = a.lse[row];
+            stats[row] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e - shift, sum[i]);
+        }
+        // rows behind the last event, and masked keys, are of no one's concern
+        if (bounds != nullptr) {
+            const long long token = row / (of_queries ? a.heads : a.kv_heads);
+            if (token < known && (of_queries || a.mask == nullptr || fresh(a.mask + token) != 0)) norm = fmaxf(norm, square[i]);
         }
     }
     if (bounds == nullptr) return;
     __shared__ float s_norm[kThreads / 32];
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, w);
+    for (int w = 16; w > 0; w >>= 1) norm = fmaxf(norm, __shfl_xor_sync(0xffffffffu, norm, w));
     if (lane_id() == 0) s_norm[t >> 5] = norm;
     __syncthreads();
     if (t == 0) {
         for (int i = 1; i < kThreads / 32; i++) norm = fmaxf(norm, s_norm[i]);
         // norms are not negative, so their bits are in the order of their values, whatever the order of the blocks
-        if (norm > 0.f) atomicMax(reinterpret_cast<unsigned *>(bounds) + (block < n_rows ? 0 : 1), __float_as_uint(norm));
+        if (norm > 0.f) atomicMax(reinterpret_cast<unsigned *>(bounds) + (of_queries ? 0 : 1), __float_as_uint(norm));
     }
 }
 
@@ -390,7 +445,8 @@ grad_queries_kernel(const __grid_constant__ Args a)
     };
     if (S > 1) load(part.x);
     const float c = a.scale * kLog2e;
-    float dq[4][C] = {}, lse[4], delta[4];
+    mma::pair dq[4][C / 2] = {};
+    float lse[4], delta[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int r = ty + 16 * i;
@@ -429,7 +485,7 @@ grad_queries_kernel(const __grid_constant__ Args a)
         for (int j = 0; j < C; j++) {
             const int d = column<DP>(tx, j);
             if (d >= a.dim) continue;
-            const float v = dq[i][j] * a.scale;
+            const float v = value_of(dq[i], j) * a.scale;
             if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = v;
             else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(v);
         }
@@ -476,7 +532,7 @@ grad_keys_kernel(const __grid_constant__ Args a)
     };
     if (S > 1) load(part.x * packs);
     const float c = a.scale * kLog2e;
-    float dk[4][C] = {}, dv[4][C] = {};
+    mma::pair dk[4][C / 2] = {}, dv[4][C / 2] = {};
     bool seen[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -518,11 +574,11 @@ grad_keys_kernel(const __grid_constant__ Args a)
             if (d >= a.dim) continue;
             if (a.splits > 1) {
                 const long long at = ((long long)blockIdx.z * a.n_k * a.kv_heads + row) * a.dim + d;
-                a.part[at] = dk[i][j] * a.scale;
-                a.part2[at] = dv[i][j];
+                a.part[at] = value_of(dk[i], j) * a.scale;
+                a.part2[at] = value_of(dv[i], j);
             } else {
-                static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(dk[i][j] * a.scale);
-                static_cast<T *>(a.to2)[row * a.dim + d] = from_float<T>(dv[i][j]);
+                static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(value_of(dk[i], j) * a.scale);
+                static_cast<T *>(a.to2)[row * a.dim + d] = from_float<T>(value_of(dv[i], j));
             }
         }
     }
@@ -704,11 +760,17 @@ int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void 
 {
     const auto aligned = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
     const bool mma = mma_takes(a, dtype) && aligned(dq) && aligned(dk) && aligned(dv), bounded = mma && dtype == HGC_FLOAT16;
-    const int n_count = a.n_events > 0 ? a.n_events : 1, n_rows = div_up((long long)a.n_q * a.heads, kThreads / 32),
-              n_values = bounded ? div_up((long long)a.n_k * a.kv_heads, kThreads / 32) : 0;
+    // whole 16-byte vectors of rows where they are that
+    constexpr int V = 16 / sizeof(T);
+    int lanes_log2 = -1;
+    if (a.dim % V == 0 && aligned(a.out) && aligned(a.grad) && (!bounded || (aligned(a.v.p) && a.v.row % V == 0 && a.v.head % V == 0)))
+        for (lanes_log2 = 0; (V << lanes_log2) < a.dim; lanes_log2++) {}
+    const int rows_a_block = kThreads / (lanes_log2 >= 0 ? 1 << lanes_log2 : 32) * kRowsALane;
+    const int n_count = a.n_events > 0 ? a.n_events : 1, n_rows = div_up((long long)a.n_q * a.heads, rows_a_block),
+              n_values = bounded ? div_up((long long)a.n_k * a.kv_heads, rows_a_block) : 0;
     if (bounded) HGC_CUDA_TRY(cudaMemsetAsync(b.bounds, 0, 2 * sizeof(float), stream));
     HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + n_rows + n_values, kThreads, 0, stream, a, b.stats, b.visible,
-                            bounded ? b.bounds : nullptr, bounded ? kHalfShift : 0.f, n_count, n_rows));
+                            bounded ? b.bounds : nullptr, bounded ? kHalfShift : 0.f, n_count, n_rows, lanes_log2));
     HGC_LAUNCH_CHECK();
     a.stats = b.stats; a.visible = b.visible; a.bounds = b.bounds;
     if (dq != nullptr && a.n_q > 0) {
