@@ -277,6 +277,7 @@ forward_kernel(const __grid_constant__ Args a)
 }
 
 // Joins the parts of a row: every part holds its own softmax and the logarithm of its sum.
+constexpr int kMaxParts = 128;
 template <typename T>
 __global__ void __launch_bounds__(256)
 join_forward_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, T *__restrict__ out, float *__restrict__ lse,
@@ -285,19 +286,40 @@ join_forward_kernel(const float *__restrict__ part, const float *__restrict__ pa
     pdl_begin();
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= n_rows) return;
-    float top = -INFINITY;
-    for (int s = 0; s < splits; s++) top = fmaxf(top, part_lse[s * n_rows + row]);
-    float sum = 0.f;
+    // a lane has every 32nd part's logarithm
+    constexpr int kEach = kMaxParts / 32;
+    float lse_of[kEach], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const int s = 32 * i + lane_id();
+        lse_of[i] = s < splits ? part_lse[s * n_rows + row] : -INFINITY;
+        top = fmaxf(top, lse_of[i]);
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
     const float base = top == -INFINITY ? 0.f : top;
-    for (int s = 0; s < splits; s++) sum += exp2f((part_lse[s * n_rows + row] - base) * kLog2e);
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        lse_of[i] = exp2f((lse_of[i] - base) * kLog2e);
+        sum += lse_of[i];
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int d = lane_id(); d < dim; d += 32) {
+    for (int d0 = 0; d0 < dim; d0 += 32) {
+        const int d = d0 + lane_id();
         float o = 0.f;
-        for (int s = 0; s < splits; s++) {
-            const float w = exp2f((part_lse[s * n_rows + row] - base) * kLog2e);
-            if (w != 0.f) o = fmaf(w, part[(s * n_rows + row) * dim + d], o);
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+#pragma unroll 8
+            for (int s = 0; s < min(32, splits - 32 * i); s++) {
+                const float w = __shfl_sync(0xffffffffu, lse_of[i], s);
+                // parts without weight were not written
+                const float v = d < dim ? part[((32ll * i + s) * n_rows + row) * dim + d] : 0.f;
+                o = fmaf(w, w == 0.f ? 0.f : v, o);
+            }
         }
-        out[row * dim + d] = from_float<T>(o * inv);
+        if (d < dim) out[row * dim + d] = from_float<T>(o * inv);
     }
     if (lane_id() == 0) lse[row] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
@@ -619,12 +641,12 @@ int split_count(long long blocks, long long mean_steps, int per_sm, int least)
     const long long want = (long long)per_sm * sm_count() / (blocks > 0 ? blocks : 1);
     long long s = mean_steps / least;
     if (s > want) s = want;
-    return s < 1 ? 1 : s > 128 ? 128 : (int)s;
+    return s < 1 ? 1 : s > kMaxParts ? kMaxParts : (int)s;
 }
 
 // What a call of these sizes needs; the kernels and the workspace queries go by the same numbers.
 struct Plan {
-    int group, pack, splits, splits_mma, splits_q, splits_q_mma, splits_k, splits_k_mma;
+    int group, pack, splits, splits_mma, parts_mma, alternate, pack_few, rows_few, splits_few, splits_q, splits_q_mma, splits_k, splits_k_mma;
     long long tiles_q, tiles_q64, tiles_k;
 };
 
@@ -652,7 +674,16 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
     p.splits = split_count(filled(n_q, m) * (heads / p.pack), steps_k, 4, 4);
     const int mma_tokens = kMmaRows / p.pack;
-    p.splits_mma = split_count(filled(n_q, 2 * mma_tokens) * (heads / p.pack), n_k / some / mma_keys(dim), 6, 4);
+    // events of no more rows than half a tile, and keys for both of its halves
+    const long long steps_mma = n_k / some / mma_keys(dim);
+    p.alternate = (long long)n_q <= (long long)some * mma_tokens && steps_mma >= 12;
+    p.splits_mma = split_count(filled(n_q, p.alternate ? mma_tokens : 2 * mma_tokens) * (heads / p.pack), steps_mma, 6, 4);
+    if (p.alternate && p.splits_mma > kMaxParts / 2) p.splits_mma = kMaxParts / 2;
+    p.parts_mma = p.splits_mma * (p.alternate ? 2 : 1);
+    // where the queries of a mean event fit a block that holds them in registers
+    p.pack_few = few_pack(p.group);
+    p.rows_few = few_rows(n_q, events, p.pack_few);
+    p.splits_few = p.rows_few > 0 ? split_count(filled(n_q, p.rows_few / p.pack_few) * (heads / p.pack_few), n_k / some / kFewStep, 20, 4) : 1;
     p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
     p.splits_q_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / kMmaGradStep, 4, 4);
     p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);
@@ -669,7 +700,8 @@ template <typename C> ForwardBuffers carve_forward(C &c, const Plan &p, int n_q,
     ForwardBuffers b;
     if constexpr (std::is_same_v<C, Carver>) b.counter = c.template take<int>(1);
     else c.template take<int>(1);
-    const int splits = p.splits > p.splits_mma ? p.splits : p.splits_mma;
+    int splits = p.splits > p.parts_mma ? p.splits : p.parts_mma;
+    if (p.splits_few > splits) splits = p.splits_few;
     if (splits > 1) {
         const size_t rows = (size_t)splits * n_q * heads;
         if constexpr (std::is_same_v<C, Carver>) {
@@ -741,16 +773,22 @@ template <typename T, int DP> int run_grad_keys(const Args &a, const Plan &p, cu
 
 template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStream_t stream)
 {
-    const bool mma = mma_takes(a, dtype);
-    a.splits = mma ? p.splits_mma : p.splits;
-    if (const int rc = mma ? mma_forward(a, dtype, stream)
+    // From four rows on the tensor cores are faster, though most of their rows are empty (64 queries on 1.28M keys, us there / here:
+    // one row a block 224 / 159, four 224 / 260, eight 230 / 457).
+    const bool few = p.rows_few > 0 && few_takes(a, dtype) && !(p.rows_few > 2 && mma_takes(a, dtype)), mma = !few && mma_takes(a, dtype);
+    if (few) a.pack = p.pack_few;
+    a.splits = few ? p.splits_few : mma ? p.splits_mma : p.splits;
+    a.alternate = mma ? p.alternate : 0;
+    const int parts = mma ? p.parts_mma : a.splits;
+    if (const int rc = few ? few_forward(a, p.rows_few, dtype, stream)
+                     : mma ? mma_forward(a, dtype, stream)
                      : a.dim <= 32 ? run_forward<T, 32>(a, p, stream)
                      : a.dim <= 64 ? run_forward<T, 64>(a, p, stream) : run_forward<T, 128>(a, p, stream))
         return rc;
-    if (a.splits == 1) return HGC_OK;
+    if (parts == 1) return HGC_OK;
     const long long rows = (long long)a.n_q * a.heads;
     HGC_CUDA_TRY(launch_pdl(join_forward_kernel<T>, div_up(rows, 8), 256, 0, stream, a.part, a.part_lse, static_cast<T *>(a.to), a.lse, rows, a.dim,
-                            a.splits));
+                            parts));
     HGC_LAUNCH_CHECK();
     return HGC_OK;
 }

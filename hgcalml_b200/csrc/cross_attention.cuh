@@ -37,7 +37,7 @@ struct Args {
     const float *bounds;           // largest squared norms of the rows of grad and of v (half precision's backward pass)
     int *counter;                  // of the tiles that the blocks of the forward pass take
     unsigned *status;
-    int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits;
+    int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits, alternate;  // alternate: of the forward pass on the tensor cores, two parts to each of the splits
     float scale;
 };
 
@@ -113,6 +113,13 @@ __device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int 
     if (event >= n_events) return make_int2(0, 0);
     return make_int2(split_at(rs, event, n), split_at(rs, event + 1, n));
 }
+
+// A few queries per event (cross_attention_few.cu): rows of whole, aligned 16-byte vectors, up to eight rows of queries a block.
+constexpr int kFewStep = 128;                        // keys that a split is a multiple of
+int few_pack(int group);                             // heads of a block
+int few_rows(int n_q, int n_events, int pack);       // rows of a block, or 0 where there are more than a few
+bool few_takes(const Args &a, int dtype);
+int few_forward(const Args &a, int rows, int dtype, cudaStream_t stream);
 
 // The kernels on the tensor cores (cross_attention_mma.cu): 16-bit types, heads of whole 16-byte vectors, aligned rows.
 bool mma_takes(const Args &a, int dtype);
