@@ -656,7 +656,10 @@ bool sizes_ok(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 {
     return n_q >= 0 && n_k >= 0 && n_rs >= 1 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && dim >= 1;
 }
-bool sizes_supported(int heads, int dim) { return heads <= 65535 && dim <= kMaxDim; }
+bool sizes_supported(int n_q, int n_k, int n_rs, int heads, int dim)
+{
+    return n_q <= kMaxCount && n_k <= kMaxCount && n_rs <= kMaxCount / 2 && heads <= 65535 && dim <= kMaxDim;
+}
 
 Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 {
@@ -773,9 +776,7 @@ template <typename T, int DP> int run_grad_keys(const Args &a, const Plan &p, cu
 
 template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStream_t stream)
 {
-    // From four rows on the tensor cores are faster, though most of their rows are empty (64 queries on 1.28M keys, us there / here:
-    // one row a block 224 / 159, four 224 / 260, eight 230 / 457).
-    const bool few = p.rows_few > 0 && few_takes(a, dtype) && !(p.rows_few > 2 && mma_takes(a, dtype)), mma = !few && mma_takes(a, dtype);
+    const bool few = few_takes(a, p.rows_few, dtype), mma = !few && mma_takes(a, dtype);
     if (few) a.pack = p.pack_few;
     a.splits = few ? p.splits_few : mma ? p.splits_mma : p.splits;
     a.alternate = mma ? p.alternate : 0;
@@ -864,7 +865,7 @@ using namespace hgc::attn;
 extern "C" size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype)
 {
     (void)dtype;
-    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_heads, dim)) return 0;
+    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return 0;
     Sizer s;
     carve_forward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim), n_q, n_heads, dim);
     return s.used;
@@ -878,7 +879,7 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !scale_ok(scale) || !strides_ok(strides) || dtype < 0 || dtype > HGC_BFLOAT16)
         return HGC_ERR_INVALID_ARGUMENT;
-    if (!sizes_supported(n_heads, dim)) return HGC_ERR_UNSUPPORTED;
+    if (!sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return HGC_ERR_UNSUPPORTED;
     if (n_q == 0) return HGC_OK;
     if (!d_q || !d_out || !d_lse || !d_q_row_splits || !d_k_row_splits || (n_k > 0 && (!d_k || !d_v))) return HGC_ERR_INVALID_ARGUMENT;
     if (const int rc = check_workspace(workspace, workspace_bytes,
@@ -897,7 +898,7 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
 extern "C" size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype)
 {
     (void)dtype;
-    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_heads, dim)) return 0;
+    if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return 0;
     Sizer s;
     carve_backward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim), n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
     return s.used;
@@ -912,7 +913,7 @@ extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q,
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !scale_ok(scale) || !strides_ok(strides) || dtype < 0 || dtype > HGC_BFLOAT16)
         return HGC_ERR_INVALID_ARGUMENT;
-    if (!sizes_supported(n_heads, dim)) return HGC_ERR_UNSUPPORTED;
+    if (!sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return HGC_ERR_UNSUPPORTED;
     if (n_q == 0 && n_k == 0) return HGC_OK;
     if (!d_q_row_splits || !d_k_row_splits || (n_q > 0 && (!d_grad_out || !d_q || !d_out || !d_lse)) || (n_k > 0 && (!d_k || !d_v)) ||
         !d_grad_k != !d_grad_v)

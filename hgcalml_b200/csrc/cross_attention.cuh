@@ -12,6 +12,7 @@ namespace attn {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMaxDim = 128;
+constexpr int kMaxCount = 0x7fffffff - 8192;  // rows of either set: a step past the end must not leave 32 bits
 // Heads that share a key head are packed into the rows of a tile up to this many, so that keys and values are read once for all
 // of them; beyond it every head has its own tiles.
 constexpr int kMaxPack = 32;
@@ -73,7 +74,7 @@ __device__ __forceinline__ Tile find_tile(const int *rs, int n, int n_events, in
     Tile t;
     t.event = lo;
     t.begin = begin < 0 || begin > last ? last : (int)begin;
-    t.end = min(last, t.begin + rows);
+    t.end = last - t.begin < rows ? last : t.begin + rows;  // no sum beyond 32 bits
     return t;
 }
 
@@ -118,7 +119,7 @@ __device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int 
 constexpr int kFewStep = 128;                        // keys that a split is a multiple of
 int few_pack(int group);                             // heads of a block
 int few_rows(int n_q, int n_events, int pack);       // rows of a block, or 0 where there are more than a few
-bool few_takes(const Args &a, int dtype);
+bool few_takes(const Args &a, int rows, int dtype);
 int few_forward(const Args &a, int rows, int dtype, cudaStream_t stream);
 
 // The kernels on the tensor cores (cross_attention_mma.cu): 16-bit types, heads of whole 16-byte vectors, aligned rows.

@@ -193,7 +193,8 @@ few_kernel(const __grid_constant__ Args a, int lanes_log2)
                 acc[r][i] = mma::pair_of(x.x * mine + y.x * theirs, x.y * mine + y.y * theirs);
             }
         }
-    // the warps, in their order; the rows' copies have all been read
+    // the warps, in their order, where the rows were: those have been read, and the zeros asked for behind the last step are there too
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float *s_top = s_mem + kWarps * R * a.dim, *s_sum = s_top + kWarps * R;
     if (group == 0) {
@@ -243,8 +244,9 @@ template <typename T> int run(Args a, int rows, cudaStream_t stream)
 {
     int lanes_log2 = 0;
     while ((kVec<T> << lanes_log2) < a.dim) lanes_log2++;
-    return rows <= 1 ? launch<T, 1>(a, lanes_log2, stream) : rows <= 2 ? launch<T, 2>(a, lanes_log2, stream)
-         : rows <= 4 ? launch<T, 4>(a, lanes_log2, stream) : launch<T, 8>(a, lanes_log2, stream);
+    if constexpr (sizeof(T) == 4)
+        if (rows > 2) return rows <= 4 ? launch<T, 4>(a, lanes_log2, stream) : launch<T, 8>(a, lanes_log2, stream);
+    return rows <= 1 ? launch<T, 1>(a, lanes_log2, stream) : launch<T, 2>(a, lanes_log2, stream);
 }
 
 }  // namespace
@@ -261,8 +263,12 @@ int few_rows(int n_q, int n_events, int pack)
     const long long mean = n_q > 0 ? ((long long)n_q + some - 1) / some : 1, rows = mean * pack;
     return mean > kFewRows / pack ? 0 : rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
 }
-bool few_takes(const Args &a, int dtype)
+bool few_takes(const Args &a, int rows, int dtype)
 {
+    // 16-bit types: from four rows on the tensor cores are faster, though most of their rows are empty (64 queries on 1.28M keys, us there /
+    // here: one row a block 224 / 159, four 224 / 260, eight 230 / 457).  Float32 has tiles of 64 rows on the other side (64 columns, the
+    // same lengths, eight heads: a row a block 5664 / 814, four 1443 / 279, eight 669 / 381; 700 keys 55 / 44).
+    if (rows == 0 || (rows > 2 && dtype != HGC_FLOAT32)) return false;
     const int bytes = dtype == HGC_FLOAT32 ? 4 : 2, vec = 16 / bytes;
     const auto fits = [&](const Strided &s) { return (reinterpret_cast<uintptr_t>(s.p) & 15u) == 0 && s.row % vec == 0 && s.head % vec == 0; };
     return a.dim % vec == 0 && a.n_k > 0 && fits(a.q) && fits(a.k) && fits(a.v);

@@ -96,7 +96,7 @@ __device__ __forceinline__ void store16(void *to, float *part, const Rows &rows,
 // copy queries, keys and values, issue scores, issue sums, and clear what must not be summed.
 //
 // Where events have no more than 128 rows, `alternate`, a tile is 128 rows, and the two times eight warps take its steps in turn, each
-// with sums of their own: twice as many parts to join (64 queries on 1.28M keys 250 -> 162 us).
+// with sums of their own: twice as many parts to join (64 queries on 1.28M keys 250 -> 224 us).
 //
 // A block takes one tile after the other from a counter, and every warp goes on to the next tile as soon as its own part is done: copies
 // and scores of a tile run under the softmax and the results of the one before.  With a tile per block, 371k queries on 1152 keys
@@ -922,7 +922,7 @@ template <typename T, int CHUNKS> int forward_mma(const Args &a, const Maps &map
 {
     const int rows = kMmaRows / a.pack * (a.alternate ? 1 : 2);
     const long long tiles = tile_count(a.n_q, rows, a.n_events), items = tiles * (a.heads / a.pack) * a.splits;
-    if (items > 0x7fffffff) return HGC_ERR_UNSUPPORTED;
+    if (items > kMaxCount) return HGC_ERR_UNSUPPORTED;
     const int blocks = items < sm_count() ? (int)items : sm_count();
     if (items > blocks) HGC_CUDA_TRY(cudaMemsetAsync(a.counter, 0, sizeof(int), stream));
     return launch(forward_mma_kernel<T, CHUNKS>, blocks, Forward<CHUNKS>::kThreads, Forward<CHUNKS>::kSmem, stream, a, maps, (int)tiles, (int)items, a.alternate);

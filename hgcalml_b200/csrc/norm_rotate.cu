@@ -18,6 +18,7 @@ namespace hgc {
 namespace {
 
 constexpr int kMaxDim = 128;
+constexpr int kMaxCount = 0x7fffffff - 8192;  // rows: a step past the end must not leave 32 bits
 constexpr int kThreads = 256, kBlocksPerSm = 4;
 constexpr int kMaxTokens = 64;  // rows of a block, whose angles are kept
 
@@ -505,6 +506,7 @@ int check(const hgc_norm_rotate_rows *sets, int n_sets, int dim, int rotary_dim,
     for (int i = 0; i < n_sets; i++) {
         const hgc_norm_rotate_rows &s = sets[i];
         if (s.n < 0 || s.n_heads < 1 || s.row_stride < 0 || s.head_stride < 0) return HGC_ERR_INVALID_ARGUMENT;
+        if (s.n > kMaxCount || s.n_heads > 65535) return HGC_ERR_UNSUPPORTED;
         if (s.n > 0 && (!s.d_x || (!backward && !s.d_y) || (backward && (!s.d_grad_y || !s.d_grad_x)))) return HGC_ERR_INVALID_ARGUMENT;
         if (s.d_weight && s.weight_type != HGC_FLOAT32 && s.weight_type != dtype) return HGC_ERR_INVALID_ARGUMENT;
         if (backward && s.d_grad_weight && !s.d_weight) return HGC_ERR_INVALID_ARGUMENT;

@@ -423,7 +423,7 @@ int hgc_push_knn_grad_ordered(
  * of rows and heads in strides = {q row, q head, k row, k head, v row, v head} (host memory; NULL: dense); columns
  * lie next to each other.  d_out, d_lse (float32) and everything the gradient takes and gives besides are dense.
  * Sums, weights and gradients are held in float32; in 16 bits, weights are rounded once to the type of the values
- * they meet.  scale > 0.  Limits: dim <= 128, n_heads <= 65535.
+ * they meet.  scale > 0.  Limits: dim <= 128, n_heads <= 65535, 2^31 - 8193 rows.
  *
  * The gradient: d_grad_out [n_q, n_heads, dim] is that of d_out; d_out and d_lse are the forward pass's, as are all
  * other arguments.  d_grad_q may be NULL, and d_grad_k and d_grad_v both, where they are not wanted; gradients of

@@ -25,7 +25,8 @@ def test_attention_entries_check_their_arguments(call):
     for bad in (dict(n_q=-1), dict(n_k=-1), dict(n_rs=0), dict(heads=0), dict(kv=0), dict(heads=3, kv=2), dict(dim=0), dict(dtype=3), dict(dtype=-1),
                 dict(scale=0.), dict(scale=-1.), dict(scale=inf), dict(scale=nan), dict(strides=(ctypes.c_longlong * 6)(-1, 0, 0, 0, 0, 0))):
         assert call(L, **bad) == -1, bad
-    assert call(L, dim=129) == -3 and call(L, heads=65536, kv=65536) == -3
+    for much in (dict(dim=129), dict(heads=65536, kv=65536), dict(n_q=2 ** 31 - 1), dict(n_k=2 ** 31 - 8192), dict(n_rs=2 ** 31 - 1)):
+        assert call(L, **much) == -3, much
     assert call(L) == -1  # null tensors
     assert call(L, n_q=0, n_k=0) == 0  # nothing to do
     assert _attend(L, n_q=0) == 0
@@ -73,7 +74,7 @@ def test_norm_rotate_entries_check_their_arguments():
                 dict(base=1.), dict(base=float("nan")), dict(eps=-1.), dict(eps=float("nan")), dict(dtype=3), dict(r=_set(_capi, n=-1)),
                 dict(r=_set(_capi, heads=0)), dict(r=_set(_capi, row=-1)), dict(r=_set(_capi, n=3)), dict(r=_set(_capi, w=1, wt=2))):
         assert call(**bad) == (-1, -1), bad
-    assert call(dim=129, rotary=8) == (-3, -3)
+    assert call(dim=129, rotary=8) == call(r=_set(_capi, n=2 ** 31 - 1)) == call(r=_set(_capi, heads=65536)) == (-3, -3)
     assert L.hgc_norm_rotate(None, 1, 8, 8, 1, 0, 0, ctypes.c_double(1e4), F(0.), 0, NUL) == -1
     assert L.hgc_norm_rotate_grad_workspace_bytes(_set(_capi, n=1000, heads=3), 1, 64) > 256
 

@@ -1,7 +1,8 @@
 """Attention between ragged sets against its formulas in 64 bits, at the sizes, layouts and masks where it can go wrong.
 
 Tolerances are bounds, not fits.  With u the largest relative error of a rounding to the tensors' type (eps / 2), e = 2^-24
-that of float32 and w the rounding of weights (u in 16 bits, where weights meet the values in their type, else 0):
+that of float32 and w what weights are off by before they meet the values (0 in float32; in 16 bits their rounding u and, in the
+weight and in the sum that it is divided by, the polynomial for their power of two, 1.0e-4 < 2^-13: u + 2^-12):
   a score is off by at most x = scale (D + 2) e sum|q_d k_d| + 4 e |lse|, so a weight by the share 2 x + 2^-21 (two scores; exp);
   o_d by u |o_d| + (w + 2 x + 2^-21 + (n + 8) e) sum_j p_j |v_jd| for n summed keys;
   ds_j = p_j (dp_j - delta) by (w + 2 x + 2^-21) |ds_j| + p_j (2 (D + 2) e sum|do_d v_jd| + sum_d |do_d| err(o_d));
@@ -25,7 +26,7 @@ def reference(q, k, v, nq, nk, scale, mask=None, grad=None):
     heads, kv_heads, dim = q.shape[1], k.shape[1], q.shape[2]
     group = heads // kv_heads
     u = torch.finfo(q.dtype).eps / 2
-    w = 0. if q.dtype == torch.float32 else u
+    w = 0. if q.dtype == torch.float32 else u + 2. ** -12
     f = lambda t: t.double()  # noqa: E731
     zero = lambda t: torch.zeros(t.shape, dtype=torch.float64, device=t.device)  # noqa: E731
     res = {n: [zero(t), zero(t)] for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", k))}
@@ -225,6 +226,28 @@ def test_single_queries_over_long_keys(cuda, dtype, dim, heads, kv_heads):
         from hgcalml_b200.cross_attention_op import CrossAttention
         for _ in range(3):
             assert torch.equal(CrossAttention(q, k, v, splits(nq, cuda), splits(nk, cuda)), out)
+
+
+@pytest.mark.parametrize("dtype", ["float", "half", "bfloat"])
+@pytest.mark.parametrize("dim", [8, 24, 64, 120, 128])
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8])
+def test_a_few_queries_of_every_event(cuda, dtype, dim, group):
+    """Single tokens with one to eight heads to a key head: masks that leave events some keys, one and none, what masked and foreign
+    rows hold, events without queries or keys, lengths around those of a step, and rows behind the last event."""
+    nq, nk = [1, 0, 1, 1, 1, 0, 1, 1], [1, 40, 0, 129, 700, 31, 1500, 64]
+    q, k, v, grad = inputs(nq, nk, 2 * group, 2, dim, dtype, cuda, seed=23, extra=(1, 9))
+    mask = torch.rand(k.shape[0], generator=torch.Generator(device=cuda).manual_seed(1), device=cuda) < 0.6
+    mask[41:170] = False
+    mask[100] = True  # one key of the event of 129
+    mask[-73 - 9:] = False  # and none of the last one
+    k[~mask], v[~mask] = float("nan"), float("inf")
+    k[-9:], v[-9:] = float("nan"), float("nan")
+    out = check(q, k, v, grad, nq, nk, mask=mask)
+    assert (out[-2:] == 0).all()
+    mask[:] = True
+    k, v = k.nan_to_num(1.), v.nan_to_num(1., 1., 1.)
+    k[-9:], v[-9:] = float("nan"), float("nan")
+    check(q, k, v, grad, nq, nk, both=False)
 
 
 @pytest.mark.parametrize("dtype,dim", [("bfloat", 64), ("float", 32)])
