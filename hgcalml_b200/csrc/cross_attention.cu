@@ -1,5 +1,5 @@
-// Attention between two ragged sets of rows of the same events, forward and backward: products in float32 on the CUDA cores,
-// for every type, width and stride, and the C entries.
+// Attention between two ragged sets of rows of the same events, forward and backward: products in float32 on the tensor cores,
+// in parts, for every type, width and stride, and the C entries.
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - m_i) / l_i,  s_ij = scale q_i.k_j over the keys j of i's event that can be seen
 //   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i.v_j - delta_i),  delta_i = do_i.o_i,  dq_i = scale sum_j ds_ij k_j,
@@ -15,86 +15,127 @@ namespace attn {
 namespace {
 
 constexpr int kRows = 64;        // rows and columns of a tile
-constexpr int kThreads = 256;    // 16 x 16; a thread has rows ty + 16 i and columns tx + 16 j
-constexpr int kPitchP = kRows + 4;
+constexpr int kThreads = 256;    // four times two warps: a warp has 16 rows and 32 columns of a tile of scores
+constexpr int kWarpRows = 16, kWarpColumns = 32, kBlocks = kWarpColumns / 8;  // of 8 columns, which one product has
 
-// Rows of `dp` floats, 4 more apart: 16-byte reads of 8 consecutive rows meet no bank twice, and one row is read by 16 threads
-// at once.
+// Products on the tensor cores, of which this form takes operands of 11 bits: x = big + small, both of 11 bits, and a product is
+// big big + big small + small big, off by what is left of either, 2^-21, and by small small, 2^-22.  Tensor cores cut off what an
+// addition leaves, so the small products have a sum of their own, and sums are taken on from there with rounding, once a step.
+// On the CUDA cores a tile of 4 x 4 per thread waited for shared memory half of the time (7 events of some 16k rows on 2.6k, 22 columns:
+// 4661 us, here 3053; a training step on three of 7k on 2k, 32 columns: 4596, here 3312), and was less exact.
+// 16-bit values are operands as they are (`EXACT`).
+//
+// A lane of a warp has the rows g and g + 8, g = lane / 4, and of 8 columns those from 2 (lane % 4) on.  What one product leaves is an
+// operand of the next one where it is: the order of summed rows is free, so lane t takes the rows 2 t and 2 t + 1 of the other operand.
+__device__ __forceinline__ void product(float (&c)[4], const unsigned (&a)[4], const unsigned (&b)[2])
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <bool EXACT> __device__ __forceinline__ void in_two(float x, unsigned &big, unsigned &small)
+{
+    if constexpr (EXACT) {
+        big = __float_as_uint(x);
+    } else {
+        big = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+        small = __float_as_uint(x - __uint_as_float(big)) & 0xffffe000u;
+    }
+}
+
+// Rows of `DP` floats, 4 more apart: neither kind of operand meets a bank twice.
 template <int DP> constexpr int kPitch = DP + 4;
 
-// acc[i][j] += a[ty + 16 i] . b[tx + 16 j].  Two columns at a time, whose sums are joined at the end: half the instructions.
-template <int DP, int TM>
-__device__ __forceinline__ void dots(float (&acc)[TM][4], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
+// s[n][i] = row of a . row of b, for 16 rows of a and 32 of b.
+template <int DP, bool EXACT>
+__device__ __forceinline__ void dots(float (&s)[kBlocks][4], const float *__restrict__ a, const float *__restrict__ b, int dim)
 {
     constexpr int P = kPitch<DP>;
-    mma::pair sum[TM][4] = {};
+    const int at = (lane_id() >> 2) * P + (lane_id() & 3);
+    float rest[kBlocks][4];
+#pragma unroll
+    for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[n][i] = rest[n][i] = 0.f;
 #pragma unroll 2
-    for (int d = 0; d < DP; d += 4) {
-        ulonglong2 y[4];
+    for (int d = 0; d < dim; d += 8) {
+        unsigned a_big[4], a_small[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) y[j] = *reinterpret_cast<const ulonglong2 *>(b + (tx + 16 * j) * P + d);
+        for (int i = 0; i < 4; i++) in_two<EXACT>(a[at + (i & 1) * 8 * P + d + (i >> 1) * 4], a_big[i], a_small[i]);
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(a + (ty + 16 * i) * P + d);
+        for (int n = 0; n < kBlocks; n++) {
+            unsigned b_big[2], b_small[2];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                sum[i][j] = mma::fma2(x.x, y[j].x, sum[i][j]);
-                sum[i][j] = mma::fma2(x.y, y[j].y, sum[i][j]);
+            for (int i = 0; i < 2; i++) in_two<EXACT>(b[at + n * 8 * P + d + i * 4], b_big[i], b_small[i]);
+            if constexpr (!EXACT) {
+                product(rest[n], a_small, b_big);
+                product(rest[n], a_big, b_small);
             }
+            product(s[n], a_big, b_big);
         }
     }
+    if constexpr (!EXACT) {
 #pragma unroll
-    for (int i = 0; i < TM; i++)
+        for (int n = 0; n < kBlocks; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 halves = mma::parts(sum[i][j]);
-            acc[i][j] += halves.x + halves.y;
-        }
+            for (int i = 0; i < 4; i++) s[n][i] += rest[n][i];
+    }
 }
 
-// acc[i][c] += sum_k a[ty + 16 i][k] b[k][column c of tx]; columns tx * V + 16 V g + v
-template <int DP> constexpr int kVec = DP / 16 < 4 ? DP / 16 : 4;
-template <int DP, int TM>
-__device__ __forceinline__ void weighted_rows(mma::pair (&acc)[TM][DP / 32], const float *__restrict__ a, const float *__restrict__ b, int ty, int tx)
+// acc[n][i] += sum over the 32 rows of b, weighted by w as dots() leaves it.
+template <int DP, bool EXACT>
+__device__ __forceinline__ void weighted_rows(float (&acc)[DP / 8][4], const float (&w)[kBlocks][4], const float *__restrict__ b, int dim)
 {
-    constexpr int P = kPitch<DP>, V = kVec<DP>, C = DP / 16;
-#pragma unroll 2
-    for (int k = 0; k < kRows; k += 4) {
-        mma::pair y[4][C / 2];
+    constexpr int P = kPitch<DP>;
+    const int at = 2 * (lane_id() & 3) * P + (lane_id() >> 2);
+    unsigned w_big[kBlocks][4], w_small[kBlocks][4];
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++)
+    for (int k = 0; k < kBlocks; k++)
 #pragma unroll
-            for (int c = 0; c < C; c += V) {
-                const float *from = b + (k + kk) * P + tx * V + c * 16;
-                if constexpr (V == 4) {
-                    const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(from);
-                    y[kk][c / 2] = q.x;
-                    y[kk][c / 2 + 1] = q.y;
-                } else {
-                    y[kk][c / 2] = *reinterpret_cast<const mma::pair *>(from);
-                }
-            }
+        for (int i = 0; i < 4; i++) in_two<false>(w[k][(i & 1) * 2 + (i >> 1)], w_big[k][i], w_small[k][i]);
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const float4 x = *reinterpret_cast<const float4 *>(a + (ty + 16 * i) * kPitchP + k);
-            const mma::pair w[4] = {mma::pair_of(x.x, x.x), mma::pair_of(x.y, x.y), mma::pair_of(x.z, x.z), mma::pair_of(x.w, x.w)};
+    for (int n = 0; n < DP / 8; n++) {
+        if (8 * n >= dim) break;
+        float sum[4] = {}, rest[4] = {};
 #pragma unroll
-            for (int c = 0; c < C / 2; c++)
+        for (int k = 0; k < kBlocks; k++) {
+            unsigned b_big[2], b_small[2];
 #pragma unroll
-                for (int kk = 0; kk < 4; kk++) acc[i][c] = mma::fma2(w[kk], y[kk][c], acc[i][c]);
+            for (int i = 0; i < 2; i++) in_two<EXACT>(b[at + (8 * k + i) * P + 8 * n], b_big[i], b_small[i]);
+            product(rest, w_small[k], b_big);
+            if constexpr (!EXACT) product(rest, w_big[k], b_small);
+            product(sum, w_big[k], b_big);
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[n][i] += sum[i] + rest[i];
     }
 }
-// value j of the pairs
-template <int N> __device__ __forceinline__ float value_of(const mma::pair (&acc)[N], int j)
+// The warps of the second 32 columns leave their sums in shared memory, after a barrier, the others have them added to theirs.
+template <int DP> __device__ __forceinline__ void leave(float *__restrict__ to, const float (&acc)[DP / 8][4])
 {
-    const float2 v = mma::parts(acc[j / 2]);
-    return j % 2 ? v.y : v.x;
+    float *at = to + (lane_id() >> 2) * kPitch<DP> + 2 * (lane_id() & 3);
+#pragma unroll
+    for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) *reinterpret_cast<float2 *>(at + i * 4 * kPitch<DP> + 8 * n) = make_float2(acc[n][i], acc[n][i + 1]);
 }
-template <int DP> __device__ __forceinline__ int column(int tx, int c)
+template <int DP> __device__ __forceinline__ void add(float (&acc)[DP / 8][4], const float *__restrict__ from, const float (&mine)[2], const float (&theirs)[2])
 {
-    constexpr int V = kVec<DP>;
-    return tx * V + c / V * (16 * V) + c % V;
+    const float *at = from + (lane_id() >> 2) * kPitch<DP> + 2 * (lane_id() & 3);
+#pragma unroll
+    for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[n][i] = acc[n][i] * mine[i >> 1] + at[(i >> 1) * 8 * kPitch<DP> + 8 * n + (i & 1)] * theirs[i >> 1];
+}
+// Row `row` (0, or 1: 8 further) of a warp's results, times `factor`, to `to`.
+template <int DP, typename T> __device__ __forceinline__ void store_row(T *__restrict__ to, const float (&acc)[DP / 8][4], int row, float factor, int dim)
+{
+#pragma unroll
+    for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int d = 8 * n + 2 * (lane_id() & 3) + i;
+            if (d < dim) to[d] = from_float<T>(acc[n][2 * row + i] * factor);
+        }
 }
 
 // Rows of one head as floats; what is not there, and the keys that cannot be seen, are zeros, whatever the memory holds: a weight of
@@ -158,8 +199,8 @@ __device__ __forceinline__ void load_queries(float *__restrict__ dst, const Stri
         return r < n ? (long long)(begin + r / pack) * s.row + (long long)(head0 + r % pack) * s.head : -1ll;
     });
 }
-// Narrow heads: the next step's rows are on their way during this one.  Wide ones have no room for that; there are other blocks.
-template <int DP> constexpr int kStages = DP == 32 ? 2 : 1;
+// The next step's rows are on their way during this one; the widest heads have no room for that, but a second block has.
+template <int DP> constexpr int kStages = DP <= 64 ? 2 : 1;
 
 // The block's tile, found by the first warp; blocks of one call that have nothing to do leave here.
 __device__ __forceinline__ Tile block_tile(const int *rs, int n, int n_events, int rows)
@@ -176,19 +217,18 @@ __device__ __forceinline__ Tile block_tile(const int *rs, int n, int n_events, i
 // ------------------------------------------------------------------------------------------------------------- forward
 // A block takes a tile of queries (with the heads that share a key head) through the keys of its event, 64 at a time, with the
 // running maximum and sum of every row.
-template <typename T, int DP, int TM>
+template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads)
 forward_kernel(const __grid_constant__ Args a)
 {
     pdl_begin();
-    constexpr int M = 16 * TM, P = kPitch<DP>, C = DP / 16;
+    constexpr int P = kPitch<DP>, S = kStages<DP>;
+    constexpr bool kExact = sizeof(T) == 2;
     extern __shared__ __align__(16) float s_mem[];
-    static_assert(M == kRows, "tiles of queries are copied as tiles of keys are");
-    constexpr int S = kStages<DP>;
-    float *s_q = s_mem, *s_k = s_q + M * P, *s_v = s_k + S * kRows * P, *s_p = s_v + S * kRows * P;
+    float *s_q = s_mem, *s_k = s_q + kRows * P, *s_v = s_k + S * kRows * P;
     __shared__ unsigned char s_seen_all[S][kRows];
-    const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
-    const int tokens = M / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
+    const int t = threadIdx.x, row0 = (t >> 5) % 4 * kWarpRows, column0 = (t >> 7) * kWarpColumns;
+    const int tokens = kRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_splits(a, t, kThreads);
     const Tile tile = block_tile(a.rs_q, a.n_q, a.n_events, tokens);
     if (tile.begin >= tile.end) return;
@@ -209,70 +249,81 @@ forward_kernel(const __grid_constant__ Args a)
     };
     if (S > 1) load(part.x);
     const float c = a.scale * kLog2e;
-    mma::pair o[TM][C / 2];
-    float m[TM], l[TM];
-#pragma unroll
-    for (int i = 0; i < TM; i++) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < C / 2; j++) o[i][j] = 0;
-    }
+    float o[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
     for (int step = part.x; step < part.y; step++) {
         __syncthreads();  // the buffers that are filled now have been read
         load(step + S - 1);
         copied<S - 1>();
         __syncthreads();
         const float *k_now = s_k + step % S * kRows * P, *v_now = s_v + step % S * kRows * P;
-        const unsigned char *s_seen = s_seen_all[step % S];
-        float s[TM][4] = {};
-        dots<DP, TM>(s, s_q, k_now, ty, tx);
+        const unsigned char *s_seen = s_seen_all[step % S] + column0 + 2 * (lane_id() & 3);
+        float s[kBlocks][4], base[2];
+        dots<DP, kExact>(s, s_q + row0 * P, k_now + column0 * P, a.dim);
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            float top = -INFINITY;
+        for (int r = 0; r < 2; r++) {
+            float top = m[r];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (!s_seen[tx + 16 * j]) s[i][j] = -INFINITY;
-                top = fmaxf(top, s[i][j]);
+            for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    if (!s_seen[8 * n + i]) s[n][2 * r + i] = -INFINITY;
+                    top = fmaxf(top, s[n][2 * r + i]);
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            base[r] = top == -INFINITY ? 0.f : top;
+            const float shrink = exp2f((m[r] - base[r]) * c);
+            m[r] = top;
+            l[r] *= shrink;  // of this lane's columns
+#pragma unroll
+            for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    s[n][2 * r + i] = exp2f((s[n][2 * r + i] - base[r]) * c);
+                    l[r] += s[n][2 * r + i];
+                }
+#pragma unroll
+            for (int n = 0; n < DP / 8; n++) {
+                o[n][2 * r] *= shrink;
+                o[n][2 * r + 1] *= shrink;
             }
-#pragma unroll
-            for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            const float next = fmaxf(m[i], top), base = next == -INFINITY ? 0.f : next;
-            const float shrink = exp2f((m[i] - base) * c);
-            m[i] = next;
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float p = exp2f((s[i][j] - base) * c);
-                sum += p;
-                s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = p;
-            }
-            l[i] = l[i] * shrink + sum;  // of this thread's columns
-#pragma unroll
-            for (int j = 0; j < C / 2; j++) o[i][j] = mma::mul2(o[i][j], mma::pair_of(shrink, shrink));
         }
-        __syncthreads();
-        weighted_rows<DP, TM>(o, s_p, v_now, ty, tx);
+        weighted_rows<DP, kExact>(o, s, v_now + column0 * P, a.dim);
     }
+    // the two times 32 columns
+    __shared__ float2 s_stats[kRows];
+    copied<0>();
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TM; i++) {
-        float sum = l[i];
+    for (int r = 0; r < 2; r++) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (column0 > 0 && (lane_id() & 3) == 0) s_stats[row0 + (lane_id() >> 2) + 8 * r] = make_float2(m[r], l[r]);
+    }
+    if (column0 > 0) leave<DP>(s_q + row0 * P, o);
+    __syncthreads();
+    if (column0 > 0) return;
+    float mine[2], theirs[2];
 #pragma unroll
-        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        const int r = ty + 16 * i;
+    for (int r = 0; r < 2; r++) {
+        const float2 other = s_stats[row0 + (lane_id() >> 2) + 8 * r];
+        const float top = fmaxf(m[r], other.x), base = top == -INFINITY ? 0.f : top;
+        mine[r] = exp2f((m[r] - base) * c);
+        theirs[r] = exp2f((other.x - base) * c);
+        l[r] = l[r] * mine[r] + other.y * theirs[r];
+        m[r] = top;
+    }
+    add<DP>(o, s_q + row0 * P, mine, theirs);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r = row0 + (lane_id() >> 2) + 8 * i;
         if (r >= n_rows) continue;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const float lse = sum == 0.f ? -INFINITY : m[i] * a.scale + logf(sum);
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
         float *lse_to = a.splits > 1 ? a.part_lse + (long long)blockIdx.z * a.n_q * a.heads : a.lse;
-        if (tx == 0) lse_to[row] = lse;
-#pragma unroll
-        for (int j = 0; j < C; j++) {
-            const int d = column<DP>(tx, j);
-            if (d >= a.dim) continue;
-            if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = value_of(o[i], j) * inv;
-            else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(value_of(o[i], j) * inv);
-        }
+        if ((lane_id() & 3) == 0) lse_to[row] = l[i] == 0.f ? -INFINITY : m[i] * a.scale + logf(l[i]);
+        if (a.splits > 1) store_row<DP>(a.part + ((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim, o, i, inv, a.dim);
+        else store_row<DP>(static_cast<T *>(a.to) + row * a.dim, o, i, inv, a.dim);
     }
 }
 
@@ -438,12 +489,12 @@ __global__ void __launch_bounds__(kThreads)
 grad_queries_kernel(const __grid_constant__ Args a)
 {
     pdl_begin();
-    constexpr int P = kPitch<DP>, C = DP / 16;
+    constexpr int P = kPitch<DP>, S = kStages<DP>;
+    constexpr bool kExact = sizeof(T) == 2;
     extern __shared__ __align__(16) float s_mem[];
-    constexpr int S = kStages<DP>;
-    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + S * kRows * P, *s_p = s_v + S * kRows * P;
+    float *s_q = s_mem, *s_g = s_q + kRows * P, *s_k = s_g + kRows * P, *s_v = s_k + S * kRows * P;
     __shared__ unsigned char s_seen_all[S][kRows];
-    const int t = threadIdx.x, ty = t >> 4, tx = t & 15;
+    const int t = threadIdx.x, row0 = (t >> 5) % 4 * kWarpRows, column0 = (t >> 7) * kWarpColumns;
     const int tokens = kRows / a.pack, head0 = blockIdx.y * a.pack, kv = head0 / a.group;
     const Tile tile = block_tile(a.rs_q, a.n_q, a.n_events, tokens);
     if (tile.begin >= tile.end) return;
@@ -467,11 +518,10 @@ grad_queries_kernel(const __grid_constant__ Args a)
     };
     if (S > 1) load(part.x);
     const float c = a.scale * kLog2e;
-    mma::pair dq[4][C / 2] = {};
-    float lse[4], delta[4];
+    float dq[DP / 8][4] = {}, lse[2], delta[2];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = ty + 16 * i;
+    for (int i = 0; i < 2; i++) {
+        const int r = row0 + (lane_id() >> 2) + 8 * i;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
         const float2 stat = r < n_rows ? a.stats[row] : make_float2(INFINITY, 0.f);
         lse[i] = stat.x;
@@ -482,35 +532,32 @@ grad_queries_kernel(const __grid_constant__ Args a)
         load(step + S - 1);
         copied<S - 1>();
         __syncthreads();
-        const float *k_now = s_k + step % S * kRows * P, *v_now = s_v + step % S * kRows * P;
-        const unsigned char *s_seen = s_seen_all[step % S];
-        float s[4][4] = {}, dp[4][4] = {};
-        dots<DP, 4>(s, s_q, k_now, ty, tx);
-        dots<DP, 4>(dp, s_g, v_now, ty, tx);
+        const float *k_now = s_k + step % S * kRows * P + column0 * P, *v_now = s_v + step % S * kRows * P + column0 * P;
+        const unsigned char *s_seen = s_seen_all[step % S] + column0 + 2 * (lane_id() & 3);
+        float s[kBlocks][4], dp[kBlocks][4];
+        dots<DP, kExact>(s, s_q + row0 * P, k_now, a.dim);
+        dots<DP, kExact>(dp, s_g + row0 * P, v_now, a.dim);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int n = 0; n < kBlocks; n++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool seen = s_seen[tx + 16 * j] && ty + 16 * i < n_rows;
-                const float p = seen ? exp2f(fmaf(s[i][j], c, -lse[i])) : 0.f;
-                s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = seen ? p * (dp[i][j] - delta[i]) : 0.f;
-            }
-        __syncthreads();
-        weighted_rows<DP, 4>(dq, s_p, k_now, ty, tx);
+            for (int i = 0; i < 4; i++)
+                s[n][i] = s_seen[8 * n + (i & 1)] ? exp2f(fmaf(s[n][i], c, -lse[i >> 1])) * (dp[n][i] - delta[i >> 1]) : 0.f;
+        weighted_rows<DP, kExact>(dq, s, k_now, a.dim);
     }
+    copied<0>();
+    __syncthreads();
+    if (column0 > 0) leave<DP>(s_k + row0 * P, dq);
+    __syncthreads();
+    if (column0 > 0) return;
+    const float one[2] = {1.f, 1.f};
+    add<DP>(dq, s_k + row0 * P, one, one);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = ty + 16 * i;
+    for (int i = 0; i < 2; i++) {
+        const int r = row0 + (lane_id() >> 2) + 8 * i;
         if (r >= n_rows) continue;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
-#pragma unroll
-        for (int j = 0; j < C; j++) {
-            const int d = column<DP>(tx, j);
-            if (d >= a.dim) continue;
-            const float v = value_of(dq[i], j) * a.scale;
-            if (a.splits > 1) a.part[((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim + d] = v;
-            else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(v);
-        }
+        if (a.splits > 1) store_row<DP>(a.part + ((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim, dq, i, a.scale, a.dim);
+        else store_row<DP>(static_cast<T *>(a.to) + row * a.dim, dq, i, a.scale, a.dim);
     }
 }
 
@@ -520,14 +567,13 @@ __global__ void __launch_bounds__(kThreads)
 grad_keys_kernel(const __grid_constant__ Args a)
 {
     pdl_begin();
-    constexpr int P = kPitch<DP>, C = DP / 16;
+    constexpr int P = kPitch<DP>, S = kStages<DP>;
+    constexpr bool kExact = sizeof(T) == 2;
     extern __shared__ __align__(16) float s_mem[];
-    constexpr int S = kStages<DP>;
-    float *s_q = s_mem, *s_g = s_q + S * kRows * P, *s_k = s_g + S * kRows * P, *s_v = s_k + kRows * P, *s_p = s_v + kRows * P,
-          *s_d = s_p + kRows * kPitchP;
+    float *s_q = s_mem, *s_g = s_q + S * kRows * P, *s_k = s_g + S * kRows * P, *s_v = s_k + kRows * P;
     __shared__ float2 s_stats_all[S][kRows];
     __shared__ unsigned char s_seen[kRows];
-    const int t = threadIdx.x, ty = t >> 4, tx = t & 15, kv = blockIdx.y;
+    const int t = threadIdx.x, row0 = (t >> 5) % 4 * kWarpRows, column0 = (t >> 7) * kWarpColumns, kv = blockIdx.y;
     const Tile tile = block_tile(a.rs_k, a.n_k, a.n_events, kRows);
     if (tile.begin >= tile.end) return;
     const int n_keys = tile.end - tile.begin, tokens = kRows / a.pack;
@@ -554,54 +600,52 @@ grad_keys_kernel(const __grid_constant__ Args a)
     };
     if (S > 1) load(part.x * packs);
     const float c = a.scale * kLog2e;
-    mma::pair dk[4][C / 2] = {}, dv[4][C / 2] = {};
-    bool seen[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = ty + 16 * i;
-        seen[i] = s_seen[r];
-    }
+    float dk[DP / 8][4] = {}, dv[DP / 8][4] = {};
+    const bool seen[2] = {s_seen[row0 + (lane_id() >> 2)] != 0, s_seen[row0 + (lane_id() >> 2) + 8] != 0};
     for (int step = part.x * packs; step < part.y * packs; step++) {
-        const int n = min(tokens, queries.y - (queries.x + step / packs * tokens)) * a.pack;
         __syncthreads();  // the buffers that are filled now have been read
         load(step + S - 1);
         copied<S - 1>();
         __syncthreads();
-        const float *q_now = s_q + step % S * kRows * P, *g_now = s_g + step % S * kRows * P;
-        const float2 *s_stats = s_stats_all[step % S];
-        float s[4][4] = {}, dp[4][4] = {};
-        dots<DP, 4>(s, s_k, q_now, ty, tx);
-        dots<DP, 4>(dp, s_v, g_now, ty, tx);
+        const float *q_now = s_q + step % S * kRows * P + column0 * P, *g_now = s_g + step % S * kRows * P + column0 * P;
+        const float2 *s_stats = s_stats_all[step % S] + column0 + 2 * (lane_id() & 3);
+        float s[kBlocks][4], dp[kBlocks][4];
+        dots<DP, kExact>(s, s_k + row0 * P, q_now, a.dim);
+        dots<DP, kExact>(dp, s_v + row0 * P, g_now, a.dim);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int n = 0; n < kBlocks; n++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool in = seen[i] && tx + 16 * j < n;
-                const float p = in ? exp2f(fmaf(s[i][j], c, -s_stats[tx + 16 * j].x)) : 0.f;
-                s_p[(ty + 16 * i) * kPitchP + tx + 16 * j] = p;
-                s_d[(ty + 16 * i) * kPitchP + tx + 16 * j] = in && varies ? p * (dp[i][j] - s_stats[tx + 16 * j].y) : 0.f;
+            for (int i = 0; i < 4; i++) {
+                const float2 stat = s_stats[8 * n + (i & 1)];  // infinity where there is no query
+                s[n][i] = seen[i >> 1] ? exp2f(fmaf(s[n][i], c, -stat.x)) : 0.f;
+                dp[n][i] = seen[i >> 1] && varies ? s[n][i] * (dp[n][i] - stat.y) : 0.f;
             }
-        __syncthreads();
-        weighted_rows<DP, 4>(dv, s_p, g_now, ty, tx);
-        weighted_rows<DP, 4>(dk, s_d, q_now, ty, tx);
+        weighted_rows<DP, kExact>(dv, s, g_now, a.dim);
+        weighted_rows<DP, kExact>(dk, dp, q_now, a.dim);
     }
+    copied<0>();
+    __syncthreads();
+    if (column0 > 0) {
+        leave<DP>(s_q + row0 * P, dk);
+        leave<DP>(s_g + row0 * P, dv);
+    }
+    __syncthreads();
+    if (column0 > 0) return;
+    const float one[2] = {1.f, 1.f};
+    add<DP>(dk, s_q + row0 * P, one, one);
+    add<DP>(dv, s_g + row0 * P, one, one);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = ty + 16 * i;
+    for (int i = 0; i < 2; i++) {
+        const int r = row0 + (lane_id() >> 2) + 8 * i;
         if (r >= n_keys) continue;
         const long long row = (long long)(tile.begin + r) * a.kv_heads + kv;
-#pragma unroll
-        for (int j = 0; j < C; j++) {
-            const int d = column<DP>(tx, j);
-            if (d >= a.dim) continue;
-            if (a.splits > 1) {
-                const long long at = ((long long)blockIdx.z * a.n_k * a.kv_heads + row) * a.dim + d;
-                a.part[at] = value_of(dk[i], j) * a.scale;
-                a.part2[at] = value_of(dv[i], j);
-            } else {
-                static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(value_of(dk[i], j) * a.scale);
-                static_cast<T *>(a.to2)[row * a.dim + d] = from_float<T>(value_of(dv[i], j));
-            }
+        if (a.splits > 1) {
+            const long long at = ((long long)blockIdx.z * a.n_k * a.kv_heads + row) * a.dim;
+            store_row<DP>(a.part + at, dk, i, a.scale, a.dim);
+            store_row<DP>(a.part2 + at, dv, i, 1.f, a.dim);
+        } else {
+            store_row<DP>(static_cast<T *>(a.to) + row * a.dim, dk, i, a.scale, a.dim);
+            store_row<DP>(static_cast<T *>(a.to2) + row * a.dim, dv, i, 1.f, a.dim);
         }
     }
 }
@@ -647,10 +691,8 @@ int split_count(long long blocks, long long mean_steps, int per_sm, int least)
 // What a call of these sizes needs; the kernels and the workspace queries go by the same numbers.
 struct Plan {
     int group, pack, splits, splits_mma, parts_mma, alternate, pack_few, rows_few, splits_few, splits_q, splits_q_mma, splits_k, splits_k_mma;
-    long long tiles_q, tiles_q64, tiles_k;
+    long long tiles_q, tiles_k;
 };
-
-constexpr int kForwardTM = 4;
 
 bool sizes_ok(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
 {
@@ -667,15 +709,14 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     const int events = n_rs - 1;
     p.group = heads / kv_heads;
     p.pack = p.group <= kMaxPack ? p.group : 1;
-    const int tokens = kRows / p.pack, m = 16 * kForwardTM / p.pack;
-    p.tiles_q = tile_count(n_q, m, events);
-    p.tiles_q64 = tile_count(n_q, tokens, events);
+    const int tokens = kRows / p.pack;
+    p.tiles_q = tile_count(n_q, tokens, events);
     p.tiles_k = tile_count(n_k, kRows, events);
     const int some = events > 0 ? events : 1;
     // tiles that have rows, if the events are alike
     const auto filled = [&](int n, int rows) { return (long long)some * ((n / some + rows) / rows); };
     const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
-    p.splits = split_count(filled(n_q, m) * (heads / p.pack), steps_k, 4, 4);
+    p.splits = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 4, 4);
     const int mma_tokens = kMmaRows / p.pack;
     // events of no more rows than half a tile, and keys for both of its halves
     const long long steps_mma = n_k / some / mma_keys(dim);
@@ -749,9 +790,8 @@ template <typename C> BackwardBuffers carve_backward(C &c, const Plan &p, int n_
 
 template <typename T, int DP> int run_forward(const Args &a, const Plan &p, cudaStream_t stream)
 {
-    constexpr int M = 16 * kForwardTM;
-    const size_t smem = sizeof(float) * ((M + 2 * kStages<DP> * kRows) * kPitch<DP> + M * kPitchP);
-    return launch(forward_kernel<T, DP, kForwardTM>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a);
+    const size_t smem = sizeof(float) * (1 + 2 * kStages<DP>) * kRows * kPitch<DP>;
+    return launch(forward_kernel<T, DP>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a);
 }
 
 template <typename T> int join_gradient(const Args &a, long long n, cudaStream_t stream)
@@ -765,12 +805,12 @@ template <typename T> int join_gradient(const Args &a, long long n, cudaStream_t
 
 template <typename T, int DP> int run_grad_queries(const Args &a, const Plan &p, cudaStream_t stream)
 {
-    const size_t smem = sizeof(float) * ((2 + 2 * kStages<DP>) * kRows * kPitch<DP> + kRows * kPitchP);
-    return launch(grad_queries_kernel<T, DP>, dim3((unsigned)p.tiles_q64, a.heads / a.pack, a.splits), smem, stream, a);
+    const size_t smem = sizeof(float) * (2 + 2 * kStages<DP>) * kRows * kPitch<DP>;
+    return launch(grad_queries_kernel<T, DP>, dim3((unsigned)p.tiles_q, a.heads / a.pack, a.splits), smem, stream, a);
 }
 template <typename T, int DP> int run_grad_keys(const Args &a, const Plan &p, cudaStream_t stream)
 {
-    const size_t smem = sizeof(float) * ((2 + 2 * kStages<DP>) * kRows * kPitch<DP> + 2 * kRows * kPitchP);
+    const size_t smem = sizeof(float) * (2 + 2 * kStages<DP>) * kRows * kPitch<DP>;
     return launch(grad_keys_kernel<T, DP>, dim3((unsigned)p.tiles_k, a.kv_heads, a.splits), smem, stream, a);
 }
 
