@@ -56,8 +56,9 @@ __device__ __forceinline__ void dots(float (&s)[kBlocks][4], const float *__rest
     for (int n = 0; n < kBlocks; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) s[n][i] = rest[n][i] = 0.f;
-#pragma unroll 2
-    for (int d = 0; d < dim; d += 8) {
+#pragma unroll
+    for (int d = 0; d < DP; d += 8) {
+        if (d >= dim) break;
         unsigned a_big[4], a_small[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) in_two<EXACT>(a[at + (i & 1) * 8 * P + d + (i >> 1) * 4], a_big[i], a_small[i]);
@@ -257,7 +258,7 @@ forward_kernel(const __grid_constant__ Args a)
         __syncthreads();
         const float *k_now = s_k + step % S * kRows * P, *v_now = s_v + step % S * kRows * P;
         const unsigned char *s_seen = s_seen_all[step % S] + column0 + 2 * (lane_id() & 3);
-        float s[kBlocks][4], base[2];
+        float s[kBlocks][4];
         dots<DP, kExact>(s, s_q + row0 * P, k_now + column0 * P, a.dim);
 #pragma unroll
         for (int r = 0; r < 2; r++) {
@@ -271,22 +272,24 @@ forward_kernel(const __grid_constant__ Args a)
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            base[r] = top == -INFINITY ? 0.f : top;
-            const float shrink = exp2f((m[r] - base[r]) * c);
-            m[r] = top;
-            l[r] *= shrink;  // of this lane's columns
+            const float base = top == -INFINITY ? 0.f : top;
+            if (__any_sync(0xffffffffu, top > m[r])) {
+                const float shrink = mma::exp2_fast((m[r] - base) * c);
+                l[r] *= shrink;  // of this lane's columns
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++) {
+                    o[n][2 * r] *= shrink;
+                    o[n][2 * r + 1] *= shrink;
+                }
+                m[r] = top;
+            }
 #pragma unroll
             for (int n = 0; n < kBlocks; n++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    s[n][2 * r + i] = exp2f((s[n][2 * r + i] - base[r]) * c);
+                    s[n][2 * r + i] = mma::exp2_fast((s[n][2 * r + i] - base) * c);
                     l[r] += s[n][2 * r + i];
                 }
-#pragma unroll
-            for (int n = 0; n < DP / 8; n++) {
-                o[n][2 * r] *= shrink;
-                o[n][2 * r + 1] *= shrink;
-            }
         }
         weighted_rows<DP, kExact>(o, s, v_now + column0 * P, a.dim);
     }
@@ -541,7 +544,7 @@ grad_queries_kernel(const __grid_constant__ Args a)
         for (int n = 0; n < kBlocks; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                s[n][i] = s_seen[8 * n + (i & 1)] ? exp2f(fmaf(s[n][i], c, -lse[i >> 1])) * (dp[n][i] - delta[i >> 1]) : 0.f;
+                s[n][i] = s_seen[8 * n + (i & 1)] ? mma::exp2_fast(fmaf(s[n][i], c, -lse[i >> 1])) * (dp[n][i] - delta[i >> 1]) : 0.f;
         weighted_rows<DP, kExact>(dq, s, k_now, a.dim);
     }
     copied<0>();
@@ -617,7 +620,7 @@ grad_keys_kernel(const __grid_constant__ Args a)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float2 stat = s_stats[8 * n + (i & 1)];  // infinity where there is no query
-                s[n][i] = seen[i >> 1] ? exp2f(fmaf(s[n][i], c, -stat.x)) : 0.f;
+                s[n][i] = seen[i >> 1] ? mma::exp2_fast(fmaf(s[n][i], c, -stat.x)) : 0.f;
                 dp[n][i] = seen[i >> 1] && varies ? s[n][i] * (dp[n][i] - stat.y) : 0.f;
             }
         weighted_rows<DP, kExact>(dv, s, g_now, a.dim);
@@ -728,9 +731,9 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     p.pack_few = few_pack(p.group);
     p.rows_few = few_rows(n_q, events, p.pack_few);
     p.splits_few = p.rows_few > 0 ? split_count(filled(n_q, p.rows_few / p.pack_few) * (heads / p.pack_few), n_k / some / kFewStep, 20, 4) : 1;
-    p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 2, 4);
+    p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 6, 4);
     p.splits_q_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / kMmaGradStep, 4, 4);
-    p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 2, 4);
+    p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 6, 4);
     p.splits_k_mma = split_count(filled(n_k, kMmaRows) * kv_heads, n_q / some / (kMmaGradStep / p.pack), 2, 4);
     return p;
 }
