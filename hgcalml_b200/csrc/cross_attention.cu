@@ -22,7 +22,8 @@ constexpr int kWarpRows = 16, kWarpColumns = 32, kBlocks = kWarpColumns / 8;  //
 // big big + big small + small big, off by what is left of either, 2^-21, and by small small, 2^-22.  Tensor cores cut off what an
 // addition leaves, so the small products have a sum of their own, and sums are taken on from there with rounding, once a step.
 // On the CUDA cores a tile of 4 x 4 per thread waited for shared memory half of the time (7 events of some 16k rows on 2.6k, 22 columns:
-// 4661 us, here 3053; a training step on three of 7k on 2k, 32 columns: 4596, here 3312), and was less exact.
+// 4661 us, here 2868; a training step on three of 7k on 2k, 32 columns: 4596, here 2739), and was less exact.  What bounds it: sixteen
+// warps, for which there are registers, with ten instructions to a product; the tensor cores are half busy.
 // 16-bit values are operands as they are (`EXACT`).
 //
 // A lane of a warp has the rows g and g + 8, g = lane / 4, and of 8 columns those from 2 (lane % 4) on.  What one product leaves is an
@@ -719,7 +720,9 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     // tiles that have rows, if the events are alike
     const auto filled = [&](int n, int rows) { return (long long)some * ((n / some + rows) / rows); };
     const long long steps_k = n_k / some / kRows, steps_q = n_q / some / tokens;
-    p.splits = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 4, 4);
+    // two blocks are resident: parts for many rounds of them, so that the last round counts little (a training step of three small events
+    // with 4 and 6 blocks a multiprocessor 2836 us, with 8 and 20 2739)
+    p.splits = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 8, 4);
     const int mma_tokens = kMmaRows / p.pack;
     // events of no more rows than half a tile, and keys for both of its halves
     const long long steps_mma = n_k / some / mma_keys(dim);
@@ -731,9 +734,9 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     p.pack_few = few_pack(p.group);
     p.rows_few = few_rows(n_q, events, p.pack_few);
     p.splits_few = p.rows_few > 0 ? split_count(filled(n_q, p.rows_few / p.pack_few) * (heads / p.pack_few), n_k / some / kFewStep, 20, 4) : 1;
-    p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 6, 4);
+    p.splits_q = split_count(filled(n_q, tokens) * (heads / p.pack), steps_k, 20, 4);
     p.splits_q_mma = split_count(filled(n_q, mma_tokens) * (heads / p.pack), n_k / some / kMmaGradStep, 4, 4);
-    p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 6, 4);
+    p.splits_k = split_count(filled(n_k, kRows) * kv_heads, steps_q, 20, 4);
     p.splits_k_mma = split_count(filled(n_k, kMmaRows) * kv_heads, n_q / some / (kMmaGradStep / p.pack), 2, 4);
     return p;
 }
