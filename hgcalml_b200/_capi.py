@@ -74,9 +74,9 @@ def _load():
         "hgc_select_knn_grad_ordered": (I, [P] * 5 + [I] * 3 + [P, P, S, P]),
         "hgc_select_knn_grad_after": (I, [P] * 5 + [I] * 3 + [P, P, S, P]),
         "hgc_cross_attention_workspace_bytes": (S, [I] * 7),
-        "hgc_cross_attention": (I, [P] * 8 + [I] * 6 + [P, ctypes.c_float, I, P, S, P]),
+        "hgc_cross_attention": (I, [P] * 9 + [I] * 6 + [P, ctypes.c_float, I, P, S, P]),
         "hgc_cross_attention_grad_workspace_bytes": (S, [I] * 7),
-        "hgc_cross_attention_grad": (I, [P] * 12 + [I] * 6 + [P, ctypes.c_float, I, P, S, P]),
+        "hgc_cross_attention_grad": (I, [P] * 13 + [I] * 6 + [P, ctypes.c_float, I, P, S, P]),
         "hgc_norm_rotate": (I, [P, I, I, I, I, I, I, ctypes.c_double, ctypes.c_float, I, P]),
         "hgc_norm_rotate_grad_workspace_bytes": (S, [P, I, I]),
         "hgc_norm_rotate_grad": (I, [P, I, I, I, I, I, I, ctypes.c_double, ctypes.c_float, I, P, S, P]),

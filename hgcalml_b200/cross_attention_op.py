@@ -53,24 +53,30 @@ def _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key
     return _rows(q), _rows(k), _rows(v), rs_q, rs_k, scale, key_mask
 
 
-def _forward(q, k, v, rs_q, rs_k, scale, mask):
-    out, lse, rc = C.native.cross_attention(q, k, v, rs_q, rs_k, mask, scale)
+def _forward(q, k, v, rs_q, rs_k, scale, mask, with_rest=False):
+    out, rest, lse, rc = C.native.cross_attention(q, k, v, rs_q, rs_k, mask, scale, with_rest)
     C.check(rc, "CrossAttention")
-    return out, lse
+    return out, rest, lse
 
 
 def CrossAttentionGrad(grad, queries, keys, values, out, lse, query_row_splits, key_row_splits, scale=None, key_mask=None,
-                       need_queries=True, need_keys=True):
+                       need_queries=True, need_keys=True, out_rest=None):
     """Gradients ``(queries, keys, values)`` of ``CrossAttention`` (None for what is not needed; those of keys and values
-    come together).  ``out`` and ``lse`` are the forward pass's."""
+    come together).  ``out`` and ``lse`` are the forward pass's.  ``out_rest``: what is left of the rows in 16 bits when
+    they are rounded, of their type, if known; it makes up for their rounding where few keys have all the weight."""
     q, k, v, rs_q, rs_k, scale, mask = _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key_mask)
     C.require_cuda(grad, out, lse)
     if grad.shape != q.shape or out.shape != q.shape or lse.shape != q.shape[:2]:
         raise C.HgcError("CrossAttentionGrad expects grad and out like the queries and one lse per row and head")
     if out.dtype != q.dtype or lse.dtype != torch.float32 or any(t.device != q.device for t in (grad, out, lse)):
         raise C.HgcError("CrossAttentionGrad expects out and lse as CrossAttention returned them, and grad beside them")
-    dq, dk, dv, rc = C.native.cross_attention_grad(grad.to(q.dtype).contiguous(), q, k, v, out.contiguous(), lse.contiguous(), rs_q,
-                                                   rs_k, mask, scale, need_queries, need_keys)
+    if out_rest is not None:
+        C.require_cuda(out_rest)
+        if out_rest.shape != out.shape or out_rest.dtype != out.dtype or out_rest.device != out.device:
+            raise C.HgcError("CrossAttentionGrad expects out_rest like out")
+        out_rest = out_rest.contiguous()
+    dq, dk, dv, rc = C.native.cross_attention_grad(grad.to(q.dtype).contiguous(), q, k, v, out.contiguous(), out_rest, lse.contiguous(),
+                                                   rs_q, rs_k, mask, scale, need_queries, need_keys)
     C.check(rc, "CrossAttentionGrad")
     return dq, dk, dv
 
@@ -78,8 +84,8 @@ def CrossAttentionGrad(grad, queries, keys, values, out, lse, query_row_splits, 
 class _CrossAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, rs_q, rs_k, scale, mask):
-        out, lse = _forward(q, k, v, rs_q, rs_k, scale, mask)
-        ctx.save_for_backward(q, k, v, out, lse, rs_q, rs_k, mask)
+        out, rest, lse = _forward(q, k, v, rs_q, rs_k, scale, mask, with_rest=ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
+        ctx.save_for_backward(q, k, v, out, rest, lse, rs_q, rs_k, mask)
         ctx.scale = scale
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)  # no zeros for the logarithms
@@ -90,9 +96,9 @@ class _CrossAttentionFunction(torch.autograd.Function):
     def backward(ctx, grad, _grad_lse):
         if grad is None:
             return (None,) * 7
-        q, k, v, out, lse, rs_q, rs_k, mask = ctx.saved_tensors
+        q, k, v, out, rest, lse, rs_q, rs_k, mask = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        dq, dk, dv = CrossAttentionGrad(grad, q, k, v, out, lse, rs_q, rs_k, ctx.scale, mask, need_q, need_k or need_v)
+        dq, dk, dv = CrossAttentionGrad(grad, q, k, v, out, lse, rs_q, rs_k, ctx.scale, mask, need_q, need_k or need_v, rest)
         return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
@@ -113,5 +119,5 @@ def CrossAttention(queries, keys, values, query_row_splits, key_row_splits, scal
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _CrossAttentionFunction.apply(q, k, v, rs_q, rs_k, scale, mask)
     else:
-        out, lse = _forward(q, k, v, rs_q, rs_k, scale, mask)
+        out, _, lse = _forward(q, k, v, rs_q, rs_k, scale, mask)
     return (out, lse) if with_lse else out

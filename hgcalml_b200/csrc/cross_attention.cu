@@ -129,26 +129,26 @@ template <int DP> __device__ __forceinline__ void add(float (&acc)[DP / 8][4], c
         for (int i = 0; i < 4; i++) acc[n][i] = acc[n][i] * mine[i >> 1] + at[(i >> 1) * 8 * kPitch<DP> + 8 * n + (i & 1)] * theirs[i >> 1];
 }
 // Row `row` (0, or 1: 8 further) of a warp's results, times `factor`, to `to`.
-template <int DP, typename T> __device__ __forceinline__ void store_row(T *__restrict__ to, const float (&acc)[DP / 8][4], int row, float factor, int dim)
+template <int DP, typename T>
+__device__ __forceinline__ void store_row(T *__restrict__ to, const float (&acc)[DP / 8][4], int row, float factor, int dim, T *__restrict__ rest = nullptr)
 {
 #pragma unroll
     for (int n = 0; n < DP / 8; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int d = 8 * n + 2 * (lane_id() & 3) + i;
-            if (d < dim) to[d] = from_float<T>(acc[n][2 * row + i] * factor);
+            if (d < dim) store_rounded(to + d, rest == nullptr ? rest : rest + d, acc[n][2 * row + i] * factor);
         }
 }
 
 // Rows of one head as floats; what is not there, and the keys that cannot be seen, are zeros, whatever the memory holds: a weight of
-// zero would not make up for an infinity.  In float32 the copies are asynchronous, in pieces of 16, 8 or 4 bytes as the rows allow
-// (copied() waits for all but the last `ahead` groups); other types are converted on their way.
+// zero would not make up for an infinity.  Copies are in pieces of 16, 8 or 4 bytes as the rows allow, single values in 16 bits.
+// In float32 they are asynchronous (copied() waits for all but the last `ahead` groups); other types are converted on their way.
 template <typename T> __device__ __forceinline__ int piece_of(const Strided &s, int dim)
 {
-    if (sizeof(T) != 4) return 1;
-    const unsigned long long all = reinterpret_cast<unsigned long long>(s.p) | (unsigned long long)(s.row * 4) | (unsigned long long)(s.head * 4) |
-                                   (unsigned long long)(dim * 4);
-    return (all & 15u) == 0 ? 4 : (all & 7u) == 0 ? 2 : 1;
+    constexpr unsigned long long kSize = sizeof(T);
+    const unsigned long long all = reinterpret_cast<unsigned long long>(s.p) | s.row * kSize | s.head * kSize | dim * kSize;
+    return (all & 15u) == 0 ? 16 / sizeof(T) : kSize == 4 && (all & 7u) == 0 ? 2 : 1;
 }
 template <int N> __device__ __forceinline__ void copy_async(float *dst, const float *src, bool in)  // zeros where not `in`
 {
@@ -169,8 +169,17 @@ __device__ __forceinline__ void copy_rows(float *__restrict__ dst, const T *__re
         const int r = i / W, d = i % W * N;
         const long long at = place(r);
         const bool in = at >= 0 && d < dim;
-        if constexpr (sizeof(T) == 4) copy_async<N>(dst + r * kPitch<DP> + d, p + (in ? at + d : 0), in);
-        else dst[r * kPitch<DP> + d] = in ? to_float(p[at + d]) : 0.f;
+        if constexpr (sizeof(T) == 4) {
+            copy_async<N>(dst + r * kPitch<DP> + d, p + (in ? at + d : 0), in);
+        } else if constexpr (N == 8) {
+            const uint4 v = in ? *reinterpret_cast<const uint4 *>(p + at + d) : make_uint4(0, 0, 0, 0);
+            const float2 f[4] = {mma::unpack2<T>(v.x), mma::unpack2<T>(v.y), mma::unpack2<T>(v.z), mma::unpack2<T>(v.w)};
+            float4 *to = reinterpret_cast<float4 *>(dst + r * kPitch<DP> + d);
+            to[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+            to[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+        } else {
+            dst[r * kPitch<DP> + d] = in ? to_float(p[at + d]) : 0.f;
+        }
     }
 }
 template <typename T, int DP, typename Place>
@@ -180,6 +189,8 @@ __device__ __forceinline__ void load_rows(float *__restrict__ dst, const Strided
     if constexpr (sizeof(T) == 4) {
         if (piece == 4) return copy_rows<T, DP, 4>(dst, p, dim, place);
         if (piece == 2) return copy_rows<T, DP, 2>(dst, p, dim, place);
+    } else {
+        if (piece == 8) return copy_rows<T, DP, 8>(dst, p, dim, place);
     }
     copy_rows<T, DP, 1>(dst, p, dim, place);
 }
@@ -327,7 +338,7 @@ forward_kernel(const __grid_constant__ Args a)
         float *lse_to = a.splits > 1 ? a.part_lse + (long long)blockIdx.z * a.n_q * a.heads : a.lse;
         if ((lane_id() & 3) == 0) lse_to[row] = l[i] == 0.f ? -INFINITY : m[i] * a.scale + logf(l[i]);
         if (a.splits > 1) store_row<DP>(a.part + ((long long)blockIdx.z * a.n_q * a.heads + row) * a.dim, o, i, inv, a.dim);
-        else store_row<DP>(static_cast<T *>(a.to) + row * a.dim, o, i, inv, a.dim);
+        else store_row<DP>(static_cast<T *>(a.to) + row * a.dim, o, i, inv, a.dim, a.rest == nullptr ? nullptr : static_cast<T *>(a.rest) + row * a.dim);
     }
 }
 
@@ -335,8 +346,8 @@ forward_kernel(const __grid_constant__ Args a)
 constexpr int kMaxParts = 128;
 template <typename T>
 __global__ void __launch_bounds__(256)
-join_forward_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, T *__restrict__ out, float *__restrict__ lse,
-                    long long n_rows, int dim, int splits)
+join_forward_kernel(const float *__restrict__ part, const float *__restrict__ part_lse, T *__restrict__ out, T *__restrict__ rest,
+                    float *__restrict__ lse, long long n_rows, int dim, int splits)
 {
     pdl_begin();
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -374,7 +385,7 @@ join_forward_kernel(const float *__restrict__ part, const float *__restrict__ pa
                 o = fmaf(w, w == 0.f ? 0.f : v, o);
             }
         }
-        if (d < dim) out[row * dim + d] = from_float<T>(o * inv);
+        if (d < dim) store_rounded(out + row * dim + d, rest == nullptr ? rest : rest + row * dim + d, o * inv);
     }
     if (lane_id() == 0) lse[row] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
@@ -415,17 +426,19 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
     const long long all = of_queries ? (long long)a.n_q * a.heads : (long long)a.n_k * a.kv_heads;
     const long long first = (long long)(of_queries ? block : block - n_rows) * (subs * kRowsALane) + t / lanes;
     const int known = of_queries ? split_at(a.rs_q, a.n_events, a.n_q) : split_at(a.rs_k, a.n_events, a.n_k);  // rows of some event
-    const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ grad = static_cast<const T *>(a.grad);
+    const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ rest = static_cast<const T *>(a.out_rest),
+            *__restrict__ grad = static_cast<const T *>(a.grad);
     float sum[kRowsALane], square[kRowsALane];
     if (whole) {
-        Vec x[kRowsALane], y[kRowsALane];
+        Vec x[kRowsALane], y[kRowsALane], z[kRowsALane];
 #pragma unroll
         for (int i = 0; i < kRowsALane; i++) {
             const long long row = first + (long long)i * subs;
             const bool in = row < all && lane * V < a.dim;
-            x[i] = y[i] = Vec{};
+            x[i] = y[i] = z[i] = Vec{};
             if (in && of_queries) {
                 x[i] = *reinterpret_cast<const Vec *>(out + row * a.dim + lane * V);
+                if (sizeof(T) == 2 && rest != nullptr) z[i] = *reinterpret_cast<const Vec *>(rest + row * a.dim + lane * V);
                 y[i] = *reinterpret_cast<const Vec *>(grad + row * a.dim + lane * V);
             } else if (in) {
                 const int key = (int)(row / a.kv_heads);
@@ -438,7 +451,7 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
 #pragma unroll
             for (int d = 0; d < V; d++) {
                 const float g = to_float(y[i].v[d]);
-                sum[i] = fmaf(to_float(x[i].v[d]), g, sum[i]);
+                sum[i] = fmaf(to_float(x[i].v[d]) + to_float(z[i].v[d]), g, sum[i]);
                 square[i] = fmaf(g, g, square[i]);
             }
         }
@@ -451,7 +464,7 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
                 const int key = of_queries ? 0 : (int)(row / a.kv_heads);
                 const float g = of_queries ? to_float(grad[row * a.dim + d])
                                            : to_float(static_cast<const T *>(a.v.p)[key * a.v.row + (row - (long long)key * a.kv_heads) * a.v.head + d]);
-                if (of_queries) sum[i] = fmaf(to_float(out[row * a.dim + d]), g, sum[i]);
+                if (of_queries) sum[i] = fmaf(to_float(out[row * a.dim + d]) + (rest == nullptr ? 0.f : to_float(rest[row * a.dim + d])), g, sum[i]);
                 square[i] = fmaf(g, g, square[i]);
             }
         }
@@ -834,7 +847,8 @@ template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStrea
         return rc;
     if (parts == 1) return HGC_OK;
     const long long rows = (long long)a.n_q * a.heads;
-    HGC_CUDA_TRY(launch_pdl(join_forward_kernel<T>, div_up(rows, 8), 256, 0, stream, a.part, a.part_lse, static_cast<T *>(a.to), a.lse, rows, a.dim,
+    HGC_CUDA_TRY(launch_pdl(join_forward_kernel<T>, div_up(rows, 8), 256, 0, stream, a.part, a.part_lse, static_cast<T *>(a.to), static_cast<T *>(a.rest),
+                            a.lse, rows, a.dim,
                             parts));
     HGC_LAUNCH_CHECK();
     return HGC_OK;
@@ -848,7 +862,7 @@ int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void 
     // whole 16-byte vectors of rows where they are that
     constexpr int V = 16 / sizeof(T);
     int lanes_log2 = -1;
-    if (a.dim % V == 0 && aligned(a.out) && aligned(a.grad) && (!bounded || (aligned(a.v.p) && a.v.row % V == 0 && a.v.head % V == 0)))
+    if (a.dim % V == 0 && aligned(a.out) && aligned(a.out_rest) && aligned(a.grad) && (!bounded || (aligned(a.v.p) && a.v.row % V == 0 && a.v.head % V == 0)))
         for (lanes_log2 = 0; (V << lanes_log2) < a.dim; lanes_log2++) {}
     const int rows_a_block = kThreads / (lanes_log2 >= 0 ? 1 << lanes_log2 : 32) * kRowsALane;
     const int n_count = a.n_events > 0 ? a.n_events : 1, n_rows = div_up((long long)a.n_q * a.heads, rows_a_block),
@@ -918,7 +932,7 @@ extern "C" size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs
 }
 
 extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void *d_v, const int *d_q_row_splits, const int *d_k_row_splits,
-                                   const unsigned char *d_key_mask, void *d_out, float *d_lse, int n_q, int n_k, int n_rs, int n_heads,
+                                   const unsigned char *d_key_mask, void *d_out, void *d_out_rest, float *d_lse, int n_q, int n_k, int n_rs, int n_heads,
                                    int n_kv_heads, int dim, const long long *strides, float scale, int dtype, void *workspace,
                                    size_t workspace_bytes, hgc_stream_t stream_)
 {
@@ -936,7 +950,7 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
                      workspace);
     Carver carver(workspace);
     const ForwardBuffers b = carve_forward(carver, p, n_q, n_heads, dim);
-    a.to = d_out; a.part = b.part; a.part_lse = b.part_lse; a.counter = b.counter;
+    a.to = d_out; a.rest = dtype == HGC_FLOAT32 ? nullptr : d_out_rest; a.part = b.part; a.part_lse = b.part_lse; a.counter = b.counter;
     return dtype == HGC_FLOAT32 ? forward_of<float>(a, p, dtype, stream)
          : dtype == HGC_FLOAT16 ? forward_of<__half>(a, p, dtype, stream) : forward_of<__nv_bfloat16>(a, p, dtype, stream);
 }
@@ -951,7 +965,7 @@ extern "C" size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int
 }
 
 extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q, const void *d_k, const void *d_v, const void *d_out,
-                                        const float *d_lse, const int *d_q_row_splits, const int *d_k_row_splits,
+                                        const void *d_out_rest, const float *d_lse, const int *d_q_row_splits, const int *d_k_row_splits,
                                         const unsigned char *d_key_mask, void *d_grad_q, void *d_grad_k, void *d_grad_v, int n_q, int n_k,
                                         int n_rs, int n_heads, int n_kv_heads, int dim, const long long *strides, float scale, int dtype,
                                         void *workspace, size_t workspace_bytes, hgc_stream_t stream_)
@@ -972,7 +986,7 @@ extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q,
                      strides, scale, p, workspace);
     Carver carver(workspace);
     const BackwardBuffers b = carve_backward(carver, p, n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
-    a.grad = d_grad_out; a.out = d_out;
+    a.grad = d_grad_out; a.out = d_out; a.out_rest = dtype == HGC_FLOAT32 ? nullptr : d_out_rest;
     return dtype == HGC_FLOAT32 ? backward_of<float>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream)
          : dtype == HGC_FLOAT16 ? backward_of<__half>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream)
                                 : backward_of<__nv_bfloat16>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream);

@@ -29,6 +29,8 @@ struct Args {
     const int *rs_q, *rs_k;        // [n_events + 1]
     const unsigned char *mask;     // [n_k], zero: no query sees the key; may be null
     const void *grad, *out;        // of the backward pass
+    const void *out_rest;          // what the rounding of out left, or null
+    void *rest;                    // of the forward pass: where that goes, or null
     const float2 *stats;           // [n_q, heads]: what the exponents of a row's weights are less by, and delta, the sum of out * grad
     const int *visible;            // [n_events], keys that can be seen, counted up to two
     float *lse;                    // [n_q, heads], natural logarithm of the sum of exp(scale * q.k)
@@ -107,6 +109,13 @@ template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// A value, and what its rounding leaves where that is kept.
+template <typename T> __device__ __forceinline__ void store_rounded(T *to, T *rest, float v)
+{
+    *to = from_float<T>(v);
+    if (sizeof(T) == 2 && rest != nullptr) *rest = from_float<T>(v - to_float<T>(*to));
+}
 
 // keys of an event; none behind the last one
 __device__ __forceinline__ int2 rows_of(const int *rs, int n, int n_events, int event)

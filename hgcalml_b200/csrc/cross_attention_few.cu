@@ -29,13 +29,10 @@ template <typename T> __device__ __forceinline__ void unpack(mma::pair (&to)[kVe
     if constexpr (sizeof(T) == 4) {
         to[0] = mma::pair_of(__uint_as_float(u[0]), __uint_as_float(u[1]));
         to[1] = mma::pair_of(__uint_as_float(u[2]), __uint_as_float(u[3]));
-    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) to[i] = mma::pair_of(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+            const float2 f = mma::unpack2<T>(u[i]);
             to[i] = mma::pair_of(f.x, f.y);
         }
     }
@@ -226,7 +223,7 @@ few_kernel(const __grid_constant__ Args a, int lanes_log2)
         o = none ? 0.f : o / total;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
         if (a.splits > 1) a.part[(blockIdx.z * all_rows + row) * a.dim + d] = o;
-        else static_cast<T *>(a.to)[row * a.dim + d] = from_float<T>(o);
+        else store_rounded(static_cast<T *>(a.to) + row * a.dim + d, a.rest == nullptr ? nullptr : static_cast<T *>(a.rest) + row * a.dim + d, o);
         if (d == 0) (a.splits > 1 ? a.part_lse + blockIdx.z * all_rows : a.lse)[row] = none ? -INFINITY : most * kLn2 + logf(total);
     }
 }

@@ -62,9 +62,9 @@ struct Rows {
         store_other = __shfl_xor_sync(0xffffffffu, (int)in, 1) != 0;
     }
 };
-// 16 columns of a row of a result; all lanes of a warp call this.
+// 16 columns of a row of a result; all lanes of a warp call this.  rest: for what the rounding leaves, or null.
 template <typename T>
-__device__ __forceinline__ void store16(void *to, float *part, const Rows &rows, int d, int dim, const unsigned (&v)[16], float factor)
+__device__ __forceinline__ void store16(void *to, void *rest, float *part, const Rows &rows, int d, int dim, const unsigned (&v)[16], float factor)
 {
     float x[16];
 #pragma unroll
@@ -75,17 +75,27 @@ __device__ __forceinline__ void store16(void *to, float *part, const Rows &rows,
         for (int i = 0; i < 4; i++)
             if (rows.store && d + 4 * i < dim) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
     } else {
-        uint4 a = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
-        uint4 b = make_uint4(pack2<T>(x[8], x[9]), pack2<T>(x[10], x[11]), pack2<T>(x[12], x[13]), pack2<T>(x[14], x[15]));
-        // first the even lanes' rows: they keep their first 16 bytes and give away the second; then the odd ones'
-        const bool odd = lane_id() & 1;
-        const uint4 give = odd ? a : b;
-        const uint4 got = make_uint4(__shfl_xor_sync(0xffffffffu, give.x, 1), __shfl_xor_sync(0xffffffffu, give.y, 1),
-                                     __shfl_xor_sync(0xffffffffu, give.z, 1), __shfl_xor_sync(0xffffffffu, give.w, 1));
-        T *const base = static_cast<T *>(to) + d + (odd ? 8 : 0);
-        if (d + (odd ? 8 : 0) < dim) {
-            if (odd ? rows.store_other : rows.store) *reinterpret_cast<uint4 *>(base + (odd ? rows.other : rows.at)) = odd ? got : a;
-            if (odd ? rows.store : rows.store_other) *reinterpret_cast<uint4 *>(base + (odd ? rows.at : rows.other)) = odd ? b : got;
+#pragma unroll 1
+        for (void *next = to; next != nullptr; next = next == to ? rest : nullptr) {
+            unsigned h[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                h[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+                const float2 there = unpack2<T>(h[i]);
+                x[2 * i] -= there.x;
+                x[2 * i + 1] -= there.y;
+            }
+            const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+            // first the even lanes' rows: they keep their first 16 bytes and give away the second; then the odd ones'
+            const bool odd = lane_id() & 1;
+            const uint4 give = odd ? a : b;
+            const uint4 got = make_uint4(__shfl_xor_sync(0xffffffffu, give.x, 1), __shfl_xor_sync(0xffffffffu, give.y, 1),
+                                         __shfl_xor_sync(0xffffffffu, give.z, 1), __shfl_xor_sync(0xffffffffu, give.w, 1));
+            T *const base = static_cast<T *>(next) + d + (odd ? 8 : 0);
+            if (d + (odd ? 8 : 0) < dim) {
+                if (odd ? rows.store_other : rows.store) *reinterpret_cast<uint4 *>(base + (odd ? rows.other : rows.at)) = odd ? got : a;
+                if (odd ? rows.store : rows.store_other) *reinterpret_cast<uint4 *>(base + (odd ? rows.at : rows.other)) = odd ? b : got;
+            }
         }
     }
 }
@@ -106,7 +116,7 @@ template <int CHUNKS> struct Forward {
     static constexpr int kTileBytes = kKeys * kTile * CHUNKS, kHalfBytes = kMmaRows * kTile * CHUNKS, kQueryBytes = 2 * kHalfBytes;
     static constexpr int kBuffers = CHUNKS == 1 ? 3 : 4, kOut = kKeys * kBuffers, kColumns = 512, kItems = 4;
     static constexpr int kTiles = kQueries * kQueryBytes + 2 * kStages * kTileBytes;
-    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers + 2 * kQueries + 2 * kItems + 4 + 8;
+    static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers + 2 * kQueries + 3 * kItems + 4 + 8;
     static constexpr int kBias = 512, kMaxAt = kBias + kStages * kKeys * 4, kItemAt = kMaxAt + 2 * 3 * 2 * kMmaRows * 4,
                          kSmem = kTiles + kItemAt + kItems * 48;  // behind the tiles
     static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= kBias && kSmem <= 232448, "room");
@@ -145,7 +155,8 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
     const unsigned bar = s_q + F::kTiles, scores_done = bar, sums_done = bar + 8, go = bar + 16, full = bar + 24, empty = full + 8 * F::kStages,
                    clean = empty + 8 * F::kStages, s_full = clean + 8 * F::kStages, p_full = s_full + 8 * B, used = p_full + 8 * B,
                    q_full = used + 8 * B, q_empty = q_full + 8 * F::kQueries, item_full = q_empty + 8 * F::kQueries,
-                   item_empty = item_full + 8 * F::kItems, o_full = item_empty + 8 * F::kItems, o_empty = o_full + 16, meet = o_empty + 16;
+                   item_empty = item_full + 8 * F::kItems, o_full = item_empty + 8 * F::kItems, o_empty = o_full + 16,
+                   item_done = o_empty + 16, meet = item_done + 8 * F::kItems;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + 8 * F::kBarriers);
     volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
     float *s_bias = reinterpret_cast<float *>(s_raw + F::kTiles + F::kBias);  // [kStages][kKeys], 0 or minus infinity
@@ -393,11 +404,15 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
         while (ok) {
             ok = wait_warp<true>(item_full + 8 * item.at, item.turn, gave_up, a.status);
             const Item it = s_item[item.at];
-            __syncwarp();
-            if (lane == 0) arrive(item_empty + 8 * item.at);
-            item.go(1);
             if (!ok || it.steps < 0) break;
-            const int groups = it.end - it.begin > tokens ? 2 : 1, begin = it.begin + (alternate ? 0 : g * tokens);
+            const int groups = it.end - it.begin > tokens ? 2 : 1, begin = it.begin + (alternate ? 0 : g * tokens), slot = item.at;
+            // The second half may have no steps.  It must not go on all the same: a wait tells a barrier's phases apart by their parity only,
+            // and would take the phase before the last for the next one.  It goes on when the first half has seen all scores of the item.
+            if (g == 1 && it.steps > 0 && groups == 1 && (!alternate || it.steps == 1))
+                ok = wait_warp<true>(item_done + 8 * slot, item.turn, gave_up, a.status);
+            __syncwarp();
+            if (g == 1 && lane == 0) arrive(item_empty + 8 * slot);
+            item.go(1);
             const int n_rows = min(tokens, it.end - begin) * a.pack;
             const bool some = it.steps > (alternate ? g : 0);  // steps for this half
             int count = 0;
@@ -445,8 +460,8 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                     next = fmaxf(next, exchange(maxima + (count & 1) * 2 * kMmaRows, next));
                     // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing
-                    // in either type.
-                    const bool grown = (next - top) * c > 8.f;
+                    // in either type.  Rows that do not count have no say: what stands there may differ from run to run.
+                    const bool grown = store && (next - top) * c > 8.f;
                     if (count == 0) {
                         top = next;
                     } else if (__any_sync(0xffffffffu, grown)) {
@@ -494,6 +509,13 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 buffer.go(groups == 1 || (g == 1 && j == it.steps - 1) ? 1 : 2);
                 count++;
             }
+            if (g == 0) {  // in this order: the next item in this slot has the next phase
+                __syncwarp();
+                if (lane == 0) {
+                    arrive(item_done + 8 * slot);
+                    arrive(item_empty + 8 * slot);
+                }
+            }
             if (g >= groups && !alternate) continue;
             const bool done = some && ok && wait_warp<true>(o_full + 8 * g, o_turn ^ 1, gave_up, a.status);
             if (done) after_sync();
@@ -516,7 +538,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     if (done) {
                         tmem_load16(o, out + d);
                     }
-                    store16<T>(a.to, to_part, to, d, a.dim, o, inv);
+                    store16<T>(a.to, a.rest, to_part, to, d, a.dim, o, inv);
                 }
             }
             if (some) {
@@ -846,7 +868,7 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             if (some) {
                 tmem_load16(o, lanes + (KEYS && g == 0 ? F::kSums2 : F::kSums) + d);
             }
-            store16<T>(to, to_part, place, d, a.dim, o, some ? by : 0.f);
+            store16<T>(to, nullptr, to_part, place, d, a.dim, o, some ? by : 0.f);
         }
     }
     if (steps > 0) {
@@ -934,7 +956,7 @@ bool mma_takes(const Args &a, int dtype)
 {
     const auto aligned = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
     return (dtype == HGC_FLOAT16 || dtype == HGC_BFLOAT16) && a.dim % 8 == 0 && a.n_q > 0 && a.n_k > 0 && rows_fit(a.q) && rows_fit(a.k) && rows_fit(a.v) &&
-           aligned(a.to) && aligned(a.to2) && aligned(a.grad);
+           aligned(a.to) && aligned(a.to2) && aligned(a.rest) && aligned(a.grad);
 }
 
 int mma_forward(const Args &a, int dtype, cudaStream_t stream)

@@ -286,6 +286,9 @@ template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b)
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
+template <typename T> __device__ __forceinline__ float2 unpack2(unsigned v);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
 
 }  // namespace mma
 }  // namespace hgc

@@ -425,8 +425,10 @@ int hgc_push_knn_grad_ordered(
  * Sums, weights and gradients are held in float32; in 16 bits, weights are rounded once to the type of the values
  * they meet.  scale > 0.  Limits: dim <= 128, n_heads <= 65535, 2^31 - 8193 rows.
  *
- * The gradient: d_grad_out [n_q, n_heads, dim] is that of d_out; d_out and d_lse are the forward pass's, as are all
- * other arguments.  d_grad_q may be NULL, and d_grad_k and d_grad_v both, where they are not wanted; gradients of
+ * The gradient: d_grad_out [n_q, n_heads, dim] is that of d_out; d_out, d_out_rest and d_lse are the forward pass's, as
+ * are all other arguments.  d_out_rest (like d_out, or NULL) is what the rounding of d_out to 16 bits left, rounded itself:
+ * without it, gradients of q and k are off by as much as the rounding of d_out moves its products with d_grad_out, which
+ * is most where few keys have the weight.  d_grad_q may be NULL, and d_grad_k and d_grad_v both, where they are not wanted; gradients of
  * masked keys, of rows behind the last event and of q and k in events with one key are zero.  Results do not change
  * from run to run.
  *
@@ -436,13 +438,13 @@ int hgc_push_knn_grad_ordered(
 size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype);
 int hgc_cross_attention(
         const void *d_q, const void *d_k, const void *d_v, const int *d_q_row_splits, const int *d_k_row_splits,
-        const unsigned char *d_key_mask, void *d_out, float *d_lse,
+        const unsigned char *d_key_mask, void *d_out, void *d_out_rest, float *d_lse,
         int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, const long long *strides, float scale, int dtype,
         void *workspace, size_t workspace_bytes, hgc_stream_t stream);
 size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype);
 int hgc_cross_attention_grad(
-        const void *d_grad_out, const void *d_q, const void *d_k, const void *d_v, const void *d_out, const float *d_lse,
-        const int *d_q_row_splits, const int *d_k_row_splits, const unsigned char *d_key_mask,
+        const void *d_grad_out, const void *d_q, const void *d_k, const void *d_v, const void *d_out, const void *d_out_rest,
+        const float *d_lse, const int *d_q_row_splits, const int *d_k_row_splits, const unsigned char *d_key_mask,
         void *d_grad_q, void *d_grad_k, void *d_grad_v,
         int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, const long long *strides, float scale, int dtype,
         void *workspace, size_t workspace_bytes, hgc_stream_t stream);

@@ -10,11 +10,11 @@ F = ctypes.c_float
 
 
 def _attend(L, n_q=4, n_k=6, n_rs=2, heads=2, kv=1, dim=8, strides=None, scale=1., dtype=0):
-    return L.hgc_cross_attention(*[NUL] * 8, n_q, n_k, n_rs, heads, kv, dim, strides, F(scale), dtype, NUL, 0, NUL)
+    return L.hgc_cross_attention(*[NUL] * 9, n_q, n_k, n_rs, heads, kv, dim, strides, F(scale), dtype, NUL, 0, NUL)
 
 
 def _attend_grad(L, n_q=4, n_k=6, n_rs=2, heads=2, kv=1, dim=8, strides=None, scale=1., dtype=0):
-    return L.hgc_cross_attention_grad(*[NUL] * 12, n_q, n_k, n_rs, heads, kv, dim, strides, F(scale), dtype, NUL, 0, NUL)
+    return L.hgc_cross_attention_grad(*[NUL] * 13, n_q, n_k, n_rs, heads, kv, dim, strides, F(scale), dtype, NUL, 0, NUL)
 
 
 @pytest.mark.parametrize("call", [_attend, _attend_grad])

@@ -261,6 +261,20 @@ def test_many_queries_over_few_keys(cuda, dtype, dim):
     check(q, k, v, grad, nq, nk)
 
 
+@pytest.mark.parametrize("dim,masked", [(32, True), (64, False), (128, True), (128, False)])
+def test_tiles_with_and_without_a_second_half(cuda, dim, masked):
+    """Events of 12 to 236 queries, three heads to a key head, on 195 to 3714 keys: tiles whose second half has rows follow ones whose has
+    none, with any number of steps between; and a few queries on keys of one step and of many.  The same results every time."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    for sizes in (lambda i: (12 + i * 97 % 225, 195 + i * 1013 % 3520), lambda i: (i % 4, [40, 1, 6000, 300, 0, 129, 9000, 64][i % 8])):
+        nq, nk = zip(*[sizes(i) for i in range(44)])
+        q, k, v, grad = inputs(nq, nk, 6, 2, dim, "bfloat", cuda, seed=24)
+        mask = torch.rand(k.shape[0], generator=torch.Generator(device=cuda).manual_seed(2), device=cuda) < 0.7 if masked else None
+        out = check(q, k, v, grad, nq, nk, mask=mask, both=False)
+        for _ in range(20):
+            assert torch.equal(CrossAttention(q, k, v, splits(nq, cuda), splits(nk, cuda), key_mask=mask), out)
+
+
 def test_gradients_are_those_of_differences(cuda):
     """Central differences of a scalar of the result, in float32."""
     from hgcalml_b200.cross_attention_op import CrossAttention
@@ -286,7 +300,9 @@ def test_what_is_not_needed_is_not_computed(cuda):
     q, k, v, grad = inputs(nq, nk, 2, 2, 64, "bfloat", cuda, seed=41)
     rs = splits(nq, cuda), splits(nk, cuda)
     out, lse = CrossAttention(q, k, v, *rs, with_lse=True)
-    dq, dk, dv = CrossAttentionGrad(grad, q, k, v, out, lse, *rs)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(CrossAttention(*leaves, *rs), leaves, grad)
+    assert torch.equal(CrossAttentionGrad(grad, q, k, v, out, lse, *rs)[2], dv)
     assert CrossAttentionGrad(grad, q, k, v, out, lse, *rs, need_keys=False)[1:] == (None, None)
     ql = q.clone().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(CrossAttention(ql, k, v, *rs), ql, grad)[0], dq)
@@ -297,7 +313,7 @@ def test_what_is_not_needed_is_not_computed(cuda):
     # the gradient of a sum comes as one value for all rows
     kl = k.clone().requires_grad_(True)
     g1, = torch.autograd.grad(CrossAttention(q, kl, v, *rs).sum(), kl)
-    assert torch.equal(g1, CrossAttentionGrad(torch.ones_like(out), q, k, v, out, lse, *rs)[1])
+    assert torch.equal(g1, torch.autograd.grad(CrossAttention(*leaves, *rs), leaves, torch.ones_like(out))[1])
     with pytest.raises(RuntimeError):  # once differentiable
         g, = torch.autograd.grad(CrossAttention(q, kl, v, *rs).float().square().sum(), kl, create_graph=True)
         g.sum().backward()
@@ -388,11 +404,11 @@ def test_splits_that_make_no_sense_are_reported(cuda):
         d = [torch.zeros_like(x) for x in (q, k, v)]
         ws = C.workspace(C.lib.hgc_cross_attention_workspace_bytes(100, 200, 3, 2, 2, 64, 2), cuda)
         tail = (100, 200, 3, 2, 2, 64, None, ctypes.c_float(0.125), 2)
-        rc = C.lib.hgc_cross_attention(C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(t[0]), C.ptr(t[1]), None, C.ptr(out), C.ptr(lse), *tail,
+        rc = C.lib.hgc_cross_attention(C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(t[0]), C.ptr(t[1]), None, C.ptr(out), None, C.ptr(lse), *tail,
                                        C.ptr(ws), ws.numel(), C.stream_of(q))
         assert rc == 0 and C.read_status(ws, raise_on_flag=False) == bad
         ws = C.workspace(C.lib.hgc_cross_attention_grad_workspace_bytes(100, 200, 3, 2, 2, 64, 2), cuda)
-        rc = C.lib.hgc_cross_attention_grad(C.ptr(grad), C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(out), C.ptr(lse), C.ptr(t[0]), C.ptr(t[1]),
+        rc = C.lib.hgc_cross_attention_grad(C.ptr(grad), C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(out), None, C.ptr(lse), C.ptr(t[0]), C.ptr(t[1]),
                                             None, *[C.ptr(x) for x in d], *tail, C.ptr(ws), ws.numel(), C.stream_of(q))
         assert rc == 0 and C.read_status(ws, raise_on_flag=False) == bad
 
