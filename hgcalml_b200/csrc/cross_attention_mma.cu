@@ -76,15 +76,10 @@ __device__ __forceinline__ void store16(void *to, void *rest, float *part, const
             if (rows.store && d + 4 * i < dim) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
     } else {
 #pragma unroll 1
-        for (void *next = to; next != nullptr; next = next == to ? rest : nullptr) {
+        for (void *next = to;; next = rest) {
             unsigned h[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                h[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-                const float2 there = unpack2<T>(h[i]);
-                x[2 * i] -= there.x;
-                x[2 * i + 1] -= there.y;
-            }
+            for (int i = 0; i < 8; i++) h[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
             const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
             // first the even lanes' rows: they keep their first 16 bytes and give away the second; then the odd ones'
             const bool odd = lane_id() & 1;
@@ -95,6 +90,13 @@ __device__ __forceinline__ void store16(void *to, void *rest, float *part, const
             if (d + (odd ? 8 : 0) < dim) {
                 if (odd ? rows.store_other : rows.store) *reinterpret_cast<uint4 *>(base + (odd ? rows.other : rows.at)) = odd ? got : a;
                 if (odd ? rows.store : rows.store_other) *reinterpret_cast<uint4 *>(base + (odd ? rows.at : rows.other)) = odd ? b : got;
+            }
+            if (rest == nullptr || next == rest) break;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float2 there = unpack2<T>(h[i]);
+                x[2 * i] -= there.x;
+                x[2 * i + 1] -= there.y;
             }
         }
     }
