@@ -541,7 +541,7 @@ grad_queries_kernel(const __grid_constant__ Args a)
         const int r = row0 + (lane_id() >> 2) + 8 * i;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
         const float2 stat = r < n_rows ? a.stats[row] : make_float2(INFINITY, 0.f);
-        lse[i] = stat.x;
+        lse[i] = stat.x + a.shift;
         delta[i] = stat.y;
     }
     for (int step = part.x; step < part.y; step++) {
@@ -610,8 +610,11 @@ grad_keys_kernel(const __grid_constant__ Args a)
             const int n = min(tokens, queries.y - q0) * a.pack;
             load_queries<T, DP>(s_q + at * kRows * P, a.q, piece_q, head0, q0, n, a.pack, a.dim);
             load_queries<T, DP>(s_g + at * kRows * P, grad, piece_g, head0, q0, n, a.pack, a.dim);
-            if (t < kRows)
-                s_stats_all[at][t] = t < n ? a.stats[(long long)(q0 + t / a.pack) * a.heads + head0 + t % a.pack] : make_float2(INFINITY, 0.f);
+            if (t < kRows) {
+                float2 stat = t < n ? a.stats[(long long)(q0 + t / a.pack) * a.heads + head0 + t % a.pack] : make_float2(INFINITY, 0.f);
+                stat.x += a.shift;
+                s_stats_all[at][t] = stat;
+            }
         }
         end_of_copies();
     };
@@ -709,6 +712,7 @@ int split_count(long long blocks, long long mean_steps, int per_sm, int least)
 struct Plan {
     int group, pack, splits, splits_mma, parts_mma, alternate, pack_few, rows_few, splits_few, splits_q, splits_q_mma, splits_k, splits_k_mma;
     long long tiles_q, tiles_k;
+    bool close, close_q, close_k;
 };
 
 bool sizes_ok(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
@@ -743,6 +747,16 @@ Plan plan_of(int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
     p.splits_mma = split_count(filled(n_q, p.alternate ? mma_tokens : 2 * mma_tokens) * (heads / p.pack), steps_mma, 6, 4);
     if (p.alternate && p.splits_mma > kMaxParts / 2) p.splits_mma = kMaxParts / 2;
     p.parts_mma = p.splits_mma * (p.alternate ? 2 : 1);
+    // Where 16-bit types are better off with the products of this file: weights and their gradients are not rounded to 16 bits there.
+    // In short calls, whose time is that of their launches, it costs nothing (32 events of 30 queries on 30 keys, forward and backward:
+    // 28 and 70 us here, 32 and 68 there).  Of a few keys, gradients are differences of products that are much larger: off by 1.5 to 1.6
+    // times their own rounding there, 1.2 here (8 events of 8192 queries on 8 keys of 8, 64 and 128 columns: 146, 427 and 805 us here,
+    // 144, 199 and 263 there).  So is the gradient of narrow queries, whose keys have a large part in common, on any number
+    // of keys: 1.5 to 1.6 for 8 and 16 columns.
+    const long long mean_k = n_k / some, mean_q = n_q / some;
+    p.close = mean_k <= kRows && mean_q * p.pack <= kRows && filled(n_q, tokens) * (heads / p.pack) <= 2 * sm_count();
+    p.close_k = p.close || mean_k <= 16;
+    p.close_q = p.close_k || dim <= 16;
     // where the queries of a mean event fit a block that holds them in registers
     p.pack_few = few_pack(p.group);
     p.rows_few = few_rows(n_q, events, p.pack_few);
@@ -835,7 +849,7 @@ template <typename T, int DP> int run_grad_keys(const Args &a, const Plan &p, cu
 
 template <typename T> int forward_of(Args a, const Plan &p, int dtype, cudaStream_t stream)
 {
-    const bool few = few_takes(a, p.rows_few, dtype), mma = !few && mma_takes(a, dtype);
+    const bool few = few_takes(a, p.rows_few, dtype), mma = !few && !p.close && mma_takes(a, dtype);
     if (few) a.pack = p.pack_few;
     a.splits = few ? p.splits_few : mma ? p.splits_mma : p.splits;
     a.alternate = mma ? p.alternate : 0;
@@ -858,7 +872,8 @@ template <typename T>
 int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void *dk, void *dv, int dtype, cudaStream_t stream)
 {
     const auto aligned = [](const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
-    const bool mma = mma_takes(a, dtype) && aligned(dq) && aligned(dk) && aligned(dv), bounded = mma && dtype == HGC_FLOAT16;
+    const bool takes = mma_takes(a, dtype) && aligned(dq) && aligned(dk) && aligned(dv), mma_q = takes && !p.close_q, mma_k = takes && !p.close_k,
+               bounded = (mma_q || mma_k) && dtype == HGC_FLOAT16;
     // whole 16-byte vectors of rows where they are that
     constexpr int V = 16 / sizeof(T);
     int lanes_log2 = -1;
@@ -871,18 +886,18 @@ int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void 
     HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + n_rows + n_values, kThreads, 0, stream, a, b.stats, b.visible,
                             bounded ? b.bounds : nullptr, bounded ? kHalfShift : 0.f, n_count, n_rows, lanes_log2));
     HGC_LAUNCH_CHECK();
-    a.stats = b.stats; a.visible = b.visible; a.bounds = b.bounds;
+    a.stats = b.stats; a.visible = b.visible; a.bounds = b.bounds; a.shift = bounded ? kHalfShift : 0.f;
     if (dq != nullptr && a.n_q > 0) {
-        a.to = dq; a.to2 = nullptr; a.part = b.part_q; a.part2 = nullptr; a.splits = mma ? p.splits_q_mma : p.splits_q;
-        if (const int rc = mma ? mma_grad_queries(a, dtype, stream)
+        a.to = dq; a.to2 = nullptr; a.part = b.part_q; a.part2 = nullptr; a.splits = mma_q ? p.splits_q_mma : p.splits_q;
+        if (const int rc = mma_q ? mma_grad_queries(a, dtype, stream)
                          : a.dim <= 32 ? run_grad_queries<T, 32>(a, p, stream)
                          : a.dim <= 64 ? run_grad_queries<T, 64>(a, p, stream) : run_grad_queries<T, 128>(a, p, stream))
             return rc;
         if (const int rc = join_gradient<T>(a, (long long)a.n_q * a.heads * a.dim, stream)) return rc;
     }
     if (dk != nullptr && a.n_k > 0) {
-        a.to = dk; a.to2 = dv; a.part = b.part_k; a.part2 = b.part_v; a.splits = mma ? p.splits_k_mma : p.splits_k;
-        if (const int rc = mma ? mma_grad_keys(a, dtype, stream)
+        a.to = dk; a.to2 = dv; a.part = b.part_k; a.part2 = b.part_v; a.splits = mma_k ? p.splits_k_mma : p.splits_k;
+        if (const int rc = mma_k ? mma_grad_keys(a, dtype, stream)
                          : a.dim <= 32 ? run_grad_keys<T, 32>(a, p, stream)
                          : a.dim <= 64 ? run_grad_keys<T, 64>(a, p, stream) : run_grad_keys<T, 128>(a, p, stream))
             return rc;

@@ -41,7 +41,7 @@ struct Args {
     int *counter;                  // of the tiles that the blocks of the forward pass take
     unsigned *status;
     int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits, alternate;  // alternate: of the forward pass on the tensor cores, two parts to each of the splits
-    float scale;
+    float scale, shift;            // shift: what `stats` is less by than the logarithms
 };
 
 // What a kernel before this one may have written is read after pdl_begin(), by a load that cannot move ahead of it as one of
