@@ -56,8 +56,8 @@ template <> __device__ __forceinline__ float rounded<float>(float v) { return v;
 template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V columns at one address; a whole 16-byte vector, or one column
-template <typename T, int V> struct Vec { alignas(V == 1 ? sizeof(T) : 16) T v[V]; };
+// V columns at one address; a whole 16-byte vector, or two columns, or one
+template <typename T, int V> struct Vec { alignas(V * sizeof(T)) T v[V]; };
 
 // two columns at a time where they come in 32 bits
 __device__ __forceinline__ float2 two(unsigned v, __nv_bfloat16) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
@@ -420,8 +420,6 @@ join_weights_kernel(const __grid_constant__ Join j, int dim)
 }
 
 // -------------------------------------------------------------------------------------------------------------- host
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 int log2_up(int n)
 {
     int b = 0;
@@ -463,13 +461,18 @@ template <typename T, bool BACKWARD>
 int run_type(Call &c, cudaStream_t stream)
 {
     constexpr int V = 16 / sizeof(T);
-    bool whole = c.dim % V == 0;
-    for (const Set &s : c.set)
-        if (s.n > 0)
-            whole = whole && aligned16(s.x) && aligned16(s.y) && s.row % V == 0 && s.head % V == 0 && (!BACKWARD || aligned16(s.grad));
+    const auto fits = [&](int v) {
+        bool all = c.dim % v == 0;
+        const auto aligned = [&](const void *p) { return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0; };
+        for (const Set &s : c.set)
+            if (s.n > 0) all = all && aligned(s.x) && aligned(s.y) && s.row % v == 0 && s.head % v == 0 && (!BACKWARD || aligned(s.grad));
+        return all;
+    };
+    const bool whole = fits(V), twos = !whole && fits(2);
     // a vector of either half to a lane, where the lanes of a row are then a power of two and all columns turn together
     const bool both = whole && !c.interleaved && c.axes == 1 && c.rotary == c.dim && c.dim % (2 * V) == 0 && (c.dim & (c.dim - 1)) == 0;
-    c.lanes_log2 = both ? log2_up(c.dim / V) - 1 : whole ? log2_up(c.dim / V) : 5;
+    c.lanes_log2 = both ? log2_up(c.dim / V) - 1 : log2_up(c.dim / (whole ? V : twos ? 2 : 1));
+    if (c.lanes_log2 > 5) c.lanes_log2 = 5;
     const int subs = kThreads >> c.lanes_log2;
     for (Set &s : c.set) {
         // about four rows for every group of lanes, which share the angles; fewer where that leaves multiprocessors without a block
@@ -478,7 +481,16 @@ int run_type(Call &c, cudaStream_t stream)
         const int tokens = s.heads > 0 ? each * subs / s.heads : 1;
         s.tokens = tokens < 1 ? 1 : tokens > kMaxTokens ? kMaxTokens : tokens;
     }
-    if (!whole) return run<T, 1, kMaxDim / 32, kAnywhere, BACKWARD>(c, stream);
+    // Two columns at a time, or one, where rows are not whole vectors, with as many per lane as the width needs (288k rows of 4 heads of 22 in
+    // bf16, forward and backward, always four single columns a lane: 1120 us, so 560).
+    if (twos) {
+        if (c.dim > 64) return run<T, 2, 2, kAnywhere, BACKWARD>(c, stream);
+        if (c.interleaved || c.pairs == 1) return run<T, 2, 1, kNeighbours, BACKWARD>(c, stream);
+        return c.pairs % 2 == 0 ? run<T, 2, 1, kHalves, BACKWARD>(c, stream) : run<T, 2, 1, kAnywhere, BACKWARD>(c, stream);
+    }
+    if (!whole)
+        return c.dim <= 32 ? run<T, 1, 1, kAnywhere, BACKWARD>(c, stream)
+             : c.dim <= 64 ? run<T, 1, 2, kAnywhere, BACKWARD>(c, stream) : run<T, 1, 4, kAnywhere, BACKWARD>(c, stream);
     if (both) return run<T, V, 2, kBothHalves, BACKWARD>(c, stream);
     if (c.interleaved) return run<T, V, 1, kNeighbours, BACKWARD>(c, stream);
     if (c.rotary == 0 || c.pairs % V == 0) return run<T, V, 1, kHalves, BACKWARD>(c, stream);

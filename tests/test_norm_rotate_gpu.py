@@ -78,7 +78,9 @@ def inputs(n, heads, dim, dtype, axes, kind, dev, seed):
 @pytest.mark.parametrize("dim,rotary,axes", [(64, 64, 0), (32, 32, 4), (22, 12, 3), (128, 128, 1), (128, 64, 2), (8, 8, 1), (2, 2, 0), (96, 32, 2),
                                              (72, 64, 0), (1, 0, 0), (127, 126, 3), (40, 24, 1), (16, 16, 1)] + [
                              # axes of few columns, which end inside a 16-byte vector
-                             (16, 4, 1), (32, 12, 3), (8, 6, 3), (64, 20, 5), (24, 8, 4), (16, 6, 1), (128, 8, 1)])
+                             (16, 4, 1), (32, 12, 3), (8, 6, 3), (64, 20, 5), (24, 8, 4), (16, 6, 1), (128, 8, 1),
+                             # two columns at a time
+                             (124, 100, 1), (50, 46, 0), (46, 40, 2), (60, 12, 6), (64, 60, 3), (66, 66, 0), (33, 32, 2), (61, 60, 5)])
 def test_forward_and_backward(cuda, dtype, interleaved, dim, rotary, axes):
     from hgcalml_b200.norm_rotate_op import NormRotate
     kinds = [torch.float32, torch.int32, torch.int64]
