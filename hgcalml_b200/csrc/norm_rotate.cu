@@ -5,7 +5,8 @@
 //   y_a = n_a cos t - n_b sin t,  y_b = n_b cos t + n_a sin t;  columns behind the rotary ones stay as they are
 //   backward: g = dy turned back,  dx = r (g w - x r^2 mean(g w x)),  dw = sum over rows and heads of g x r
 //
-// Bound by memory: a row is read once and written once.  A row belongs to as many lanes as it has 16-byte vectors.  The angle of
+// Bound by memory: a row is read once and written once.  A row belongs to as many lanes as it has 16-byte vectors (or pairs of columns,
+// or columns, where it is not whole vectors).  The angle of
 // a far position needs more digits than float32 has: its turns are counted in double and only their fraction is kept, once for all
 // heads of a row (position * frequency in float32 is off by 0.06 rad at a million).
 #include <cuda_bf16.h>
