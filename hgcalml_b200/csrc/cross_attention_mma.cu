@@ -407,14 +407,13 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             ok = wait_warp<true>(item_full + 8 * item.at, item.turn, gave_up, a.status);
             const Item it = s_item[item.at];
             if (!ok || it.steps < 0) break;
-            const int groups = it.end - it.begin > tokens ? 2 : 1, begin = it.begin + (alternate ? 0 : g * tokens), slot = item.at;
+            const int groups = it.end - it.begin > tokens ? 2 : 1, begin = it.begin + (alternate ? 0 : g * tokens);
             // The second half may have no steps.  It must not go on all the same: a wait tells a barrier's phases apart by their parity only,
             // and would take the phase before the last for the next one.  It goes on when the first half has seen all scores of the item.
             if (g == 1 && it.steps > 0 && groups == 1 && (!alternate || it.steps == 1))
-                ok = wait_warp<true>(item_done + 8 * slot, item.turn, gave_up, a.status);
+                ok = wait_warp<true>(item_done + 8 * item.at, item.turn, gave_up, a.status);
             __syncwarp();
-            if (g == 1 && lane == 0) arrive(item_empty + 8 * slot);
-            item.go(1);
+            if (g == 1 && lane == 0) arrive(item_empty + 8 * item.at);
             const int n_rows = min(tokens, it.end - begin) * a.pack;
             const bool some = it.steps > (alternate ? g : 0);  // steps for this half
             int count = 0;
@@ -514,10 +513,11 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             if (g == 0) {  // in this order: the next item in this slot has the next phase
                 __syncwarp();
                 if (lane == 0) {
-                    arrive(item_done + 8 * slot);
-                    arrive(item_empty + 8 * slot);
+                    arrive(item_done + 8 * item.at);
+                    arrive(item_empty + 8 * item.at);
                 }
             }
+            item.go(1);
             if (g >= groups && !alternate) continue;
             const bool done = some && ok && wait_warp<true>(o_full + 8 * g, o_turn ^ 1, gave_up, a.status);
             if (done) after_sync();
