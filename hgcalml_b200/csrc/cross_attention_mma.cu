@@ -141,7 +141,9 @@ template <int N> struct Ring {
     }
 };
 
-template <typename T, int CHUNKS>
+// REST: what the rounding of the results leaves is kept too; with that in every call, 1000 queries on 400k masked
+// keys, 8 heads of 32, took 685 us, not 655.
+template <typename T, int CHUNKS, bool REST>
 __global__ void __launch_bounds__(Forward<CHUNKS>::kThreads, 1)
 forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps, int n_tiles, int n_items, int alternate)
 {
@@ -540,7 +542,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     if (done) {
                         tmem_load16(o, out + d);
                     }
-                    store16<T>(a.to, a.rest, to_part, to, d, a.dim, o, inv);
+                    store16<T>(a.to, REST ? a.rest : nullptr, to_part, to, d, a.dim, o, inv);
                 }
             }
             if (some) {
@@ -949,7 +951,9 @@ template <typename T, int CHUNKS> int forward_mma(const Args &a, const Maps &map
     if (items > kMaxCount) return HGC_ERR_UNSUPPORTED;
     const int blocks = items < sm_count() ? (int)items : sm_count();
     if (items > blocks) HGC_CUDA_TRY(cudaMemsetAsync(a.counter, 0, sizeof(int), stream));
-    return launch(forward_mma_kernel<T, CHUNKS>, blocks, Forward<CHUNKS>::kThreads, Forward<CHUNKS>::kSmem, stream, a, maps, (int)tiles, (int)items, a.alternate);
+    const bool rest = a.rest != nullptr && a.splits == 1 && !a.alternate;  // parts are rounded where they are joined
+    return launch(rest ? forward_mma_kernel<T, CHUNKS, true> : forward_mma_kernel<T, CHUNKS, false>, blocks, Forward<CHUNKS>::kThreads,
+                  Forward<CHUNKS>::kSmem, stream, a, maps, (int)tiles, (int)items, a.alternate);
 }
 
 }  // namespace
