@@ -249,6 +249,7 @@ forward_kernel(const __grid_constant__ Args a)
     const int2 keys = rows_of(a.rs_k, a.n_k, a.n_events, tile.event);
     const int2 part = part_of(max(0, (keys.y - keys.x + kRows - 1) / kRows), blockIdx.z, a.splits);
     load_queries<T, DP>(s_q, a.q, piece_of<T>(a.q, a.dim), head0, tile.begin, n_rows, a.pack, a.dim);
+    end_of_copies();  // a group of their own: with no step after it, they are waited for at the end all the same
     const int piece_k = piece_of<T>(a.k, a.dim), piece_v = piece_of<T>(a.v, a.dim);
     const auto load = [&](int step) {  // with a barrier inside
         const int at = step % S, k0 = keys.x + step * kRows;
@@ -522,6 +523,7 @@ grad_queries_kernel(const __grid_constant__ Args a)
     const Strided grad{a.grad, (long long)a.heads * a.dim, a.dim};
     load_queries<T, DP>(s_q, a.q, piece_of<T>(a.q, a.dim), head0, tile.begin, n_rows, a.pack, a.dim);
     load_queries<T, DP>(s_g, grad, piece_of<T>(grad, a.dim), head0, tile.begin, n_rows, a.pack, a.dim);
+    end_of_copies();
     const int piece_k = piece_of<T>(a.k, a.dim), piece_v = piece_of<T>(a.v, a.dim);
     const auto load = [&](int step) {  // with a barrier inside
         const int at = step % S, k0 = keys.x + step * kRows;
@@ -603,6 +605,7 @@ grad_keys_kernel(const __grid_constant__ Args a)
     __syncthreads();
     load_keys<T, DP>(s_k, a.k, piece_of<T>(a.k, a.dim), kv, tile.begin, a.dim, s_seen);
     load_keys<T, DP>(s_v, a.v, piece_of<T>(a.v, a.dim), kv, tile.begin, a.dim, s_seen);
+    end_of_copies();
     const int piece_q = piece_of<T>(a.q, a.dim), piece_g = piece_of<T>(grad, a.dim);
     const auto load = [&](int step) {
         if (step < part.y * packs) {
