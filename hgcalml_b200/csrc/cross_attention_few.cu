@@ -219,7 +219,7 @@ few_kernel(const __grid_constant__ Args a, int lanes_log2)
             total += s_sum[w * R + r] * f;
             o = fmaf(s_mem[(w * R + r) * a.dim + d], f, o);
         }
-        const bool none = most == -INFINITY;
+        const bool none = most == -INFINITY && total == 0.f;  // a maximum passes over what is no number, the sum does not
         o = none ? 0.f : o / total;
         const long long row = (long long)(tile.begin + r / a.pack) * a.heads + head0 + r % a.pack;
         if (a.splits > 1) a.part[(blockIdx.z * all_rows + row) * a.dim + d] = o;

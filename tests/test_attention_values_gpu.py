@@ -29,3 +29,36 @@ def test_queries_that_see_no_key_hold_anything(cuda, dtype, dim):
         assert (out[blind] == 0).all() and (lse[blind] == -float("inf")).all()
         assert_near(out.detach(), want["out"], "out")
     assert (torch.autograd.grad(out, leaves, grad)[0][blind] == 0).all()
+
+
+# one query, a few, as many as fill half a tile with keys for both halves, several tiles; widths without whole vectors; short calls
+CALLS = [([1, 1], [700, 900], 4, 2, 64), ([1, 1], [700, 900], 2, 2, 128), ([3, 2], [9000, 400], 4, 2, 64), ([100, 90], [6000, 500], 2, 2, 64),
+         ([100, 90], [6000, 500], 4, 1, 128), ([700, 300], [900, 400], 2, 1, 64), ([700, 300], [900, 400], 2, 1, 96), ([200, 90], [300, 400], 2, 1, 22),
+         ([20, 30], [30, 40], 2, 1, 32), ([1, 1], [300, 20], 2, 1, 7)]
+
+
+@pytest.mark.parametrize("call,dtype", [(c, t) for c in range(len(CALLS)) for t in ("float", "half", "bfloat") if c < 2 or t == "float"])
+@pytest.mark.parametrize("where", ["query", "keys", "value"])
+def test_what_is_no_number_stays_none(cuda, call, dtype, where):
+    """A NaN in a query, in all keys of a part, or in a value that is seen gives NaN in every result that it is a term of, and changes
+    no other."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk, heads, kv_heads, dim = CALLS[call]
+    q, k, v, _ = inputs(nq, nk, heads, kv_heads, dim, dtype, cuda, seed=81 + call)
+    rs = splits(nq, cuda), splits(nk, cuda)
+    clean, clean_lse = CrossAttention(q, k, v, *rs, with_lse=True)
+    group, nan = heads // kv_heads, float("nan")
+    gone = torch.zeros(clean.shape, dtype=torch.bool, device=cuda)
+    if where == "query":
+        q[nq[0] - 1, heads - 1, dim // 2] = nan
+        gone[nq[0] - 1, heads - 1] = True
+    elif where == "value":
+        v[nk[0] // 2, 0, dim - 1] = nan
+        gone[:nq[0], :group, dim - 1] = True
+    else:
+        k[nk[0] // 2:nk[0], 0, 0] = nan
+        gone[:nq[0], :group] = True
+    out, lse = CrossAttention(q, k, v, *rs, with_lse=True)
+    assert torch.equal(out.isnan(), gone) and torch.equal(out[~gone], clean[~gone])
+    rows = gone.all(-1)
+    assert torch.equal(lse.isnan(), rows) and torch.equal(lse[~rows], clean_lse[~rows])
