@@ -121,7 +121,7 @@ template <int CHUNKS> struct Forward {
     static constexpr int kBarriers = 3 + 3 * kStages + 3 * kBuffers + 2 * kQueries + 3 * kItems + 4 + 8;
     static constexpr int kBias = 512, kMaxAt = kBias + kStages * kKeys * 4, kItemAt = kMaxAt + 2 * 3 * 2 * kMmaRows * 4,
                          kSmem = kTiles + kItemAt + kItems * 48;  // behind the tiles
-    static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 <= kBias && kSmem <= 232448, "room");
+    static_assert(kOut + 128 * CHUNKS <= kColumns && 8 * kBarriers + 8 + 4 * kStages <= kBias && kSmem <= 232448, "room");
 };
 
 // What the warps of a block have to know of a tile; steps < 0: there is none any more.
@@ -163,6 +163,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                    item_done = o_empty + 16, meet = item_done + 8 * F::kItems;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(s_raw + F::kTiles + 8 * F::kBarriers);
     volatile int *gave_up = reinterpret_cast<volatile int *>(s_tmem + 1);
+    volatile int *s_any = gave_up + 1;  // [kStages], whether a key of a step that is not whole is seen
     float *s_bias = reinterpret_cast<float *>(s_raw + F::kTiles + F::kBias);  // [kStages][kKeys], 0 or minus infinity
     Item *s_item = reinterpret_cast<Item *>(s_raw + F::kTiles + F::kItemAt);
     if (t == 0) {
@@ -377,8 +378,13 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     clear_unseen<W>(s_v + kv.at * F::kTileBytes, CHUNKS, seen);
                     writes_before_products();
                 }
+                unsigned any = 0;
 #pragma unroll
-                for (int w = 0; w < W; w++) s_bias[kv.at * N + 32 * w + lane] = (seen[w] >> lane) & 1u ? 0.f : -INFINITY;
+                for (int w = 0; w < W; w++) {
+                    s_bias[kv.at * N + 32 * w + lane] = (seen[w] >> lane) & 1u ? 0.f : -INFINITY;
+                    any |= seen[w];
+                }
+                if (lane == 0) s_any[kv.at] = any != 0;
                 __syncwarp();
                 if (lane == 0) arrive(clean + 8 * kv.at);
             }
@@ -421,6 +427,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             int count = 0;
             const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;  // idle: none of the warp's rows counts
             float top = -INFINITY, sum = 0.f;
+            bool any = false;  // whether a key is seen
             if (groups == 2 && g == 1 && it.steps > 0) buffer.go(1);  // this half's place among the two
             for (int j = 0; j < it.steps; j++, kv.go(1)) {
                 const bool whole_step = j < it.dirty;
@@ -433,6 +440,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                 const unsigned rows = lanes + N * buffer.at + half * (N / 2);
                 ok = wait_warp<true>(s_full + 8 * buffer.at, buffer.turn, gave_up, a.status) && ok;
                 if (!whole_step) ok = wait_warp<true>(clean + 8 * kv.at, clean_turn, gave_up, a.status) && ok;
+                any = any || whole_step || s_any[kv.at] != 0;
                 // every phase of the sums' barrier is waited for: here, where they are scaled, else when this step's weights are done
                 bool summed = count == 0;
                 if (!idle) {
@@ -525,7 +533,9 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             if (done) after_sync();
             const long long row = (long long)(begin + r / a.pack) * a.heads + it.head0 + r % a.pack;
             if (some && !idle) sum += exchange(maxima + 2 * 2 * kMmaRows, sum);
-            const bool none = top == -INFINITY;  // no key was seen
+            // Scores of a query of NaN or infinity are no numbers where keys are cleared either, so that its sums say nothing; and those of
+            // keys that are seen must not be lost for the maximum, which passes over them.
+            const bool none = !any || (top == -INFINITY && sum == sum);
             const float inv = none ? 0.f : 1.f / sum;
             const long long all_rows = (long long)a.n_q * a.heads;
             const bool parts = a.splits > 1 || alternate;
@@ -541,6 +551,9 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     unsigned o[16] = {};
                     if (done) {
                         tmem_load16(o, out + d);
+                        if (none)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] = 0;
                     }
                     store16<T>(a.to, REST ? a.rest : nullptr, to_part, to, d, a.dim, o, inv);
                 }
