@@ -252,7 +252,8 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 // 2^x of two floats of at most 127 without the special function unit: 2^n from the integer n next to x, put into the exponent,
 // times a polynomial of degree three in x - n that is off by 1.0e-04 at most (root mean square 6.4e-05), less than a quarter of half
 // precision's largest rounding.  Its coefficients give the least maximal relative error on [-1/2, 1/2] that goes with 2^0 = 1.
-// Below 2^-126 it stays there; what is no number gives none, or an infinity.
+// Below 2^-126 it stays there; what is no number gives none (2^n is a factor, and not added to the exponent: that made a finite
+// number of it).
 __device__ __forceinline__ float at_least(float a, float b)
 {
     float r;
@@ -268,9 +269,8 @@ __device__ __forceinline__ float2 exp2_arithmetic(float2 v)
     pair y = fma2(f, pair_of(0.0550091006f, 0.0550091006f), pair_of(0.242210984f, 0.242210984f));
     y = fma2(y, f, pair_of(0.693282902f, 0.693282902f));
     y = fma2(y, f, pair_of(1.f, 1.f));
-    const float2 p = parts(y), n = parts(t);
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+    const float2 n = parts(t);
+    return parts(mul2(y, pair_of(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u))));
 }
 // two floats rounded to 16 bits, the first in the lower half
 template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);

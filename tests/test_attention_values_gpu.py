@@ -63,3 +63,21 @@ def test_what_is_no_number_stays_none(cuda, call, dtype, where):
     assert torch.equal(out.isnan(), gone) and torch.equal(out[~gone], clean[~gone])
     rows = gone.all(-1)
     assert torch.equal(lse.isnan(), rows) and torch.equal(lse[~rows], clean_lse[~rows])
+
+
+@pytest.mark.parametrize("dtype", ["half", "bfloat"])
+@pytest.mark.parametrize("call", [2, 3, 4, 5, 6])
+def test_a_key_that_is_no_number_is_one_in_every_column(cuda, dtype, call):
+    """Some of the weights' powers of two are worked out on the multipliers: NaN in any of eight neighbouring keys gives NaN."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk, heads, kv_heads, dim = CALLS[call]
+    q, k, v, _ = inputs(nq, nk, heads, kv_heads, dim, dtype, cuda, seed=95)
+    rs = splits(nq, cuda), splits(nk, cuda)
+    clean = CrossAttention(q, k, v, *rs)
+    for at in range(nk[0] // 2, nk[0] // 2 + 8):
+        bad = k.clone()
+        bad[at, 0, 0] = float("nan")
+        out, lse = CrossAttention(q, bad, v, *rs, with_lse=True)
+        group = heads // kv_heads
+        assert out[:nq[0], :group].isnan().all() and lse[:nq[0], :group].isnan().all()
+        assert torch.equal(out[nq[0]:], clean[nq[0]:]) and torch.equal(out[:, group:], clean[:, group:])
