@@ -471,16 +471,17 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                     next = fmaxf(next, exchange(maxima + (count & 1) * 2 * kMmaRows, next));
                     // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing
-                    // in either type.  Rows that do not count have no say: what stands there may differ from run to run.
+                    // in either type.  The others of the warp stay as they are then, so that no result depends on which rows share a warp;
+                    // and rows that do not count have no say: what stands there may differ from run to run.
                     const bool grown = store && (next - top) * c > 8.f;
+                    const float before = top;
+                    if (count == 0 || grown) top = next;
                     if (count == 0) {
-                        top = next;
                     } else if (__any_sync(0xffffffffu, grown)) {
                         ok = wait_warp<true>(o_full + 8 * g, o_turn ^ 1, gave_up, a.status) && ok;
                         summed = true;
                         after_sync();
-                        const float shrink = exp2_fast((top - (next == -INFINITY ? 0.f : next)) * c);
-                        top = next;
+                        const float shrink = exp2_fast((before - (top == -INFINITY ? 0.f : top)) * c);
                         sum *= shrink;
                         for (int d = 16 * half; d < a.dim; d += 32) {
                             unsigned o[16];

@@ -81,3 +81,18 @@ def test_a_key_that_is_no_number_is_one_in_every_column(cuda, dtype, call):
         group = heads // kv_heads
         assert out[:nq[0], :group].isnan().all() and lse[:nq[0], :group].isnan().all()
         assert torch.equal(out[nq[0]:], clean[nq[0]:]) and torch.equal(out[:, group:], clean[:, group:])
+
+
+@pytest.mark.parametrize("dtype", ["half", "bfloat", "float"])
+@pytest.mark.parametrize("call", range(len(CALLS)))
+def test_a_row_does_not_depend_on_its_neighbours(cuda, dtype, call):
+    """Other queries of the event, some with much larger scores, change no bit of a query's result."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk, heads, kv_heads, dim = CALLS[call]
+    q, k, v, _ = inputs(nq, nk, heads, kv_heads, dim, dtype, cuda, seed=97)
+    rs = splits(nq, cuda), splits(nk, cuda)
+    clean = CrossAttention(q, k, v, *rs)
+    stay = torch.arange(len(q), device=cuda) % 3 != 1
+    for size in (0.01, 1., 30.):
+        other = torch.where(stay[:, None, None], q, size * q.flip(0, 1))
+        assert torch.equal(CrossAttention(other, k, v, *rs)[stay], clean[stay])
