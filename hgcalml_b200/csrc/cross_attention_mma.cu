@@ -130,6 +130,13 @@ struct Item {
     int begin, end, head0, split;       // of queries
 };
 
+// Weights are held 2^kShift times as large as they are next to the row's scale, and that may lag behind the row's maximum by a factor
+// of 2^kGrowth before the sums are scaled again.  Half precision reaches from 2^15 down to 2^-24 only, and many keys far below one that
+// dominates have a share together: what is rounded away of n of them is n 2^-37 of the largest value (without a shift, one key
+// 17.5 above 400k others took all of their 1 %).  2^14 and 2^1 cost wide heads 10 %: 128 columns, 200k queries on 1000 keys 545 -> 600 us.
+template <typename T> struct Weights { static constexpr float kShift = 0.f, kGrowth = 8.f; };
+template <> struct Weights<__half> { static constexpr float kShift = 12.f, kGrowth = 3.f; };
+
 // Counts through rounds of N.
 template <int N> struct Ring {
     int at = 0;
@@ -470,10 +477,10 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     }
                     float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                     next = fmaxf(next, exchange(maxima + (count & 1) * 2 * kMmaRows, next));
-                    // The sums are scaled again only where a row's maximum has grown by more than 2^8: weights up to that lose nothing
-                    // in either type.  The others of the warp stay as they are then, so that no result depends on which rows share a warp;
-                    // and rows that do not count have no say: what stands there may differ from run to run.
-                    const bool grown = store && (next - top) * c > 8.f;
+                    // The sums are scaled again only where a row's maximum has grown by more than that.  The others of the warp stay as
+                    // they are then, so that no result depends on which rows share a warp; and rows that do not count have no say: what
+                    // stands there may differ from run to run.
+                    const bool grown = store && (next - top) * c > Weights<T>::kGrowth;
                     const float before = top;
                     if (count == 0 || grown) top = next;
                     if (count == 0) {
@@ -491,7 +498,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                             tmem_store16(out + d, o);
                         }
                     }
-                    const float base = (top == -INFINITY ? 0.f : top) * c;
+                    const float base = (top == -INFINITY ? 0.f : top) * c - Weights<T>::kShift;
                     const pair base2 = pair_of(-base, -base);
                     pair sums[2] = {0, 0};
                     // The special function unit takes 8 cycles for a warp's exponentials; a quarter of them goes without it.  (There, a masked
@@ -543,7 +550,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             const int part = alternate ? 2 * it.split + g : it.split;
             if (store && half == 0) {
                 float *lse = parts ? a.part_lse + part * all_rows : a.lse;
-                lse[row] = none ? -INFINITY : top * a.scale + logf(sum);
+                lse[row] = none ? -INFINITY : top * a.scale + (logf(sum) - Weights<T>::kShift * kLn2);
             }
             float *to_part = parts ? a.part + part * all_rows * a.dim : nullptr;
             if (!idle && (done || !parts)) {  // a part without keys has no weight

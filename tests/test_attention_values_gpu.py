@@ -1,9 +1,11 @@
 """Attention between ragged sets: what its rows may hold (no number, infinities, weights and gradients of very different size), and what
 it refuses.  Formulas and the derivation of the bounds are those of test_cross_attention_gpu."""
+import math
+
 import pytest
 import torch
 
-from test_cross_attention_gpu import assert_near, inputs, reference, splits
+from test_cross_attention_gpu import E, TYPES, assert_near, inputs, reference, splits
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +98,33 @@ def test_a_row_does_not_depend_on_its_neighbours(cuda, dtype, call):
     for size in (0.01, 1., 30.):
         other = torch.where(stay[:, None, None], q, size * q.flip(0, 1))
         assert torch.equal(CrossAttention(other, k, v, *rs)[stay], clean[stay])
+
+
+@pytest.mark.parametrize("dtype", ["half", "bfloat"])
+@pytest.mark.parametrize("n_q,heads", [(100, 2), (300, 1), (1, 2), (4, 4)])
+@pytest.mark.parametrize("n_k", [200_000, 400_000])
+def test_one_key_far_above_all_others(cuda, dtype, n_q, heads, n_k):
+    """One key dominates, and hundreds of thousands have a share together, wherever the one is.  Values are one but for its zero, so a
+    result is the others' share.  With u the rounding of the type it is off by 2 u + 2^-12 (its own, the weights' and their powers of two),
+    by 2 x for the scores (see test_cross_attention_gpu), by 2^-23 for each of n / 16 sums that are cut off, and in half
+    precision by n 2^-37 for weights below its normal numbers."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    dim, one = 64, 1 if n_q == 4 else heads
+    q = torch.zeros((n_q, heads, dim), dtype=TYPES[dtype], device=cuda)
+    q[..., 0] = 8.  # the score is the key's first column
+    v = torch.ones((n_k, one, dim), dtype=q.dtype, device=cuda)
+    rs = splits([n_q], cuda), splits([n_k], cuda)
+    for gap in (10., 14., 16., 17., 17.5, 18., 20.):
+        for at in (0, 5, n_k // 2, n_k - 1):
+            k = torch.zeros_like(v)
+            k[at, :, 0], v[at] = gap, 0.
+            out, lse = CrossAttention(q, k, v, *rs, with_lse=True)
+            v[at] = 1.
+            others = (n_k - 1) * math.exp(-gap)
+            share = others / (1. + others)
+            u = torch.finfo(q.dtype).eps / 2
+            bound = share * (2 * u + 2. ** -12 + 2 * (3 * dim + 22) * E * gap + n_k / 16 * 2. ** -23)
+            if dtype == "half":
+                bound += n_k * 2. ** -37 + 2. ** -25
+            assert float((out.double() - share).abs().max()) <= bound, (gap, at, share, float(out.min()), float(out.max()))
+            assert float((lse.double() - gap - math.log1p(others)).abs().max()) <= 1e-5 * (1 + gap)
