@@ -475,12 +475,12 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                     }
-                    float next = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                    next = fmaxf(next, exchange(maxima + (count & 1) * 2 * kMmaRows, next));
+                    float next = max2(max3(m[0], m[1], m[2]), m[3]);
+                    next = max2(next, exchange(maxima + (count & 1) * 2 * kMmaRows, next));
                     // The sums are scaled again only where a row's maximum has grown by more than that.  The others of the warp stay as
                     // they are then, so that no result depends on which rows share a warp; and rows that do not count have no say: what
                     // stands there may differ from run to run.
-                    const bool grown = store && (next - top) * c > Weights<T>::kGrowth;
+                    const bool grown = store && !((next - top) * c <= Weights<T>::kGrowth);  // or is no number
                     const float before = top;
                     if (count == 0 || grown) top = next;
                     if (count == 0) {
@@ -541,9 +541,8 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
             if (done) after_sync();
             const long long row = (long long)(begin + r / a.pack) * a.heads + it.head0 + r % a.pack;
             if (some && !idle) sum += exchange(maxima + 2 * 2 * kMmaRows, sum);
-            // Scores of a query of NaN or infinity are no numbers where keys are cleared either, so that its sums say nothing; and those of
-            // keys that are seen must not be lost for the maximum, which passes over them.
-            const bool none = !any || (top == -INFINITY && sum == sum);
+            // Scores of a query of NaN or infinity are no numbers where keys are cleared either, so that its maximum says nothing.
+            const bool none = !any || top == -INFINITY;
             const float inv = none ? 0.f : 1.f / sum;
             const long long all_rows = (long long)a.n_q * a.heads;
             const bool parts = a.splits > 1 || alternate;

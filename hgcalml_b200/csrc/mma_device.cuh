@@ -243,34 +243,36 @@ __device__ __forceinline__ pair mul2(pair a, pair b)
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// What is no number stays it.
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of two floats of at most 127 without the special function unit: 2^n from the integer n next to x, put into the exponent,
-// times a polynomial of degree three in x - n that is off by 1.0e-04 at most (root mean square 6.4e-05), less than a quarter of half
-// precision's largest rounding.  Its coefficients give the least maximal relative error on [-1/2, 1/2] that goes with 2^0 = 1.
-// Below 2^-126 it stays there; what is no number gives none (2^n is a factor, and not added to the exponent: that made a finite
-// number of it).
-__device__ __forceinline__ float at_least(float a, float b)
+__device__ __forceinline__ float max2(float a, float b)
 {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// 2^x of two floats of at most 127 without the special function unit: 2^n from the integer n next to x, put into the exponent,
+// times a polynomial of degree three in x - n that is off by 1.0e-04 at most (root mean square 6.4e-05), less than a quarter of half
+// precision's largest rounding.  Its coefficients give the least maximal relative error on [-1/2, 1/2] that goes with 2^0 = 1.
+// Below 2^-126 it stays there.  What is no number gives a finite one or an infinity, so a row that may hold it has to tell by
+// something else, as its maximum does.
 __device__ __forceinline__ float2 exp2_arithmetic(float2 v)
 {
-    const pair x = pair_of(at_least(v.x, -126.f), at_least(v.y, -126.f));
+    const pair x = pair_of(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
     const pair magic = pair_of(12582912.f, 12582912.f), unmagic = pair_of(-12582912.f, -12582912.f), minus = pair_of(-1.f, -1.f);
     const pair t = add2(x, magic);                        // n in the low bits
     const pair f = fma2(add2(t, unmagic), minus, x);
     pair y = fma2(f, pair_of(0.0550091006f, 0.0550091006f), pair_of(0.242210984f, 0.242210984f));
     y = fma2(y, f, pair_of(0.693282902f, 0.693282902f));
     y = fma2(y, f, pair_of(1.f, 1.f));
-    const float2 n = parts(t);
-    return parts(mul2(y, pair_of(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u))));
+    const float2 p = parts(y), n = parts(t);
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
 }
 // two floats rounded to 16 bits, the first in the lower half
 template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
