@@ -661,6 +661,10 @@ grad_keys_kernel(const __grid_constant__ Args a)
     for (int i = 0; i < 2; i++) {
         const int r = row0 + (lane_id() >> 2) + 8 * i;
         if (r >= n_keys) continue;
+        if (!seen[i]) {  // a weight of zero does not make up for a query of NaN
+#pragma unroll
+            for (int n = 0; n < DP / 8; n++) dk[n][2 * i] = dk[n][2 * i + 1] = dv[n][2 * i] = dv[n][2 * i + 1] = 0.f;
+        }
         const long long row = (long long)(tile.begin + r) * a.kv_heads + kv;
         if (a.splits > 1) {
             const long long at = ((long long)blockIdx.z * a.n_k * a.kv_heads + row) * a.dim;

@@ -891,6 +891,9 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
             unsigned o[16] = {};
             if (some) {
                 tmem_load16(o, lanes + (KEYS && g == 0 ? F::kSums2 : F::kSums) + d);
+                if (KEYS)  // a key that is not seen: a weight of zero does not make up for a query of NaN
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] &= seen_row;
             }
             store16<T>(to, nullptr, to_part, place, d, a.dim, o, some ? by : 0.f);
         }

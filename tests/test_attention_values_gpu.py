@@ -128,3 +128,25 @@ def test_one_key_far_above_all_others(cuda, dtype, n_q, heads, n_k):
                 bound += n_k * 2. ** -37 + 2. ** -25
             assert float((out.double() - share).abs().max()) <= bound, (gap, at, share, float(out.min()), float(out.max()))
             assert float((lse.double() - gap - math.log1p(others)).abs().max()) <= 1e-5 * (1 + gap)
+
+
+@pytest.mark.parametrize("dtype,dim", [("float", 64), ("float", 128), ("half", 64), ("bfloat", 64), ("bfloat", 128), ("bfloat", 22)])
+def test_gradients_of_hidden_keys_are_zero_whatever_the_queries_are(cuda, dtype, dim):
+    """Masked keys of events whose queries, or their gradients, hold NaN and infinities: exactly zero; other events as without."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk = [140, 70, 300], [200, 90, 400]
+    q, k, v, grad = inputs(nq, nk, 4, 2, dim, dtype, cuda, seed=91)
+    mask = torch.rand(len(k), generator=torch.Generator(device=cuda).manual_seed(1), device=cuda) < 0.7
+    mask[200:290] = False
+    rs = splits(nq, cuda), splits(nk, cuda)
+
+    def run():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(CrossAttention(*leaves, *rs, key_mask=mask), leaves, grad)
+
+    clean = run()
+    q[7], q[150], grad[9], grad[160] = float("nan"), float("inf"), float("inf"), float("nan")
+    dq, dk, dv = run()
+    for got, before in ((dk, clean[1]), (dv, clean[2])):
+        assert (got[~mask] == 0).all() and torch.equal(got[290:], before[290:])
+    assert (dq[140:210] == 0).all() and torch.equal(dq[210:], clean[0][210:])
