@@ -395,12 +395,13 @@ join_forward_kernel(const float *__restrict__ part, const float *__restrict__ pa
 // What both gradients go by.  The first `n_count` blocks: the keys of an event that can be seen, counted up to two; with one key
 // the weights do not depend on the scores, so the gradients of q and k are zero and not what is left of two sums that cancel.
 // The next `n_rows` blocks, for every row of the queries: what its exponents are less by (log2 of its sum, less `shift`; infinity
-// without keys) and delta.  bounds: the largest squared norm of the rows of grad there, and of v in the blocks that follow.
+// without keys) and delta.  With `bounds`: the squared norms of the rows of grad there, and of every event the largest one that
+// counts of these, and of the rows of v in the blocks that follow.
 constexpr int kRowsALane = 4;
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ stats, int *__restrict__ visible, float *__restrict__ bounds, float shift,
-                        int n_count, int n_rows, int lanes_log2)
+prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ stats, int *__restrict__ visible, float *__restrict__ norms,
+                        float *__restrict__ bounds, float shift, int n_count, int n_rows, int lanes_log2)
 {
     pdl_begin();
     const int t = threadIdx.x;
@@ -427,6 +428,14 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
     const long long all = of_queries ? (long long)a.n_q * a.heads : (long long)a.n_k * a.kv_heads;
     const long long first = (long long)(of_queries ? block : block - n_rows) * (subs * kRowsALane) + t / lanes;
     const int known = of_queries ? split_at(a.rs_q, a.n_events, a.n_q) : split_at(a.rs_k, a.n_events, a.n_k);  // rows of some event
+    const int *__restrict__ rs = of_queries ? a.rs_q : a.rs_k;
+    const int n = of_queries ? a.n_q : a.n_k, per_row = of_queries ? a.heads : a.kv_heads;
+    __shared__ int s_event;  // of all of the block's rows, or -1
+    if (bounds != nullptr && t < 32) {
+        const long long begin = (long long)(of_queries ? block : block - n_rows) * (subs * kRowsALane), end = min(begin + subs * kRowsALane, all);
+        const int event = event_of_warp(rs, n, a.n_events, (int)(begin / per_row));
+        if (t == 0) s_event = event + 1 >= a.n_events || (end - 1) / per_row < split_at(rs, event + 1, n) ? event : -1;
+    }
     const T *__restrict__ out = static_cast<const T *>(a.out), *__restrict__ rest = static_cast<const T *>(a.out_rest),
             *__restrict__ grad = static_cast<const T *>(a.grad);
     float sum[kRowsALane], square[kRowsALane];
@@ -481,14 +490,23 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
         if (of_queries && lane == 0) {
             const float lse = a.lse[row];
             stats[row] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e - shift, sum[i]);
-        }
-        // rows behind the last event, and masked keys, are of no one's concern
-        if (bounds != nullptr) {
-            const long long token = row / (of_queries ? a.heads : a.kv_heads);
-            if (token < known && (of_queries || a.mask == nullptr || fresh(a.mask + token) != 0)) norm = fmaxf(norm, square[i]);
+            if (bounds != nullptr) norms[row] = square[i];
         }
     }
     if (bounds == nullptr) return;
+    __syncthreads();
+    // Norms are not negative, so their bits are in the order of their values: the largest one does not depend on the order of the blocks.
+    // Rows behind the last event, and masked keys, are of no one's concern.
+    const bool one_event = s_event >= 0;
+#pragma unroll
+    for (int i = 0; i < kRowsALane; i++) {
+        const long long row = first + (long long)i * subs, token = row / per_row;
+        if (row >= all || token >= known || (!of_queries && a.mask != nullptr && fresh(a.mask + token) == 0)) continue;
+        if (one_event) norm = fmaxf(norm, square[i]);
+        else if (lane == 0 && square[i] > 0.f)
+            atomicMax(reinterpret_cast<unsigned *>(bounds) + 2 * event_of(rs, n, a.n_events, (int)token) + (of_queries ? 0 : 1), __float_as_uint(square[i]));
+    }
+    if (!one_event) return;
     __shared__ float s_norm[kThreads / 32];
 #pragma unroll
     for (int w = 16; w > 0; w >>= 1) norm = fmaxf(norm, __shfl_xor_sync(0xffffffffu, norm, w));
@@ -496,8 +514,7 @@ prepare_backward_kernel(const __grid_constant__ Args a, float2 *__restrict__ sta
     __syncthreads();
     if (t == 0) {
         for (int i = 1; i < kThreads / 32; i++) norm = fmaxf(norm, s_norm[i]);
-        // norms are not negative, so their bits are in the order of their values, whatever the order of the blocks
-        if (norm > 0.f) atomicMax(reinterpret_cast<unsigned *>(bounds) + (of_queries ? 0 : 1), __float_as_uint(norm));
+        if (norm > 0.f) atomicMax(reinterpret_cast<unsigned *>(bounds) + 2 * s_event + (of_queries ? 0 : 1), __float_as_uint(norm));
     }
 }
 
@@ -801,26 +818,29 @@ template <typename C> ForwardBuffers carve_forward(C &c, const Plan &p, int n_q,
 
 struct BackwardBuffers {
     float2 *stats = nullptr;
-    float *bounds = nullptr, *part_q = nullptr, *part_k = nullptr, *part_v = nullptr;
+    float *norms = nullptr, *bounds = nullptr, *part_q = nullptr, *part_k = nullptr, *part_v = nullptr;
     int *visible = nullptr;
 };
-template <typename C> BackwardBuffers carve_backward(C &c, const Plan &p, int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim)
+template <typename C> BackwardBuffers carve_backward(C &c, const Plan &p, int n_q, int n_k, int n_rs, int heads, int kv_heads, int dim, int dtype)
 {
     BackwardBuffers b;
     const int splits_q = p.splits_q > p.splits_q_mma ? p.splits_q : p.splits_q_mma, splits_k = p.splits_k > p.splits_k_mma ? p.splits_k : p.splits_k_mma;
+    const size_t norms = dtype == HGC_FLOAT16 ? (size_t)n_q * heads : 0;
     const size_t rows = (size_t)n_q * heads, parts_q = splits_q > 1 ? splits_q * rows * dim : 0,
                  parts_k = splits_k > 1 ? (size_t)splits_k * n_k * kv_heads * dim : 0;
     if constexpr (std::is_same_v<C, Carver>) {
         b.stats = c.template take<float2>(rows);
         b.visible = c.template take<int>(n_rs);
-        b.bounds = c.template take<float>(2);
+        b.norms = c.template take<float>(norms);
+        b.bounds = c.template take<float>(2 * (size_t)n_rs);
         b.part_q = c.template take<float>(parts_q);
         b.part_k = c.template take<float>(parts_k);
         b.part_v = c.template take<float>(parts_k);
     } else {
         c.template take<float2>(rows);
         c.template take<int>(n_rs);
-        c.template take<float>(2);
+        c.template take<float>(norms);
+        c.template take<float>(2 * (size_t)n_rs);
         c.template take<float>(parts_q);
         c.template take<float>(parts_k);
         c.template take<float>(parts_k);
@@ -889,11 +909,11 @@ int backward_of(Args a, const Plan &p, const BackwardBuffers &b, void *dq, void 
     const int rows_a_block = kThreads / (lanes_log2 >= 0 ? 1 << lanes_log2 : 32) * kRowsALane;
     const int n_count = a.n_events > 0 ? a.n_events : 1, n_rows = div_up((long long)a.n_q * a.heads, rows_a_block),
               n_values = bounded ? div_up((long long)a.n_k * a.kv_heads, rows_a_block) : 0;
-    if (bounded) HGC_CUDA_TRY(cudaMemsetAsync(b.bounds, 0, 2 * sizeof(float), stream));
-    HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + n_rows + n_values, kThreads, 0, stream, a, b.stats, b.visible,
+    if (bounded) HGC_CUDA_TRY(cudaMemsetAsync(b.bounds, 0, 2 * sizeof(float) * (size_t)n_count, stream));
+    HGC_CUDA_TRY(launch_pdl(prepare_backward_kernel<T>, n_count + n_rows + n_values, kThreads, 0, stream, a, b.stats, b.visible, b.norms,
                             bounded ? b.bounds : nullptr, bounded ? kHalfShift : 0.f, n_count, n_rows, lanes_log2));
     HGC_LAUNCH_CHECK();
-    a.stats = b.stats; a.visible = b.visible; a.bounds = b.bounds; a.shift = bounded ? kHalfShift : 0.f;
+    a.stats = b.stats; a.visible = b.visible; a.norms = b.norms; a.bounds = b.bounds; a.shift = bounded ? kHalfShift : 0.f;
     if (dq != nullptr && a.n_q > 0) {
         a.to = dq; a.to2 = nullptr; a.part = b.part_q; a.part2 = nullptr; a.splits = mma_q ? p.splits_q_mma : p.splits_q;
         if (const int rc = mma_q ? mma_grad_queries(a, dtype, stream)
@@ -979,10 +999,9 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
 
 extern "C" size_t hgc_cross_attention_grad_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype)
 {
-    (void)dtype;
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return 0;
     Sizer s;
-    carve_backward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim), n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
+    carve_backward(s, plan_of(n_q, n_k, n_rs, n_heads, n_kv_heads, dim), n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype);
     return s.used;
 }
 
@@ -1007,7 +1026,7 @@ extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q,
     Args a = args_of(d_q, d_k, d_v, d_q_row_splits, d_k_row_splits, d_key_mask, const_cast<float *>(d_lse), n_q, n_k, n_rs, n_heads, n_kv_heads, dim,
                      strides, scale, p, workspace);
     Carver carver(workspace);
-    const BackwardBuffers b = carve_backward(carver, p, n_q, n_k, n_rs, n_heads, n_kv_heads, dim);
+    const BackwardBuffers b = carve_backward(carver, p, n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype);
     a.grad = d_grad_out; a.out = d_out; a.out_rest = dtype == HGC_FLOAT32 ? nullptr : d_out_rest;
     return dtype == HGC_FLOAT32 ? backward_of<float>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream)
          : dtype == HGC_FLOAT16 ? backward_of<__half>(a, p, b, d_grad_q, d_grad_k, d_grad_v, dtype, stream)

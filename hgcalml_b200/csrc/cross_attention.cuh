@@ -37,7 +37,9 @@ struct Args {
     void *to, *to2;                // result: out, dq, or dk and dv
     float *part, *part2;           // the same of every part of a split, in float32
     float *part_lse;               // [splits, n_q, heads]
-    const float *bounds;           // largest squared norms of the rows of grad and of v (half precision's backward pass)
+    // of half precision's backward pass: squared norms of the rows of grad, [n_q, heads], and the largest ones of the rows of grad and of v
+    // that count in an event, [n_events, 2]
+    const float *norms, *bounds;
     int *counter;                  // of the tiles that the blocks of the forward pass take
     unsigned *status;
     int n_q, n_k, n_events, heads, kv_heads, group, pack, dim, splits, alternate;  // alternate: of the forward pass on the tensor cores, two parts to each of the splits
@@ -78,6 +80,31 @@ __device__ __forceinline__ Tile find_tile(const int *rs, int n, int n_events, in
     t.begin = begin < 0 || begin > last ? last : (int)begin;
     t.end = last - t.begin < rows ? last : t.begin + rows;  // no sum beyond 32 bits
     return t;
+}
+
+// The event of a row below `known`, the end of the last one: the last event that begins there or before.
+__device__ __forceinline__ int event_of(const int *rs, int n, int n_events, int row)
+{
+    int lo = 0, hi = n_events;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (split_at(rs, mid, n) <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// The same by the 32 lanes of a warp together.
+__device__ __forceinline__ int event_of_warp(const int *rs, int n, int n_events, int row)
+{
+    int lo = 0, hi = n_events;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5, at = lo + lane_id() * step;
+        const unsigned votes = __ballot_sync(0xffffffffu, at < hi && split_at(rs, at, n) <= row);
+        lo += (max(votes == 0xffffffffu ? 32 : __ffs(~votes) - 1, 1) - 1) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
 }
 
 // Steps [first, last) of part `s` of `n_parts` of a row of `steps`.

@@ -580,15 +580,17 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
 
 // ------------------------------------------------------------------------------------------------------------ backward
 // Half precision reaches down to 2^-24 only, and a weight among many keys lies below that: weights are held 2^14 times as large
-// there, and their gradients are scaled by a power of two under which none can overflow (|do.v - delta| <= 2 max|do| max|v|).
+// there, and their gradients are scaled by a power of two under which none can overflow (|do.v - delta| <= 2 max|do| max|v|): one for
+// each row of the gradient of queries, and, as the gradient of a key is a sum over the queries, one for each event there.
 // Both factors are taken out of the float32 sums.
 template <typename T> struct Range { static constexpr float kShift = 0.f; };
 template <> struct Range<__half> { static constexpr float kShift = kHalfShift; };
 
-template <typename T> __device__ __forceinline__ float slope_factor(const Args &a)
+// `row`: of the gradient, or -1 for the largest of the event
+template <typename T> __device__ __forceinline__ float slope_factor(const Args &a, int event, long long row)
 {
-    if (Range<T>::kShift == 0.f) return 1.f;
-    const float bound = sqrtf(fresh(a.bounds)) * sqrtf(fresh(a.bounds + 1));
+    if (Range<T>::kShift == 0.f || event >= a.n_events) return 1.f;
+    const float bound = sqrtf(fresh(row < 0 ? a.bounds + 2 * event : a.norms + row)) * sqrtf(fresh(a.bounds + 2 * event + 1));
     return bound > 0.f && bound < 1e30f ? exp2f(-ceilf(log2f(bound))) : 1.f;
 }
 
@@ -777,13 +779,13 @@ grad_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps map
         const int g = warp >> 2, r = t & 127;  // the lane has row r in every other step, beginning with step g
         const unsigned lanes = tmem + ((unsigned)(warp & 3) << 21);
         const bool idle = (warp & 3) * 32 >= n_rows, store = r < n_rows;
-        const float scale = a.scale * kLog2e, factor = slope_factor<T>(a);
-        const pair c = pair_of(scale, scale), f = pair_of(factor, factor);
         // KEYS: of the columns, in the warp's own shared memory, negative, first the exponents' and then the slopes'.  Else of this
         // lane's row.
         float *stats = reinterpret_cast<float *>(s_raw + F::kTiles) + warp * 2 * N;
         const long long row = KEYS ? ((long long)(tile.begin + r) * a.kv_heads + kv)
                                    : (long long)(tile.begin + r / a.pack) * a.heads + blockIdx.y * a.pack + r % a.pack;
+        const float scale = a.scale * kLog2e, factor = KEYS || store ? slope_factor<T>(a, tile.event, KEYS ? -1 : row) : 1.f;
+        const pair c = pair_of(scale, scale), f = pair_of(factor, factor);
         pair shift = 0, delta = 0;
         unsigned seen_row = 0xffffffffu;
         if (KEYS) {

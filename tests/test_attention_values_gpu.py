@@ -150,3 +150,63 @@ def test_gradients_of_hidden_keys_are_zero_whatever_the_queries_are(cuda, dtype,
     for got, before in ((dk, clean[1]), (dv, clean[2])):
         assert (got[~mask] == 0).all() and torch.equal(got[290:], before[290:])
     assert (dq[140:210] == 0).all() and torch.equal(dq[210:], clean[0][210:])
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 2, 2), (128, 2, 1), (40, 3, 1)])
+def test_gradients_in_half_do_not_depend_on_other_events(cuda, dim, heads, kv_heads):
+    """Rows of another event that are 2^20 times as large, or infinite, change no bit."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk = [150, 7, 300, 0, 90], [2000, 300, 700, 50, 4000]
+    q, k, v, grad = inputs(nq, nk, heads, kv_heads, dim, "half", cuda, seed=101)
+    rs = splits(nq, cuda), splits(nk, cuda)
+    mask = torch.ones(len(k), dtype=torch.bool, device=cuda)
+    mask[2001] = mask[5] = False
+    grad *= 2. ** -10
+
+    def run():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(CrossAttention(*leaves, *rs, key_mask=mask), leaves, grad)
+
+    clean = run()
+    want, _ = reference(q, k, v, nq, nk, dim ** -0.5, mask, grad)
+    for got, name in zip(clean, ("dq", "dk", "dv")):
+        assert_near(got, want[name], name)
+    for large in (1024., 60000., float("inf")):
+        grad[151:153], grad[200:210], v[2001:2010], v[2400:2410], v[5] = large, -large, large, large, large  # of events 1 and 2, and a masked key
+        for got, before, gone in zip(run(), clean, (slice(150, 457), slice(2000, 3000), slice(2000, 3000))):
+            keep = torch.ones(len(got), dtype=torch.bool, device=cuda)
+            keep[gone] = False
+            assert torch.equal(got[keep], before[keep])
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 2, 1), (128, 1, 1)])
+def test_gradients_of_very_different_size_in_half(cuda, dim, heads, kv_heads):
+    """Rows of the gradient 2^20 apart in an event, on so many keys that a weight is 2^-15.  A slope of half precision is off by 2^-25 where it is below
+    the normal numbers, in units of 2^14 times a power of two of at least 1 / (2 |do| max|v|), with do the row's gradient for dq and
+    the event's largest for dk: by 2^-38 |do| max|v|; a weight by 2^-39."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk = [300, 40], [40000, 3000]
+    q, k, v, grad = inputs(nq, nk, heads, kv_heads, dim, "half", cuda, seed=102)
+    grad[::7] *= 2. ** 10
+    grad[1::7] *= 2. ** -10
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(CrossAttention(*leaves, splits(nq, cuda), splits(nk, cuda)), leaves, grad)
+    want, _ = reference(q.detach(), k.detach(), v.detach(), nq, nk, dim ** -0.5, None, grad)
+    with torch.no_grad():
+        a = b = 0
+        for n, m in zip(nq, nk):
+            rows, keys = slice(a, a + n), slice(b, b + m)
+            a, b = a + n, b + m
+            do, vs = grad[rows].double().norm(dim=-1), v[keys].double().norm(dim=-1).max()
+            for h in range(heads):
+                kv = h * kv_heads // heads
+                want["dq"][1][rows, h] += dim ** -0.5 * 2. ** -38 * do[:, h, None] * vs * k[keys, kv].double().abs().sum(0)
+                want["dk"][1][keys, kv] += dim ** -0.5 * 2. ** -38 * do.max() * vs * q[rows, h].double().abs().sum(0)
+                want["dv"][1][keys, kv] += 2. ** -39 * grad[rows, h].double().abs().sum(0)
+        for g, name in zip(got, ("dq", "dk", "dv")):
+            assert_near(g, want[name], name)
+    # the gradient of a query depends on its own row alone
+    small = torch.arange(len(q), device=cuda) % 7 == 1
+    grad[~small] *= 2. ** -10
+    again, = torch.autograd.grad(CrossAttention(*leaves, splits(nq, cuda), splits(nk, cuda)), leaves[:1], grad)
+    assert torch.equal(again[small], got[0][small])
