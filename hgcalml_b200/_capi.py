@@ -150,6 +150,16 @@ def read_status(ws: torch.Tensor, raise_on_flag: bool = True) -> int:
     return out.value
 
 
+# HGC_CHECK_STATUS=1: ops that hand over their workspace wait for their end and raise what the device found wrong (row
+# splits that do not ascend, a wait that was given up).  Off, no call waits, and results are unspecified then.
+CHECK_STATUS = os.environ.get("HGC_CHECK_STATUS", "0") not in ("", "0")
+
+
+def check_status(ws) -> None:
+    if CHECK_STATUS and ws is not None and not torch.cuda.is_current_stream_capturing():
+        read_status(ws)
+
+
 def _as(t, dtype, device):
     # the usual argument is a dense tensor of the right type and needs no call into torch
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_contiguous() and (device is None or t.device == device):

@@ -54,8 +54,9 @@ def _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key
 
 
 def _forward(q, k, v, rs_q, rs_k, scale, mask, with_rest=False):
-    out, rest, lse, rc = C.native.cross_attention(q, k, v, rs_q, rs_k, mask, scale, with_rest)
+    out, rest, lse, ws, rc = C.native.cross_attention(q, k, v, rs_q, rs_k, mask, scale, with_rest)
     C.check(rc, "CrossAttention")
+    C.check_status(ws)
     return out, rest, lse
 
 
@@ -75,9 +76,10 @@ def CrossAttentionGrad(grad, queries, keys, values, out, lse, query_row_splits, 
         if out_rest.shape != out.shape or out_rest.dtype != out.dtype or out_rest.device != out.device:
             raise C.HgcError("CrossAttentionGrad expects out_rest like out")
         out_rest = out_rest.contiguous()
-    dq, dk, dv, rc = C.native.cross_attention_grad(grad.to(q.dtype).contiguous(), q, k, v, out.contiguous(), out_rest, lse.contiguous(),
-                                                   rs_q, rs_k, mask, scale, need_queries, need_keys)
+    dq, dk, dv, ws, rc = C.native.cross_attention_grad(grad.to(q.dtype).contiguous(), q, k, v, out.contiguous(), out_rest, lse.contiguous(),
+                                                       rs_q, rs_k, mask, scale, need_queries, need_keys)
     C.check(rc, "CrossAttentionGrad")
+    C.check_status(ws)
     return dq, dk, dv
 
 
@@ -109,7 +111,8 @@ def CrossAttention(queries, keys, values, query_row_splits, key_row_splits, scal
     ``queries [N, heads, D]``, ``keys`` and ``values [M, key heads, D]`` of one type (float32, float16, bfloat16; D up to
     128), rows and heads at any distance; the heads are shared evenly among the key heads, head h reads key head
     ``h // (heads // key_heads)``.  ``query_row_splits`` and ``key_row_splits [E+1]``: the rows of every event, which may be
-    none, and which may end before the tensors do.  ``scale`` is ``D ** -0.5`` unless given.  ``key_mask [M]`` (bool): keys
+    none, and which may end before the tensors do; they have to ascend from zero (HGC_CHECK_STATUS=1 in the environment checks
+    that).  ``scale`` is ``D ** -0.5`` unless given.  ``key_mask [M]`` (bool): keys
     that no query may see are False, and what their rows hold does not matter.  A query that sees no key gets zeros.
 
     Returns the rows ``[N, heads, D]``, with ``with_lse`` also the float32 logarithm of every row's sum of

@@ -948,6 +948,13 @@ Args args_of(const void *q, const void *k, const void *v, const int *rs_q, const
     return a;
 }
 
+// A workspace that comes along is left with a status word all the same.
+int nothing_to_do(void *workspace, size_t bytes, cudaStream_t stream)
+{
+    if (workspace != nullptr && bytes >= sizeof(unsigned)) HGC_CUDA_TRY(cudaMemsetAsync(workspace, 0, sizeof(unsigned), stream));
+    return HGC_OK;
+}
+
 bool scale_ok(float scale) { return scale > 0.f && scale <= 3.4e38f; }
 bool strides_ok(const long long *strides)
 {
@@ -982,7 +989,7 @@ extern "C" int hgc_cross_attention(const void *d_q, const void *d_k, const void 
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !scale_ok(scale) || !strides_ok(strides) || dtype < 0 || dtype > HGC_BFLOAT16)
         return HGC_ERR_INVALID_ARGUMENT;
     if (!sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return HGC_ERR_UNSUPPORTED;
-    if (n_q == 0) return HGC_OK;
+    if (n_q == 0) return nothing_to_do(workspace, workspace_bytes, stream);
     if (!d_q || !d_out || !d_lse || !d_q_row_splits || !d_k_row_splits || (n_k > 0 && (!d_k || !d_v))) return HGC_ERR_INVALID_ARGUMENT;
     if (const int rc = check_workspace(workspace, workspace_bytes,
                                        hgc_cross_attention_workspace_bytes(n_q, n_k, n_rs, n_heads, n_kv_heads, dim, dtype)))
@@ -1015,7 +1022,7 @@ extern "C" int hgc_cross_attention_grad(const void *d_grad_out, const void *d_q,
     if (!sizes_ok(n_q, n_k, n_rs, n_heads, n_kv_heads, dim) || !scale_ok(scale) || !strides_ok(strides) || dtype < 0 || dtype > HGC_BFLOAT16)
         return HGC_ERR_INVALID_ARGUMENT;
     if (!sizes_supported(n_q, n_k, n_rs, n_heads, dim)) return HGC_ERR_UNSUPPORTED;
-    if (n_q == 0 && n_k == 0) return HGC_OK;
+    if (n_q == 0 && n_k == 0) return nothing_to_do(workspace, workspace_bytes, stream);
     if (!d_q_row_splits || !d_k_row_splits || (n_q > 0 && (!d_grad_out || !d_q || !d_out || !d_lse)) || (n_k > 0 && (!d_k || !d_v)) ||
         !d_grad_k != !d_grad_v)
         return HGC_ERR_INVALID_ARGUMENT;

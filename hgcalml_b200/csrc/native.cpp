@@ -157,12 +157,12 @@ void distances(const Tensor &t, long long *to)
 
 bool fits(const Tensor &t) { return t.size(0) <= 0x7fffffff; }
 
-// (rows, logarithms of the sums, status)
-std::tuple<Tensor, MaybeTensor, Tensor, int> cross_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &rs_q, const Tensor &rs_k,
+// (rows, what their rounding left or None, logarithms of the sums, workspace, status)
+std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor, int> cross_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &rs_q, const Tensor &rs_k,
                                                              const MaybeTensor &mask, double scale, bool with_rest)
 {
     MaybeTensor rest;
-    if (!fits(q) || !fits(k) || !fits(rs_q)) return {q, rest, q, HGC_ERR_UNSUPPORTED};
+    if (!fits(q) || !fits(k) || !fits(rs_q)) return {q, rest, q, std::nullopt, HGC_ERR_UNSUPPORTED};
     const int n_q = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), n_k = (int)k.size(0), kv_heads = (int)k.size(1);
     const int n_rs = (int)rs_q.size(0), type = type_code(q);
     long long strides[6];
@@ -175,17 +175,16 @@ std::tuple<Tensor, MaybeTensor, Tensor, int> cross_attention(const Tensor &q, co
     const int rc = hgc_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), data<int>(rs_q), data<int>(rs_k), data<unsigned char>(mask), out.data_ptr(),
                                        rest.has_value() ? rest->data_ptr() : nullptr, data<float>(lse), n_q, n_k, n_rs, heads, kv_heads, dim, strides, (float)scale, type, ws.data_ptr(),
                                        (size_t)ws.numel(), stream_of(q));
-    return {out, rest, lse, rc};
+    return {out, rest, lse, ws, rc};
 }
 
-// (gradients of q, k, v or None, status)
-std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, int> cross_attention_grad(const Tensor &grad, const Tensor &q, const Tensor &k, const Tensor &v,
-                                                                            const Tensor &out, const MaybeTensor &rest, const Tensor &lse,
-                                                                            const Tensor &rs_q, const Tensor &rs_k, const MaybeTensor &mask, double scale,
-                                                                            bool need_q, bool need_k)
+// (gradients of q, k, v or None, workspace, status)
+std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor, int> cross_attention_grad(
+        const Tensor &grad, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &out, const MaybeTensor &rest, const Tensor &lse,
+        const Tensor &rs_q, const Tensor &rs_k, const MaybeTensor &mask, double scale, bool need_q, bool need_k)
 {
     MaybeTensor dq, dk, dv;
-    if (!fits(q) || !fits(k) || !fits(rs_q)) return {dq, dk, dv, HGC_ERR_UNSUPPORTED};
+    if (!fits(q) || !fits(k) || !fits(rs_q)) return {dq, dk, dv, std::nullopt, HGC_ERR_UNSUPPORTED};
     const int n_q = (int)q.size(0), heads = (int)q.size(1), dim = (int)q.size(2), n_k = (int)k.size(0), kv_heads = (int)k.size(1);
     const int n_rs = (int)rs_q.size(0), type = type_code(q);
     long long strides[6];
@@ -202,7 +201,7 @@ std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, int> cross_attention_grad(cons
     const int rc = hgc_cross_attention_grad(grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), at(rest), data<float>(lse),
                                             data<int>(rs_q), data<int>(rs_k), data<unsigned char>(mask), at(dq), at(dk), at(dv), n_q, n_k, n_rs, heads, kv_heads,
                                             dim, strides, (float)scale, type, ws.data_ptr(), (size_t)ws.numel(), stream_of(q));
-    return {dq, dk, dv, rc};
+    return {dq, dk, dv, ws, rc};
 }
 
 // One of the two sets of rows of a norm_rotate call.

@@ -433,7 +433,7 @@ int hgc_push_knn_grad_ordered(
  * from run to run.
  *
  * Splits that do not ascend from 0 to at most the number of rows set HGC_STATUS_ROW_SPLITS; the results are then
- * unspecified.  A wait inside a kernel that did not end in time sets HGC_STATUS_ITERATION_CAP.
+ * unspecified, as they are where a wait inside a kernel did not end in time, which sets HGC_STATUS_ITERATION_CAP.
  * ------------------------------------------------------------------------------------- */
 size_t hgc_cross_attention_workspace_bytes(int n_q, int n_k, int n_rs, int n_heads, int n_kv_heads, int dim, int dtype);
 int hgc_cross_attention(

@@ -210,3 +210,27 @@ def test_gradients_of_very_different_size_in_half(cuda, dim, heads, kv_heads):
     grad[~small] *= 2. ** -10
     again, = torch.autograd.grad(CrossAttention(*leaves, splits(nq, cuda), splits(nk, cuda)), leaves[:1], grad)
     assert torch.equal(again[small], got[0][small])
+
+
+@pytest.mark.parametrize("dtype", ["float", "bfloat"])
+def test_what_the_device_finds_wrong_is_raised_on_demand(cuda, dtype, monkeypatch):
+    from hgcalml_b200 import _capi as C
+    from hgcalml_b200.cross_attention_op import CrossAttention, CrossAttentionGrad
+    q, k, v, grad = inputs([100], [200], 2, 2, 64, dtype, cuda)
+    good = splits([40, 60], cuda), splits([50, 100], cuda)
+    bad = splits([40, 60], cuda), torch.tensor([0, 150, 100], dtype=torch.int32, device=cuda)
+    want, lse = CrossAttention(q, k, v, *good, with_lse=True)
+    CrossAttention(q, k, v, *bad)  # unspecified, and nothing waits
+    monkeypatch.setattr(C, "CHECK_STATUS", True)
+    assert torch.equal(CrossAttention(q, k, v, *good), want)
+    CrossAttentionGrad(grad, q, k, v, want, lse, *good)
+    assert CrossAttention(q[:0], k, v, *[torch.zeros_like(good[0])] * 2).shape == (0, 2, 64)
+    with pytest.raises(C.HgcError, match="row splits"):
+        CrossAttention(q, k, v, *bad)
+    with pytest.raises(C.HgcError, match="row splits"):
+        CrossAttentionGrad(grad, q, k, v, want, lse, *bad)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # a capture cannot wait
+        held = CrossAttention(q, k, v, *good)
+    graph.replay()
+    assert torch.equal(held, want)
