@@ -11,6 +11,7 @@ import os
 from ctypes import c_int, c_size_t, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhgcalml_b200.so")
@@ -276,6 +277,12 @@ def noted_lists(idx):
     """The lists of the search that this table came from, unless it was written to since."""
     lists = _noted(idx, "_hgc_lists", BackwardLists)
     return lists if lists is not None and lists.version is not None and lists.version == version_of(idx) else None
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """For ops without a forward-mode derivative, which hand raw pointers on: a dual tensor would lose its tangent without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise HgcError(f"{what} has no forward-mode derivative")
 
 
 def require_cuda(*tensors):

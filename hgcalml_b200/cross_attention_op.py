@@ -24,6 +24,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key_mask):
     C.require_cuda(queries, keys, values)
+    C.refuse_tangents("CrossAttention", queries, keys, values)
     q, k, v = queries, keys, values
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
         raise C.HgcError("CrossAttention expects queries [N, heads, D] and keys and values [M, key heads, D], not "
@@ -67,6 +68,7 @@ def CrossAttentionGrad(grad, queries, keys, values, out, lse, query_row_splits, 
     they are rounded, of their type, if known; it makes up for their rounding where few keys have all the weight."""
     q, k, v, rs_q, rs_k, scale, mask = _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key_mask)
     C.require_cuda(grad, out, lse)
+    C.refuse_tangents("CrossAttentionGrad", grad, out, lse)
     if grad.shape != q.shape or out.shape != q.shape or lse.shape != q.shape[:2]:
         raise C.HgcError("CrossAttentionGrad expects grad and out like the queries and one lse per row and head")
     if out.dtype != q.dtype or lse.dtype != torch.float32 or any(t.device != q.device for t in (grad, out, lse)):
@@ -117,7 +119,8 @@ def CrossAttention(queries, keys, values, query_row_splits, key_row_splits, scal
 
     Returns the rows ``[N, heads, D]``, with ``with_lse`` also the float32 logarithm of every row's sum of
     exponentials ``[N, heads]`` (``-inf`` without keys), from which results over parts of the keys can be joined.
-    Differentiable in queries, keys and values, once, with results that do not change from run to run."""
+    Differentiable in queries, keys and values, once and backwards only, with results that do not change from run to run.
+    The logarithms carry no gradient: what is joined with them is for use without one."""
     q, k, v, rs_q, rs_k, scale, mask = _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key_mask)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _CrossAttentionFunction.apply(q, k, v, rs_q, rs_k, scale, mask)

@@ -40,6 +40,7 @@ def _check_set(what, x, weight, positions, like):
 
 def _prepare(queries, keys, query_weight, key_weight, query_positions, key_positions, rotary_dim, base, eps):
     C.require_cuda(queries, keys)
+    C.refuse_tangents("NormRotate", queries, keys, query_weight, key_weight, query_positions, key_positions)
     if queries.dim() != 3 or queries.dtype not in _TYPES or not 1 <= queries.shape[2] <= _MAX_DIM:
         raise C.HgcError(f"NormRotate expects queries [N, heads, D] in float32, float16 or bfloat16 with D from 1 to {_MAX_DIM}, not "
                          f"{tuple(queries.shape)} in {queries.dtype}")
@@ -117,7 +118,7 @@ def NormRotate(queries, keys=None, query_weight=None, key_weight=None, query_pos
     ``interleaved`` -- and pair i turns by ``position / base ** (i / pairs)``.
 
     Returns ``(queries, keys)`` as dense tensors of the inputs' type (keys None if not given).  Differentiable in rows and
-    weights, once; positions get no gradient.  Results do not change from run to run."""
+    weights, once and backwards only; positions get no gradient.  Results do not change from run to run."""
     q, k, wq, wk, pq, pk, rotary, axes = _prepare(queries, keys, query_weight, key_weight, query_positions, key_positions, rotary_dim,
                                                   base, eps)
     how = (rotary, axes, bool(interleaved), float(base), float(eps))
