@@ -122,7 +122,8 @@ def CrossAttention(queries, keys, values, query_row_splits, key_row_splits, scal
     Differentiable in queries, keys and values, once and backwards only, with results that do not change from run to run.
     The logarithms carry no gradient: what is joined with them is for use without one."""
     q, k, v, rs_q, rs_k, scale, mask = _prepare(queries, keys, values, query_row_splits, key_row_splits, scale, key_mask)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    # a trace needs a node that stands for the call
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) or torch.jit.is_tracing():
         out, lse = _CrossAttentionFunction.apply(q, k, v, rs_q, rs_k, scale, mask)
     else:
         out, _, lse = _forward(q, k, v, rs_q, rs_k, scale, mask)

@@ -122,6 +122,7 @@ def NormRotate(queries, keys=None, query_weight=None, key_weight=None, query_pos
     q, k, wq, wk, pq, pk, rotary, axes = _prepare(queries, keys, query_weight, key_weight, query_positions, key_positions, rotary_dim,
                                                   base, eps)
     how = (rotary, axes, bool(interleaved), float(base), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
+    # a trace needs a node that stands for the call
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)) or torch.jit.is_tracing():
         return _NormRotateFunction.apply(q, k, wq, wk, pq, pk, *how)
     return _forward(q, k, wq, wk, pq, pk, *how)

@@ -35,6 +35,17 @@ def test_tangents_are_refused(cuda, which):
     assert torch.equal(call(*args), want)
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_a_trace_does_not_keep_a_result_as_a_constant(cuda, which, grad):
+    call, args = _calls(cuda)[which]
+    leaves = [args[0].clone().requires_grad_(grad), *args[1:]]
+    traced = torch.jit.trace(call, tuple(leaves), check_trace=False)
+    other = [2. * args[0].roll(1, 0) + 1., *args[1:]]
+    assert torch.equal(traced(*other), call(*other)) and not torch.equal(call(*other), call(*args))
+
+
 def test_gradients_of_given_tensors_refuse_tangents(cuda):
     from hgcalml_b200 import _capi as C
     from hgcalml_b200.cross_attention_op import CrossAttention, CrossAttentionGrad
