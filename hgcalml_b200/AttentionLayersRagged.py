@@ -16,8 +16,9 @@ class RaggedCrossAttention(torch.nn.Module):
 
     ``n_heads`` heads of ``n_head_features`` columns, which share ``n_key_heads`` key heads; queries and keys are scaled to unit
     size per head and, where positions are given (coordinates ``[N, axes]`` or integers ``[N]``, as ``NormRotate`` takes them),
-    turned by them.  ``key_mask [M]``: rows of the context that nobody may see are False.  A row without any gets what the
-    output transform makes of zeros.
+    turned by them.  ``key_mask [M]``: rows of the context that nobody may see are False, and what they and their positions hold
+    does not matter.  A row without any gets what the output transform makes of zeros.  Rows behind the last event get the same;
+    where gradients are asked for they have to be finite, as the rows of any dense layer.
 
     The context is projected to keys and values at once; ``prepare`` does that ahead of time, for a context that many
     queries are asked of one after the other, and its result may be passed in place of the context."""
@@ -36,12 +37,22 @@ class RaggedCrossAttention(torch.nn.Module):
         self.key_scale = torch.nn.Parameter(torch.ones(n_head_features))
         self.output_transform = _Dense(n_heads * n_head_features, n_out, activation)
 
+    @staticmethod
+    def _seen(key_mask, context, key_positions):
+        """Zeros where nobody looks: a gradient of zero does not make up for a row of NaN in the gradients of the transforms."""
+        if key_mask is None or not torch.is_grad_enabled() or key_mask.numel() != context.shape[0]:  # CrossAttention refuses the last
+            return context, key_positions
+        key_mask = key_mask.reshape(-1) != 0
+        return [None if t is None else t.masked_fill(~key_mask.reshape(-1, *[1] * (t.dim() - 1)), 0) for t in (context, key_positions)]
+
     def _keys_values(self, context):
         both = self.context_transform(context).unflatten(-1, (2, self.n_key_heads, self.n_head_features))
         return both[:, 0], both[:, 1]
 
-    def prepare(self, context, key_positions=None):
-        """Keys, scaled and turned, and values of a context."""
+    def prepare(self, context, key_positions=None, key_mask=None):
+        """Keys, scaled and turned, and values of a context.  ``key_mask`` is needed where gradients are and masked rows may hold
+        anything."""
+        context, key_positions = self._seen(key_mask, context, key_positions)
         keys, values = self._keys_values(context)
         keys, _ = NormRotate(keys, None, self.key_scale, None, key_positions, **self.how)
         return keys, values
@@ -55,6 +66,7 @@ class RaggedCrossAttention(torch.nn.Module):
             keys, values = context
             queries, _ = NormRotate(queries, None, self.query_scale, None, query_positions, **self.how)
         else:
+            context, key_positions = self._seen(key_mask, context, key_positions)
             keys, values = self._keys_values(context)
             queries, keys = NormRotate(queries, keys, self.query_scale, self.key_scale, query_positions, key_positions, **self.how)
         out = CrossAttention(queries, keys, values, row_splits, context_row_splits, key_mask=key_mask)
