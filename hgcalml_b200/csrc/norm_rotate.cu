@@ -108,7 +108,7 @@ __device__ __forceinline__ void store(T *__restrict__ to, const float (&from)[V]
 // lanes these do not meet in the same banks.
 template <int V, Pairs P> __device__ __forceinline__ int place(int pair, int n_pairs)
 {
-    constexpr int A = P == kHalves || P == kBothHalves ? V : V / 2;  // angles of a lane
+    constexpr int A = P == kHalves || P == kBothHalves ? V : (V + 1) / 2;  // angles of a lane
     if constexpr (P == kAnywhere || A < 4) return pair;
     else return pair < n_pairs / A * A ? (pair % A / 2 * (n_pairs / A) + pair / A) * 2 + pair % 2 : pair;
 }
@@ -167,13 +167,13 @@ template <int V, int E, Pairs P> struct Columns {
         if constexpr (P == kBothHalves) pair[0] = lane_in_row * V;
         if constexpr (P < kHalves) pair[0] = max(column[0], 0) / 2;  // a lane's columns hold whole axes, or neighbours
         if constexpr (P == kHalves) {
-            const int span = 2 * c.pairs, axis = max(column[0], 0) / span, off = max(column[0], 0) - axis * span;
+            const int span = max(2 * c.pairs, 1), axis = max(column[0], 0) / span, off = max(column[0], 0) - axis * span;
             const bool second = off >= c.pairs;
             pair[0] = axis * c.pairs + (second ? off - c.pairs : off);
             sign = second ? 1.f : -1.f;
             if (turned[0] && column[0] >= 0) partner_lane += (second ? -c.pairs : c.pairs) / V;
         }
-        constexpr int A = P == kHalves || P == kBothHalves ? V : V / 2;
+        constexpr int A = P == kHalves || P == kBothHalves ? V : (V + 1) / 2;
         const int n_pairs = c.rotary / 2;
         const bool in_order = A < 4 || pair[0] >= n_pairs / A * A;
         at = in_order ? pair[0] : pair[0] / A * 2;

@@ -1,4 +1,4 @@
-"""Rotation by positions so far on that the digits of double precision count."""
+"""Rotation by positions so far on that the digits of double precision count, and none at all."""
 import math
 from decimal import Decimal, getcontext
 
@@ -32,3 +32,19 @@ def test_far_positions(cuda, dim, base, interleaved):
         bound = size * (off + (dim + 16) * 2. ** -24)
         assert ((y[row][:, first].double() - (a * angle.cos() - b * angle.sin())).abs() <= bound).all()
         assert ((y[row][:, second].double() - (b * angle.cos() + a * angle.sin())).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 8, 22, 33, 64, 100, 128])
+def test_no_column_turns(cuda, dtype, dim):
+    """``rotary_dim`` of zero is no rotation, whatever the positions are, forward and backward."""
+    from hgcalml_b200.norm_rotate_op import NormRotate
+    g = torch.Generator(device=cuda).manual_seed(dim)
+    x, grad = (torch.randn((37, 3, dim), generator=g, device=cuda).to(dtype) for _ in range(2))
+    w = torch.randn(dim, generator=g, device=cuda).to(dtype)
+    results = []
+    for pos in (None, torch.arange(37, device=cuda), torch.full((37, 2), float("nan"), device=cuda)):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+        y, _ = NormRotate(leaves[0], None, leaves[1], None, pos, rotary_dim=0)
+        results.append((y, *torch.autograd.grad(y, leaves, grad)))
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0])) and results[0][0].isfinite().all()
