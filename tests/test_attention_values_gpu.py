@@ -234,3 +234,28 @@ def test_what_the_device_finds_wrong_is_raised_on_demand(cuda, dtype, monkeypatc
         held = CrossAttention(q, k, v, *good)
     graph.replay()
     assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize("dtype", ["float", "half", "bfloat"])
+@pytest.mark.parametrize("call", range(len(CALLS)))
+def test_gradients_of_what_is_no_number_are_none(cuda, dtype, call):
+    """A NaN in a query: its gradient, and those of all keys and values that it sees, and no others."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk, heads, kv_heads, dim = CALLS[call]
+    q, k, v, grad = inputs(nq, nk, heads, kv_heads, dim, dtype, cuda, seed=98)
+    mask = torch.rand(len(k), generator=torch.Generator(device=cuda).manual_seed(3), device=cuda) < 0.8
+    rs = splits(nq, cuda), splits(nk, cuda)
+
+    def run():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(CrossAttention(*leaves, *rs, key_mask=mask), leaves, grad)
+
+    clean = run()
+    q[0, 0, 0] = float("nan")
+    got = run()
+    seen = mask.clone()
+    seen[nk[0]:] = False
+    for g, before, rows in zip(got, clean, (torch.arange(len(q), device=cuda) == 0, seen, seen)):
+        gone = torch.zeros(g.shape, dtype=torch.bool, device=cuda)
+        gone[rows, 0] = True
+        assert torch.equal(g.isnan(), gone) and torch.equal(g[~gone], before[~gone])
