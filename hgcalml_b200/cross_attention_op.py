@@ -113,9 +113,10 @@ def CrossAttention(queries, keys, values, query_row_splits, key_row_splits, scal
     ``queries [N, heads, D]``, ``keys`` and ``values [M, key heads, D]`` of one type (float32, float16, bfloat16; D up to
     128), rows and heads at any distance; the heads are shared evenly among the key heads, head h reads key head
     ``h // (heads // key_heads)``.  ``query_row_splits`` and ``key_row_splits [E+1]``: the rows of every event, which may be
-    none, and which may end before the tensors do; they have to ascend from zero (HGC_CHECK_STATUS=1 in the environment checks
-    that).  ``scale`` is ``D ** -0.5`` unless given.  ``key_mask [M]`` (bool): keys
-    that no query may see are False, and what their rows hold does not matter.  A query that sees no key gets zeros.
+    none, and which may end before the tensors do; they ascend from zero (checked with HGC_CHECK_STATUS=1 in the
+    environment).  ``scale`` is ``D ** -0.5`` unless given.  ``key_mask [M]`` (bool): keys that no query may see are False, and
+    what their rows hold does not matter.  A query that sees no key gets zeros.  Rows that are seen are finite; a NaN among
+    them stays one in all that it is a term of.
 
     Returns the rows ``[N, heads, D]``, with ``with_lse`` also the float32 logarithm of every row's sum of
     exponentials ``[N, heads]`` (``-inf`` without keys), from which results over parts of the keys can be joined.

@@ -6,7 +6,8 @@
 //   dk_j = scale sum_i ds_ij q_i
 //
 // A row without keys has o = 0, and -inf for the logarithm of its sum.  Gradients of shared key heads are summed inside the
-// kernel and parts of a split are joined in their order: no atomics, so results do not change from run to run.
+// kernel and parts of a split are joined in their order, so results do not change from run to run (atomics take the largest of some
+// norms, and the next tile, whose order changes none).
 #include "cross_attention.cuh"
 #include "mma_device.cuh"
 

@@ -418,12 +418,18 @@ int hgc_push_knn_grad_ordered(
  *   d_out[i,h,:] = sum_j p_ij d_v[j,:],  p_ij = exp(scale q_i.k_j) / sum_j' exp(scale q_i.k_j')
  * over the keys j of i's event with d_key_mask[j] != 0 (d_key_mask may be NULL: all of them).  What stands in
  * masked rows of d_k and d_v does not matter, infinities and NaN included.  A query without keys, and a row behind
- * the last event, gets zeros.  d_lse[i,h] = log of the sum of exp(scale q_i.k_j), -infinity without keys.
+ * the last event, gets zeros, whatever it holds.  NaN in a row that is seen stays NaN in all that it is a term of; rows that
+ * are seen have to be finite otherwise (with an infinite one, what it is a term of may be NaN in one type or size and not in
+ * another).  d_lse[i,h] = log of the sum of exp(scale q_i.k_j), -infinity without keys.
  * d_q [n_q, n_heads, dim], d_k and d_v [n_k, n_kv_heads, dim], of the type `dtype`, with the distances in elements
  * of rows and heads in strides = {q row, q head, k row, k head, v row, v head} (host memory; NULL: dense); columns
  * lie next to each other.  d_out, d_lse (float32) and everything the gradient takes and gives besides are dense.
- * Sums, weights and gradients are held in float32; in 16 bits, weights are rounded once to the type of the values
- * they meet.  scale > 0.  Limits: dim <= 128, n_heads <= 65535, 2^31 - 8193 rows.
+ * Sums, weights and gradients are held in float32.  In 16 bits, weights and their gradients may be rounded to the type
+ * of the values they meet (not where queries are few, calls short, or the mean event of a gradient has up to 16 keys: which
+ * products a call takes goes by the batch, and a small event beside long ones takes theirs), and some of the weights
+ * are off by up to 1.0e-4, as d_lse may then be.  In half precision what is rounded away below its normal numbers is at
+ * most 2^-37 of the largest value for each key, in the gradient of queries 2^-38 |grad_i| max|v| for each key and in that of
+ * keys 2^-38 max|grad| max|v| for each query of the event.  scale > 0.  Limits: dim <= 128, n_heads <= 65535, 2^31 - 8193 rows.
  *
  * The gradient: d_grad_out [n_q, n_heads, dim] is that of d_out; d_out, d_out_rest and d_lse are the forward pass's, as
  * are all other arguments.  d_out_rest (like d_out, or NULL) is what the rounding of d_out to 16 bits left, rounded itself:
