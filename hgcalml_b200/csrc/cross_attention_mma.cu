@@ -480,7 +480,7 @@ forward_mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps 
                     // The sums are scaled again only where a row's maximum has grown by more than that.  The others of the warp stay as
                     // they are then, so that no result depends on which rows share a warp; and rows that do not count have no say: what
                     // stands there may differ from run to run.
-                    const bool grown = store && !((next - top) * c <= Weights<T>::kGrowth);  // or is no number
+                    const bool grown = store && ((next - top) * c > Weights<T>::kGrowth || next != next);
                     const float before = top;
                     if (count == 0 || grown) top = next;
                     if (count == 0) {
