@@ -259,3 +259,23 @@ def test_gradients_of_what_is_no_number_are_none(cuda, dtype, call):
         gone = torch.zeros(g.shape, dtype=torch.bool, device=cuda)
         gone[rows, 0] = True
         assert torch.equal(g.isnan(), gone) and torch.equal(g[~gone], before[~gone])
+
+
+@pytest.mark.parametrize("dtype", ["float", "half", "bfloat"])
+@pytest.mark.parametrize("call", range(len(CALLS)))
+def test_keys_that_are_masked_first_or_last(cuda, dtype, call):
+    """Whole steps and parts without a key that is seen, before the first one and behind the last, hold anything and change nothing."""
+    from hgcalml_b200.cross_attention_op import CrossAttention
+    nq, nk, heads, kv_heads, dim = CALLS[call]
+    q, k, v, grad = inputs(nq, nk, heads, kv_heads, dim, dtype, cuda, seed=99)
+    for event in (slice(0, nk[0]), slice(nk[0], nk[0] + nk[1])):
+        for hide in (slice(event.start, event.stop - 2), slice(event.start + 2, event.stop), slice(event.start, (event.start + event.stop) // 2)):
+            mask = torch.ones(len(k), dtype=torch.bool, device=cuda)
+            mask[hide] = False
+            want, _ = reference(q, k, v, nq, nk, dim ** -0.5, mask, grad)
+            bad = [t.masked_fill(~mask[:, None, None], float("nan")).requires_grad_(True) for t in (k, v)]
+            leaves = [q.detach().requires_grad_(True), *bad]
+            out = CrossAttention(*leaves, splits(nq, cuda), splits(nk, cuda), key_mask=mask)
+            assert_near(out.detach(), want["out"], "out")
+            for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, grad)):
+                assert_near(g, want[name], name)
