@@ -40,10 +40,15 @@ class RaggedCrossAttention(torch.nn.Module):
     @staticmethod
     def _seen(key_mask, context, key_positions):
         """Zeros where nobody looks: a gradient of zero does not make up for a row of NaN in the gradients of the transforms."""
-        if key_mask is None or not torch.is_grad_enabled() or key_mask.numel() != context.shape[0]:  # CrossAttention refuses the last
+        if key_mask is None or not torch.is_grad_enabled():
             return context, key_positions
-        key_mask = key_mask.reshape(-1) != 0
-        return [None if t is None else t.masked_fill(~key_mask.reshape(-1, *[1] * (t.dim() - 1)), 0) for t in (context, key_positions)]
+        hidden = key_mask.reshape(-1) == 0
+
+        def clear(t):  # the ops refuse what does not fit
+            fits = t is not None and t.dim() > 0 and t.shape[0] == hidden.shape[0] and t.device == hidden.device
+            return t.masked_fill(hidden.reshape(-1, *[1] * (t.dim() - 1)), 0) if fits else t
+
+        return clear(context), clear(key_positions)
 
     def _keys_values(self, context):
         both = self.context_transform(context).unflatten(-1, (2, self.n_key_heads, self.n_head_features))

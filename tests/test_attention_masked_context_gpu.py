@@ -45,11 +45,15 @@ def test_what_masked_rows_hold_does_not_matter(cuda, dtype, prepared, kind):
         assert torch.equal(layer([x, context, *rs], pq, clean_p, key_mask=mask), want[0])
 
 
-def test_a_mask_of_another_length_is_refused(cuda):
+def test_masks_and_positions_that_do_not_fit_are_refused(cuda):
     from hgcalml_b200 import _capi as C
     from hgcalml_b200.AttentionLayersRagged import RaggedCrossAttention
     layer = RaggedCrossAttention(2, 8, 4, n_in=5, n_context=6).to(cuda)
     x, context, rs = _rows(3, 5, cuda, 1, torch.float32), _rows(7, 6, cuda, 2, torch.float32), (_splits([3], cuda), _splits([7], cuda))
-    for n in (1, 6, 8):
+    mask = torch.ones(7, dtype=torch.bool, device=cuda)
+    for bad in (*(torch.ones(n, dtype=torch.bool, device=cuda) for n in (1, 6, 8)), mask.cpu(), mask.float()):
         with pytest.raises(C.HgcError, match="key_mask"):
-            layer([x, context, *rs], key_mask=torch.ones(n, dtype=torch.bool, device=cuda))
+            layer([x, context, *rs], key_mask=bad)
+    for bad in (torch.zeros(6, device=cuda), torch.zeros(7, 2, 1, device=cuda), torch.zeros(7), torch.zeros(7, device=cuda, requires_grad=True)):
+        with pytest.raises(C.HgcError, match="positions|CUDA"):
+            layer([x, context, *rs], None, bad, key_mask=mask)
